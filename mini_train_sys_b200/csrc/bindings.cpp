@@ -586,6 +586,7 @@ Tensor status_tensor(int64_t device) { return status_word(int(device)); }
 
 void bind_attention(pybind11::module_& m);
 void bind_comm(pybind11::module_& m);
+void bind_decode(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
@@ -628,4 +629,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("status_tensor", &status_tensor);
   bind_attention(m);
   bind_comm(m);
+  bind_decode(m);
 }

@@ -1,0 +1,75 @@
+// Launchers of the decoding-step kernels: the 8-bit key / value cache (append, read back, attention over it) and the
+// mixture-of-experts layer for a few tokens.  Raw pointers and a stream, as in ops.cuh.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace mts {
+
+// ---- the cache of one layer -----------------------------------------------------------------------------------------
+// Tokens of a (sequence, K/V head) are grouped in blocks of kCacheBlock.  A finished block is held in 8 bits, the unfinished
+// one in the activation type, so that a value is rounded to 8 bits once, whatever calls brought the tokens.
+//   codes [B, Hkv, blocks, 2, 64 * D] uint8: excess-128 codes, K as [token][dim], V as [dim][slot of the token]
+//   scale [B, Hkv, blocks, 2] fp32: value = (code - 128) * scale
+//   tail  [B, Hkv, 2, 2, 64 * D] activation type: block j is at index j & 1, laid out as the codes are
+// The slot of token 16 m + u of a V row is cache_slot(16 m + u): the four tokens that one lane of an m16n8k16 product needs per
+// step are adjacent, and the sixteen that it needs per block are one 16-byte load.
+constexpr int kCacheBlock = 64;
+__host__ __device__ constexpr int cache_slot(int token) {
+  return ((token & 7) >> 1) * 16 + (token >> 4) * 4 + ((token >> 3) & 1) * 2 + (token & 1);
+}
+
+struct CacheView {
+  uint8_t* codes;
+  float* scale;
+  void* tail;
+  const int* start;      // [B] tokens before this step
+  const int* count;      // [B] new tokens of this step
+  int B, Hkv, blocks, D;
+  bool fp16;             // activation type: fp16 or bf16
+};
+
+struct Strided {         // [B, heads, T, D] view with a unit inner stride
+  const void* p;
+  long long sb, sh, st;
+};
+
+// Appends token t < count[b] at position start[b] + t; keys and queries are rotated when `cosv` is given (tables [P, D]).
+// q_out: [B, Hq, T, D] over [B, T, Hq, D] storage; rows t >= count[b] are zeroed.  q.p may be null.
+cudaError_t launch_kv_append(const CacheView& c, const Strided& q, int Hq, const Strided& k, const Strided& v, void* q_out, const void* cosv,
+                             const void* sinv, int table_rows, int T, cudaStream_t stream);
+// k / v [B, Hkv, n, D] fp32: positions first[b] + i; zeros outside [0, start + count).
+cudaError_t launch_kv_read(const CacheView& c, const int* first, int n, float* k, float* v, cudaStream_t stream);
+
+struct CachedAttentionArgs {
+  CacheView cache;
+  Strided q;             // [B, Hq, T, D]
+  void* o;               // [B, T, Hq, D] storage
+  int Hq, T;
+  float scale;
+  float* workspace;      // cached_attention_workspace_floats(...) floats; may be null when that is 0
+  cudaStream_t stream;
+};
+size_t cached_attention_workspace_floats(int B, int Hkv, int Hq, int T, int D, int blocks);
+cudaError_t launch_cached_attention(const CachedAttentionArgs& a);
+
+// ---- mixture of experts for a few tokens ----------------------------------------------------------------------------
+constexpr int kMoeTokensMax = 64;
+struct MoeTokensArgs {
+  const void* x;         // [T, H] bf16, row stride ldx
+  long long ldx;
+  const void* router;    // [E, H] fp32 or bf16
+  bool router_bf16;
+  const void* gate_up;   // [E, 2 I, H] bf16
+  const void* down;      // [E, H, I] bf16
+  void* y;               // [T, H] bf16, contiguous
+  void* hidden;          // workspace: [2, T * K, I] bf16
+  int* routes;           // workspace: [T * K] expert of every route
+  int T, E, K, H, I;
+  bool normalize;
+  cudaStream_t stream;
+};
+cudaError_t launch_moe_tokens(const MoeTokensArgs& a);
+
+}  // namespace mts

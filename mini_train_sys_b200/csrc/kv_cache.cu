@@ -1,0 +1,319 @@
+// Appending to the 8-bit key / value cache, and reading it back (layout: decode.cuh).
+//
+//   a = max |x| over the 64 x D values of a finished block,  scale = a / 127,  code = rint(127 x / a)  (half to even)
+//
+// For 16-bit x the product 127 x is exact in fp32 and 127 x / a is either a half exactly or at least 2^-12 away from one, so
+// a correctly rounded quotient gives the code that exact arithmetic gives.
+#include "decode.cuh"
+#include "ops.cuh"
+#include "mma_sync.cuh"
+
+#include <math_constants.h>
+
+namespace mts {
+
+namespace {
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T> union Vec8T { uint4 q; T v[8]; };
+
+// x c -+ y s as the rotary kernel computes it: the products of 16-bit factors are exact in fp32, their sum is rounded there and
+// then to T.
+template <typename T>
+__device__ __forceinline__ T rotate_one(T x, T c, T y, T s, bool minus) {
+  const float p = __fmul_rn(to_f(x), to_f(c)), q = __fmul_rn(to_f(y), to_f(s));
+  return from_f<T>(minus ? __fsub_rn(p, q) : __fadd_rn(p, q));
+}
+
+template <typename T>
+__device__ __forceinline__ void rotate8(Vec8T<T>& lo, Vec8T<T>& hi, const T* c, const T* s) {
+  Vec8T<T> cv, sv;
+  cv.q = *reinterpret_cast<const uint4*>(c);
+  sv.q = *reinterpret_cast<const uint4*>(s);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const T a = lo.v[j], b = hi.v[j];
+    lo.v[j] = rotate_one(a, cv.v[j], b, sv.v[j], true);
+    hi.v[j] = rotate_one(b, cv.v[j], a, sv.v[j], false);
+  }
+}
+
+// 127 x / a to the nearest integer: the product with 127 / a decides except within 0.001 of a half, where the quotient does.
+__device__ __forceinline__ uint32_t code_of(float x, float amax, float inv) {
+  const float y = x * inv;
+  float r = rintf(y);
+  if (!(fabsf(y - r) < 0.499f) || amax < 1e-30f) {
+    const float down = amax > 1e30f ? 0x1p-10f : 1.f;      // 127 x must not overflow; scaling by a power of two is exact
+    r = rintf(__fdiv_rn(x * down * 127.f, amax * down));
+  }
+  return uint32_t(int(r) + 128) & 0xFFu;
+}
+
+constexpr int kAppendThreads = 256;
+
+// One CTA per (block that the step touches, K/V head, sequence); the CTAs behind those rotate q.
+// A thread owns eight dims of the lower half of a head and their partners in the upper half, for one token.
+template <typename T, int D>
+__global__ void __launch_bounds__(kAppendThreads)
+kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __restrict__ q_out, const T* __restrict__ cosv,
+                 const T* __restrict__ sinv, int table_rows, int Tn, int kv_ctas, int blocks_per_head) {
+  constexpr int VEC = D / 16;                              // threads per token
+  constexpr int ITER = (kCacheBlock * VEC + kAppendThreads - 1) / kAppendThreads;
+  constexpr int BLK = kCacheBlock;
+  const int tid = threadIdx.x;
+  if (int(blockIdx.x) >= kv_ctas) {                        // ---- q ----
+    const long long total = (long long)c.B * Hq * Tn * VEC;
+    for (long long i = (long long)(blockIdx.x - kv_ctas) * kAppendThreads + tid; i < total;
+         i += (long long)(gridDim.x - kv_ctas) * kAppendThreads) {
+      const int vec = int(i % VEC);
+      long long r = i / VEC;
+      const int h = int(r % Hq); r /= Hq;
+      const int t = int(r % Tn);
+      const int b = int(r / Tn);
+      T* dst = q_out + (((long long)b * Tn + t) * Hq + h) * D + vec * 8;
+      Vec8T<T> lo, hi;
+      lo.q = hi.q = make_uint4(0, 0, 0, 0);
+      const int p = c.start[b] + t;
+      if (t < c.count[b] && p >= 0 && p < c.blocks * BLK) {
+        const T* src = static_cast<const T*>(q.p) + b * q.sb + h * q.sh + t * q.st + vec * 8;
+        lo.q = *reinterpret_cast<const uint4*>(src);
+        hi.q = *reinterpret_cast<const uint4*>(src + D / 2);
+        if (cosv != nullptr && p < table_rows) rotate8(lo, hi, cosv + (long long)p * D + vec * 8, sinv + (long long)p * D + vec * 8);
+      }
+      *reinterpret_cast<uint4*>(dst) = lo.q;
+      *reinterpret_cast<uint4*>(dst + D / 2) = hi.q;
+    }
+    return;
+  }
+
+  __shared__ unsigned amax_sm[2][kAppendThreads / 32];
+  __shared__ __align__(16) uint8_t v_sm[D * BLK];
+  const int item = int(blockIdx.x) % blocks_per_head;
+  const int bh = int(blockIdx.x) / blocks_per_head;
+  const int h = bh % c.Hkv, b = bh / c.Hkv;
+  const int limit = c.blocks * BLK;
+  const int start = min(max(c.start[b], 0), limit);
+  const int end = min(start + min(max(c.count[b], 0), Tn), limit);
+  if (end <= start) return;
+  const int first_block = start / BLK, last_block = (end - 1) / BLK;
+  const int block = first_block + item;
+  if (block > last_block) return;
+  // The first block takes its older tokens from the tail, and a last, unfinished block may go to the same half of it: then this
+  // CTA writes that block too, after it has read.
+  const bool last_open = (end % BLK) != 0;
+  const bool shared_half = last_open && last_block > first_block && ((last_block - first_block) & 1) == 0 && (start % BLK) != 0;
+  if (shared_half && item > 0 && block == last_block) return;
+
+  const T* kb = static_cast<const T*>(k.p) + b * k.sb + h * k.sh;
+  const T* vb = static_cast<const T*>(v.p) + b * v.sb + h * v.sh;
+  T* tail = static_cast<T*>(c.tail) + (long long)bh * 4 * BLK * D;
+  for (int pass = 0; pass < (shared_half && item == 0 ? 2 : 1); ++pass) {
+    const int blk = pass == 0 ? block : last_block;
+    const int base = blk * BLK;
+    T* tk = tail + (blk & 1) * 2 * BLK * D;
+    T* tv = tk + BLK * D;
+    const bool closes = end >= base + BLK;
+    if (pass == 1) __syncthreads();
+    Vec8T<T> klo[ITER], khi[ITER], vlo[ITER], vhi[ITER];
+#pragma unroll
+    for (int it = 0; it < ITER; ++it) {
+      const int idx = it * kAppendThreads + tid;
+      const int tok = idx / VEC, vec = idx % VEC;
+      const int p = base + tok;
+      klo[it].q = khi[it].q = vlo[it].q = vhi[it].q = make_uint4(0, 0, 0, 0);
+      if (tok >= BLK) continue;
+      if (p >= start && p < end) {
+        const T* ks = kb + (p - start) * k.st + vec * 8;
+        const T* vs = vb + (p - start) * v.st + vec * 8;
+        klo[it].q = *reinterpret_cast<const uint4*>(ks);
+        khi[it].q = *reinterpret_cast<const uint4*>(ks + D / 2);
+        vlo[it].q = *reinterpret_cast<const uint4*>(vs);
+        vhi[it].q = *reinterpret_cast<const uint4*>(vs + D / 2);
+        if (cosv != nullptr && p < table_rows)
+          rotate8(klo[it], khi[it], cosv + (long long)p * D + vec * 8, sinv + (long long)p * D + vec * 8);
+      } else if (closes && p < start) {
+        klo[it].q = *reinterpret_cast<const uint4*>(tk + tok * D + vec * 8);
+        khi[it].q = *reinterpret_cast<const uint4*>(tk + tok * D + D / 2 + vec * 8);
+        const int slot = cache_slot(tok);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          vlo[it].v[j] = tv[(vec * 8 + j) * BLK + slot];
+          vhi[it].v[j] = tv[(D / 2 + vec * 8 + j) * BLK + slot];
+        }
+      }
+    }
+    if (!closes) {                                         // the block stays open: the new tokens go to the tail
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        const int idx = it * kAppendThreads + tid;
+        const int tok = idx / VEC, vec = idx % VEC;
+        const int p = base + tok;
+        if (tok >= BLK || p < start || p >= end) continue;
+        *reinterpret_cast<uint4*>(tk + tok * D + vec * 8) = klo[it].q;
+        *reinterpret_cast<uint4*>(tk + tok * D + D / 2 + vec * 8) = khi[it].q;
+        const int slot = cache_slot(tok);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          tv[(vec * 8 + j) * BLK + slot] = vlo[it].v[j];
+          tv[(D / 2 + vec * 8 + j) * BLK + slot] = vhi[it].v[j];
+        }
+      }
+      continue;
+    }
+    // largest magnitude as an integer: the order of the bits is the order of the values, and a NaN is above infinity
+    unsigned ka = 0, va = 0;
+#pragma unroll
+    for (int it = 0; it < ITER; ++it)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ka = max(ka, max(__float_as_uint(fabsf(to_f(klo[it].v[j]))), __float_as_uint(fabsf(to_f(khi[it].v[j])))));
+        va = max(va, max(__float_as_uint(fabsf(to_f(vlo[it].v[j]))), __float_as_uint(fabsf(to_f(vhi[it].v[j])))));
+      }
+    ka = __reduce_max_sync(0xffffffffu, ka);
+    va = __reduce_max_sync(0xffffffffu, va);
+    if ((tid & 31) == 0) { amax_sm[0][tid >> 5] = ka; amax_sm[1][tid >> 5] = va; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) { ka = max(ka, amax_sm[0][w]); va = max(va, amax_sm[1][w]); }
+    const bool k_ok = ka < 0x7f800000u, v_ok = va < 0x7f800000u;
+    const float kamax = __uint_as_float(ka), vamax = __uint_as_float(va);
+    const float kinv = k_ok && ka != 0 ? __fdiv_rn(127.f, kamax) : 0.f, vinv = v_ok && va != 0 ? __fdiv_rn(127.f, vamax) : 0.f;
+    uint8_t* kc = c.codes + (((long long)bh * c.blocks + blk) * 2) * BLK * D;
+    uint8_t* vc = kc + BLK * D;
+    if (tid == 0) {
+      float* sc = c.scale + ((long long)bh * c.blocks + blk) * 2;
+      sc[0] = k_ok ? __fdiv_rn(kamax, 127.f) : CUDART_NAN_F;     // a block that holds a NaN or an infinity reads NaN
+      sc[1] = v_ok ? __fdiv_rn(vamax, 127.f) : CUDART_NAN_F;
+    }
+#pragma unroll
+    for (int it = 0; it < ITER; ++it) {
+      const int idx = it * kAppendThreads + tid;
+      const int tok = idx / VEC, vec = idx % VEC;
+      if (tok >= BLK) continue;
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = kinv > 0.f ? code_of(to_f(klo[it].v[j]), kamax, kinv) : 128u;
+        const uint32_t d = kinv > 0.f ? code_of(to_f(khi[it].v[j]), kamax, kinv) : 128u;
+        w[j >> 2] |= a << (8 * (j & 3));
+        w[2 + (j >> 2)] |= d << (8 * (j & 3));
+      }
+      *reinterpret_cast<uint2*>(kc + tok * D + vec * 8) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(kc + tok * D + D / 2 + vec * 8) = make_uint2(w[2], w[3]);
+      const int slot = cache_slot(tok);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v_sm[(vec * 8 + j) * BLK + slot] = uint8_t(vinv > 0.f ? code_of(to_f(vlo[it].v[j]), vamax, vinv) : 128u);
+        v_sm[(D / 2 + vec * 8 + j) * BLK + slot] = uint8_t(vinv > 0.f ? code_of(to_f(vhi[it].v[j]), vamax, vinv) : 128u);
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < D * BLK / 16; i += kAppendThreads)
+      reinterpret_cast<uint4*>(vc)[i] = reinterpret_cast<const uint4*>(v_sm)[i];
+  }
+}
+
+// One CTA per 64 positions of a (sequence, K/V head); consecutive threads take consecutive positions, so that the bytes of one
+// V row are read together.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restrict__ ko, float* __restrict__ vo, int chunks) {
+  constexpr int BLK = kCacheBlock;
+  const int chunk = int(blockIdx.x) % chunks;
+  const int bh = int(blockIdx.x) / chunks;
+  const int b = bh / c.Hkv;
+  const int total = min(min(max(c.start[b], 0), c.blocks * BLK) + max(c.count[b], 0), c.blocks * BLK);
+  const int tok = threadIdx.x & 63;
+  const int i = chunk * 64 + tok;
+  if (i >= n) return;
+  const long long p = (long long)first[b] + i;
+  const bool live = p >= 0 && p < total;
+  const int blk = live ? int(p / BLK) : 0, at = live ? int(p % BLK) : 0;
+  const bool open = blk == total / BLK;
+  const uint8_t* kc = c.codes + (((long long)bh * c.blocks + blk) * 2) * BLK * D;
+  const T* tk = static_cast<const T*>(c.tail) + ((long long)bh * 2 + (blk & 1)) * 2 * BLK * D;
+  float ks = 0.f, vs = 0.f;
+  if (live && !open) {
+    const float* sc = c.scale + ((long long)bh * c.blocks + blk) * 2;
+    ks = sc[0];
+    vs = sc[1];
+  }
+  const int slot = cache_slot(at);
+  float* kd = ko + ((long long)bh * n + i) * D;
+  float* vd = vo + ((long long)bh * n + i) * D;
+  for (int d = (threadIdx.x >> 6) * 8; d < D; d += 32) {
+    float kf[8], vf[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) kf[j] = vf[j] = 0.f;
+    if (live && open) {
+      Vec8T<T> x;
+      x.q = *reinterpret_cast<const uint4*>(tk + at * D + d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { kf[j] = to_f(x.v[j]); vf[j] = to_f(tk[BLK * D + (d + j) * BLK + slot]); }
+    } else if (live) {
+      const uint2 w = *reinterpret_cast<const uint2*>(kc + at * D + d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        kf[j] = float(int(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xFFu) - 128) * ks;
+        vf[j] = float(int(kc[BLK * D + (d + j) * BLK + slot]) - 128) * vs;
+      }
+    }
+    *reinterpret_cast<float4*>(kd + d) = make_float4(kf[0], kf[1], kf[2], kf[3]);
+    *reinterpret_cast<float4*>(kd + d + 4) = make_float4(kf[4], kf[5], kf[6], kf[7]);
+    *reinterpret_cast<float4*>(vd + d) = make_float4(vf[0], vf[1], vf[2], vf[3]);
+    *reinterpret_cast<float4*>(vd + d + 4) = make_float4(vf[4], vf[5], vf[6], vf[7]);
+  }
+}
+
+template <typename T, int D>
+cudaError_t append_typed(const CacheView& c, const Strided& q, int Hq, const Strided& k, const Strided& v, void* q_out, const void* cosv,
+                         const void* sinv, int table_rows, int Tn, cudaStream_t stream) {
+  const int per_head = (Tn + kCacheBlock - 2) / kCacheBlock + 1;       // blocks that T tokens can touch
+  const long long kv_ctas = (long long)c.B * c.Hkv * per_head;
+  const long long q_threads = q.p == nullptr ? 0 : (long long)c.B * Hq * Tn * (D / 16);
+  const long long q_want = (q_threads + kAppendThreads - 1) / kAppendThreads, q_cap = (long long)device_sm_count() * 16;
+  const long long q_ctas = q_want < q_cap ? q_want : q_cap;
+  if (kv_ctas + q_ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  kv_append_kernel<T, D><<<unsigned(kv_ctas + q_ctas), kAppendThreads, 0, stream>>>(
+      c, q, Hq, k, v, static_cast<T*>(q_out), static_cast<const T*>(cosv), static_cast<const T*>(sinv), table_rows, Tn, int(kv_ctas), per_head);
+  ++g_launch_count;
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t read_typed(const CacheView& c, const int* first, int n, float* k, float* v, cudaStream_t stream) {
+  const int chunks = (n + 63) / 64;
+  const long long ctas = (long long)c.B * c.Hkv * chunks;
+  if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  kv_read_kernel<T, D><<<unsigned(ctas), 256, 0, stream>>>(c, first, n, k, v, chunks);
+  ++g_launch_count;
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const CacheView& c, const Strided& q, int Hq, const Strided& k, const Strided& v, void* q_out, const void* cosv,
+                             const void* sinv, int table_rows, int T, cudaStream_t stream) {
+  if (c.D == 32) return c.fp16 ? append_typed<__half, 32>(c, q, Hq, k, v, q_out, cosv, sinv, table_rows, T, stream)
+                               : append_typed<__nv_bfloat16, 32>(c, q, Hq, k, v, q_out, cosv, sinv, table_rows, T, stream);
+  if (c.D == 64) return c.fp16 ? append_typed<__half, 64>(c, q, Hq, k, v, q_out, cosv, sinv, table_rows, T, stream)
+                               : append_typed<__nv_bfloat16, 64>(c, q, Hq, k, v, q_out, cosv, sinv, table_rows, T, stream);
+  if (c.D == 128) return c.fp16 ? append_typed<__half, 128>(c, q, Hq, k, v, q_out, cosv, sinv, table_rows, T, stream)
+                                : append_typed<__nv_bfloat16, 128>(c, q, Hq, k, v, q_out, cosv, sinv, table_rows, T, stream);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_kv_read(const CacheView& c, const int* first, int n, float* k, float* v, cudaStream_t stream) {
+  if (c.D == 32) return c.fp16 ? read_typed<__half, 32>(c, first, n, k, v, stream) : read_typed<__nv_bfloat16, 32>(c, first, n, k, v, stream);
+  if (c.D == 64) return c.fp16 ? read_typed<__half, 64>(c, first, n, k, v, stream) : read_typed<__nv_bfloat16, 64>(c, first, n, k, v, stream);
+  if (c.D == 128) return c.fp16 ? read_typed<__half, 128>(c, first, n, k, v, stream) : read_typed<__nv_bfloat16, 128>(c, first, n, k, v, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace mts

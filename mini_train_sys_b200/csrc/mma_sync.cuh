@@ -1,0 +1,48 @@
+// Warp-level matrix products and fragment helpers shared by the decoding kernels.  These kernels are bound by reading
+// 8-bit keys or expert weights once; eight query rows or tokens ride on every weight, far below what one 128-row tcgen05 tile
+// would need to be worth its shared-memory staging, so fragments are loaded straight from global memory into registers.
+//
+// m16n8k16, lane = 4 g + c:  A: a0 (row g, k 2c..), a1 (row g + 8, k 2c..), a2 (row g, k 2c + 8..), a3 (row g + 8, k 2c + 8..)
+//                            B: b0 (k 2c.., column g), b1 (k 2c + 8.., column g);  C: c0 c1 (row g, columns 2c 2c+1), c2 c3 (row g + 8)
+// The order of k is free as long as A and B agree, which is what lets a lane take 8 or 16 adjacent elements per load.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace mts {
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transpose of an 8 x 8 matrix of 16-bit values held as fragments (row = lane / 4, columns 2c, 2c + 1).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf162(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four excess-128 codes to two pairs of fp16 integers: a byte under the exponent of 1024 reads 1024 + code, and the subtraction
+// of 1152 is exact.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+  const uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&l), bias), b = __hsub2(*reinterpret_cast<const __half2*>(&h), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+}  // namespace mts

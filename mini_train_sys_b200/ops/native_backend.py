@@ -23,8 +23,9 @@ from collections import Counter
 import torch
 
 from mini_train_sys_b200.models.ops import RouterPostprocessOutput
+from mini_train_sys_b200.ops import kv_cache
 from mini_train_sys_b200.ops.build import load_extension
-from mini_train_sys_b200.ops.torch_backend import TorchOpsBackend, check_router_args
+from mini_train_sys_b200.ops.torch_backend import TorchOpsBackend, check_moe_tokens, check_router_args
 
 GEMM_DENSE, GEMM_GROUPED_M, GEMM_GROUPED_K = 0, 1, 2
 EPI_STORE, EPI_SWIGLU, EPI_SWIGLU_BWD = 0, 1, 2
@@ -903,6 +904,53 @@ class NativeOpsBackend(TorchOpsBackend):
         if self._count("attention", native_attention.supported(q, k, v, is_causal=is_causal, dropout_p=dropout_p)):
             return native_attention.flash_attention(q, k, v, is_causal=is_causal, dropout_p=dropout_p)
         return super().attention(q, k, v, is_causal=is_causal, dropout_p=dropout_p)
+
+    # -- decoding step ------------------------------------------------------------------------
+    def _cache_ok(self, cache, *rows) -> bool:
+        return (cache.codes.is_cuda and cache.dtype in (torch.bfloat16, torch.float16) and cache.head_dim in kv_cache.HEAD_DIMS
+                and all(_rows16(t) for t in rows))
+
+    def kv_append(self, cache, layer, k, v, *, q=None, cos=None, sin=None):
+        kv_cache.check_append(cache, k, v, q, cos, sin)
+        ok = self._cache_ok(cache, k, v, *(() if q is None else (q,)))
+        ok = ok and (cos is None or (cos.is_contiguous() and sin.is_contiguous()))
+        if self._count("kv_append", ok):
+            return ext().kv_append(*cache.layer(layer), k, v, q, cos, sin)
+        return super().kv_append(cache, layer, k, v, q=q, cos=cos, sin=sin)
+
+    def kv_read(self, cache, layer, first, n):
+        kv_cache.check_read(cache, first, n)
+        if self._count("kv_read", self._cache_ok(cache) and first.is_contiguous()):
+            return tuple(ext().kv_read(*cache.layer(layer), first, n))
+        return super().kv_read(cache, layer, first, n)
+
+    def cached_attention(self, q, cache, layer):
+        kv_cache.check_attention(cache, q)
+        if self._count("cached_attention", self._cache_ok(cache, q)):
+            return ext().cached_attention(*cache.layer(layer), q, scaled_dot_scale(cache.head_dim))
+        return super().cached_attention(q, cache, layer)
+
+    def moe_tokens(self, x, router_weight, gate_up_proj, down_proj, top_k, *, normalize):
+        check_moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k)
+        n_exp, hidden, inter = down_proj.shape
+        weights = (router_weight, gate_up_proj, down_proj)
+        ok = (x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] <= MOE_TOKENS_MAX and hidden % 8 == 0 and inter % 8 == 0
+              and n_exp <= 64 and top_k <= 8 and x.stride(1) == 1 and x.data_ptr() % 16 == 0
+              and (x.shape[0] <= 1 or x.stride(0) % 8 == 0)
+              and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in weights)
+              and all(w.is_contiguous() and w.data_ptr() % 16 == 0 for w in weights))
+        if self._count("moe_tokens", ok):
+            return ext().moe_tokens(x, router_weight.detach(), bf16_weight(gate_up_proj), bf16_weight(down_proj), top_k, bool(normalize))
+        return super().moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k, normalize=normalize)
+
+
+MOE_TOKENS_MAX = 64     # of the few-token MoE kernels
+
+
+def _rows16(t: torch.Tensor) -> bool:
+    """``[B, heads, T, D]`` whose rows the kernels can read in 16-byte pieces."""
+
+    return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], t.stride()[:3]))
 
 
 def scaled_dot_scale(head_dim: int) -> float:
