@@ -3,10 +3,15 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(q . k_j / sqrt(D) - max),  j <= position of the query
 //
 // One pass over the cache with a running maximum and sum.  Keys and values are read once per tile of query rows (the heads that
-// share a K/V head, times the new tokens of the step) and go from global memory straight into matrix fragments: a lane's 16
-// bytes are the K or V fragment of several steps (the V rows are stored in that order), 4 bytes become two fp16 pairs in four
-// instructions, and both products run on m16n8k16 with the tokens (K) or the head's dims (V) as rows and eight query rows as
-// columns.  What bounds it: reading the codes, 2 D bytes per token and K/V head.
+// share a K/V head, times the new tokens of the step).  Every warp has a ring of blocks of its own in shared memory, which bulk
+// copies fill (one for the keys of a block with its scales, one for its values), so the warps run without barriers and each
+// keeps 8 to 16 KB of the cache in flight.  A lane's 16 adjacent bytes are its K or V fragment of several steps (the V rows are
+// stored in that order); 4 bytes become two fp16 pairs in four instructions; both products run on m16n8k16 with the tokens (K) or
+// the head's dims (V) as rows and eight query rows as columns.  The (sequence, head, row tile, block) units of
+// the whole batch are one list, cut into equal parts for the warps that fit on the machine: sequences of unlike lengths, and a
+// single long one, keep every SM busy, and a warp streams across the ends of sequences.  A second kernel joins the parts of
+// the (sequence, head, row tile) items that were cut.
+// What bounds it: reading the codes, 2 D bytes per token and K/V head.
 //
 // Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
 // queries keep their eight bits in fp16.  Probabilities are rounded to fp16 (2^-11 of each, at a scale of 2^14 so that the
@@ -15,6 +20,7 @@
 #include "decode.cuh"
 #include "ops.cuh"
 #include "mma_sync.cuh"
+#include "ptx_sm100.cuh"
 
 #include <math_constants.h>
 
@@ -24,22 +30,99 @@ namespace {
 
 constexpr int BLK = kCacheBlock;
 constexpr int kWarps = 4;
+// Resident CTAs an SM: three rings of 64 KB fit; more than eight query rows need the registers of the third.
+__host__ __device__ constexpr int ctas_per_sm(int nq) { return nq == 1 ? 3 : 2; }
+constexpr int kBatchMax = 2048;          // sequences: their units are counted in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kProbShift = 14.f;       // probabilities are held times 2^14
 
 struct Params {
-  const uint8_t* codes;
-  const float* scale;
+  const uint8_t* records;
   const void* tail;
   const int* start;
   const int* count;
-  int Hkv, blocks, Hq, T, group, row_tiles, splits;
+  int B, Hkv, blocks, Hq, T, group, row_tiles;
   const void* q;
   long long sb, sh, st;
   void* o;
-  float* part;                           // [item][split][rows][D + 2]
+  float* part;                           // [2 * warps][rows of a tile][D + 2]: parts of items that were cut
+  int ctas;
   float sm_log2;                         // log2(e) / sqrt(D)
+  int* status;
 };
+
+// Tokens of sequence b: before the step, and of it.
+__device__ __forceinline__ int2 span_of(const Params& p, int b) {
+  const int capacity = p.blocks * BLK;
+  const int start = min(max(__ldg(p.start + b), 0), capacity);
+  return make_int2(start, min(min(max(__ldg(p.count + b), 0), p.T), capacity - start));
+}
+// Units of a (head, row tile) of it: the finished blocks, and the unfinished one in halves of 32 tokens, which are as many bytes.
+__device__ __forceinline__ int units_of(int2 span) {
+  const int total = span.x + span.y, rest = total % BLK;
+  return span.y > 0 ? total / BLK + (rest > 0) + (rest > BLK / 2) : 0;
+}
+
+// prefix[b] = units of the sequences before b; every thread of the CTA takes part.
+template <int THREADS>
+__device__ __forceinline__ void count_units(const Params& p, int* prefix, int* scratch) {
+  const int heads = p.Hkv * p.row_tiles, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) prefix[0] = 0;
+  int carry = 0;
+  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+    const int b = b0 + threadIdx.x;
+    int v = b < p.B ? units_of(span_of(p, b)) * heads : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, off);
+      if (lane >= off) v += u;
+    }
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    int before = carry;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += scratch[w];
+      carry += scratch[w];
+    }
+    if (b < p.B) prefix[b + 1] = before + v;
+    __syncthreads();
+  }
+}
+
+// The list of N units in equal parts: part i of n begins at unit cut(N, i, n), and unit u is in part owner(N, u, n).
+__device__ __forceinline__ int cut(int N, int i, int n) { return int((long long)N * i / n); }
+__device__ __forceinline__ int owner(int N, int u, int n) { return int(((long long)(u + 1) * n - 1) / N); }
+
+// A stage of a warp's ring: the head of a record (its scales), keys, values, and the query rows of an item that begins.  The codes are
+// 16 KB a warp at any head dimension.
+__host__ __device__ constexpr int ring_stages(int D) { return 128 / D; }
+__host__ __device__ constexpr int stage_bytes(int D, int NQ) { return record_bytes(D) + 8 * NQ * D * 2; }
+__host__ __device__ constexpr int shared_bytes(int D, int NQ) {
+  const int ring = kWarps * ring_stages(D) * stage_bytes(D, NQ), exchange = kWarps * D * (8 * NQ + 1) * 4;
+  return ring > exchange ? ring : exchange;
+}
+
+// `bytes` (a multiple of 16, like both addresses) from global to shared memory; completion is counted on the barrier.
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// WORDS words (4 or 8 of them 16 bytes at a time) at p in shared memory.
+template <int WORDS>
+__device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + i * 16);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
+}
 
 template <typename T> struct Act;
 template <> struct Act<__nv_bfloat16> {
@@ -47,6 +130,10 @@ template <> struct Act<__nv_bfloat16> {
   static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
   static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t from_half2(uint32_t w) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pack_bf162(v.x, v.y);
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     mma_bf16(d, a[0], a[1], a[2], a[3], b0, b1);
   }
@@ -56,25 +143,11 @@ template <> struct Act<__half> {
   static __device__ __forceinline__ float lo(uint32_t w) { return __low2float(*reinterpret_cast<const __half2*>(&w)); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __high2float(*reinterpret_cast<const __half2*>(&w)); }
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t from_half2(uint32_t w) { return w; }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     mma_f16(d, a[0], a[1], a[2], a[3], b0, b1);
   }
 };
-
-// N bytes (8, 16 or 32) into N / 4 words; cache lines of the codes are read once, so they do not stay in L1.
-template <int WORDS>
-__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[WORDS]) {
-  if constexpr (WORDS == 2) {
-    const uint2 v = __ldg(static_cast<const uint2*>(p));
-    w[0] = v.x; w[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < WORDS / 4; ++i) {
-      const uint4 v = __ldg(static_cast<const uint4*>(p) + i);
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  }
-}
 
 // Running statistics and output of 8 * NQ query rows in one warp.  A lane holds the columns 2c and 2c + 1 of every tile of
 // eight rows (the statistics are the same in the eight lanes that share c) and the dims g and g + 8 of every 16.
@@ -83,10 +156,10 @@ struct State {
   float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];
 };
 
-// Scores of one block (log2 domain, -inf where masked) -> probabilities as fragments; rescales the state.
+// Scores of 16 M tokens (log2 domain, -inf where masked) -> probabilities as fragments; rescales the state.
 // s[m][n][i]: token 16 m + g + 8 (i >> 1), query 2c + (i & 1) of tile n.
-template <int D, int NQ>
-__device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[4][NQ][4]) {
+template <int D, int NQ, int M>
+__device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[M][NQ][4]) {
   bool moved = false;
   float alpha[NQ][2];
 #pragma unroll
@@ -95,7 +168,7 @@ __device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[4][NQ][4
     for (int j = 0; j < 2; ++j) {
       float mx = -CUDART_INF_F;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) mx = fmaxf(mx, fmaxf(s[m][n][j], s[m][n][j + 2]));
+      for (int m = 0; m < M; ++m) mx = fmaxf(mx, fmaxf(s[m][n][j], s[m][n][j + 2]));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
       mx = fmaxf(mx, st.m[n][j]);
@@ -106,7 +179,7 @@ __device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[4][NQ][4
       const float shift = base - kProbShift;
       float sum = 0.f;
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int m = 0; m < M; ++m)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           s[m][n][j + 2 * i] = exp2f(s[m][n][j + 2 * i] - shift);
@@ -124,250 +197,393 @@ __device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[4][NQ][4
   }
 }
 
+// True when the copies of a stage have come, false when they have not within the limit.
+__device__ __forceinline__ bool wait_copy(uint64_t* bar, uint32_t parity) {
+  if (mbar_test(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_test(bar, parity))
+    if (global_timer_ns() - t0 > kWaitDeadlineNs) return false;
+  return true;
+}
+
+// Where a warp is in the list of units: number `at` of the `units` of row tile `tile` of head h of sequence b, whose first
+// `closed` are finished blocks.
+struct Cursor {
+  int b, h, tile, at, units, closed;
+  __device__ __forceinline__ void enter(const Params& p, int seq) {
+    b = seq;
+    const int2 s = span_of(p, b);
+    units = units_of(s);
+    closed = (s.x + s.y) / BLK;
+  }
+  __device__ __forceinline__ void seek(const Params& p, const int* prefix, int u) {
+    int lo = 0, hi = p.B - 1;            // the last sequence whose units begin at or before u (one with none ends where it begins)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    enter(p, lo);
+    const int rest = u - prefix[lo];
+    at = rest % units;
+    tile = rest / units % p.row_tiles;
+    h = rest / units / p.row_tiles;
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    if (++at < units) return;
+    at = 0;
+    if (++tile < p.row_tiles) return;
+    tile = 0;
+    if (++h < p.Hkv) return;
+    h = 0;
+    units = 0;
+    for (int seq = b + 1; seq < p.B && units == 0; ++seq) enter(p, seq);
+  }
+};
+
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NQ))
 cached_attention_kernel(const Params p) {
   constexpr int KW = D / 16;             // K words per lane and token = steps of 16 dims
   constexpr int DT = D / 16;             // tiles of 16 dims of the output
   constexpr int ROWS = 8 * NQ;
   constexpr int OP = ROWS + 1;           // pitch of the output exchange
+  constexpr int STAGES = ring_stages(D);
+  constexpr int STAGE = stage_bytes(D, NQ), KEYS = kCacheHead, VALUES = KEYS + BLK * D, QUERIES = VALUES + BLK * D;
+  constexpr int KB = D / 4;              // bytes of a key that a lane owns
+  extern __shared__ __align__(16) uint8_t smem[];          // rings (afterwards the exchange of the outputs), prefix
   __shared__ float ml_sm[kWarps][ROWS][2];
-  __shared__ float o_sm[kWarps][D * OP];
+  __shared__ int scratch[kWarps];
+  __shared__ uint64_t bars[kWarps][STAGES][2];             // keys, values of a stage
+  int* prefix = reinterpret_cast<int*>(smem + shared_bytes(D, NQ));
+  float* o_sm = reinterpret_cast<float*>(smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int split = blockIdx.x, item = blockIdx.y + blockIdx.z * gridDim.y;
-  const int tile = item % p.row_tiles, bh = item / p.row_tiles;
-  const int h = bh % p.Hkv, b = bh / p.Hkv;
-  const int rows = p.group * p.T, row0 = tile * ROWS;
-  const int capacity = p.blocks * BLK;
-  const int start = min(max(p.start[b], 0), capacity);
-  const int total = min(start + min(max(p.count[b], 0), p.T), capacity);
-  const int fresh = total - start;       // rows of tokens t >= fresh are padding
-  const int t_last = min(min(row0 + ROWS, rows) - 1, fresh * p.group - 1) / p.group;
-  const bool live = row0 < fresh * p.group;
-  const int blocks = live ? (start + t_last) / BLK + 1 : 0;
-  const int closed = total / BLK;
-  const int lo = int((long long)blocks * split / p.splits), hi = int((long long)blocks * (split + 1) / p.splits);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");    // the joining kernel may be set up; it waits for this one's end
+  count_units<kWarps * 32>(p, prefix, scratch);
+  const int N = prefix[p.B];
+  const int c0 = cut(N, blockIdx.x, p.ctas), c1 = cut(N, blockIdx.x + 1, p.ctas);
+  if (c0 == c1) return;
+  const int u0 = c0 + cut(c1 - c0, warp, kWarps), u1 = c0 + cut(c1 - c0, warp + 1, kWarps);
+  const int rows = p.group * p.T;
 
   State<D, NQ> st;
-  int limit[NQ][2];                      // last position that a column sees
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      st.m[n][j] = -CUDART_INF_F;
-      st.l[n][j] = 0.f;
-      const int r = row0 + n * 8 + 2 * c + j;
-      limit[n][j] = r < fresh * p.group ? start + r / p.group : -1;
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[n][d][i] = 0.f;
-  }
-
-  if (lo + warp < hi) {
-    // ---- query fragments: column g of every tile, dims 4 KW c ... of the head ----
-    uint32_t qf[NQ][KW][2];              // fp16, scaled
-    float qscale[NQ][2];                 // log2(e) / sqrt(D) times the power of two taken out, for the columns 2c, 2c + 1
-    const T* qrow[NQ];
+  auto reset = [&]() {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int r = row0 + n * 8 + g;
-      const bool ok = r < rows;
-      const int t = ok ? r / p.group : 0, head = h * p.group + (ok ? r % p.group : 0);
-      qrow[n] = static_cast<const T*>(p.q) + b * p.sb + head * p.sh + t * p.st + c * (4 * KW);
-      uint32_t w[2 * KW];
-      load_words<2 * KW>(qrow[n], w);
-      float amax = 0.f;
-      if (!Act<T>::kHalf) {
 #pragma unroll
-        for (int i = 0; i < 2 * KW; ++i) amax = fmaxf(amax, fmaxf(fabsf(Act<T>::lo(w[i])), fabsf(Act<T>::hi(w[i]))));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      }
-      // exponent of the largest value (fp16 queries stay as they are); kept within what 2^-e and 2^e can express
-      int e = Act<T>::kHalf ? 0 : int(__float_as_uint(amax) >> 23) - 127;
-      e = min(max(e, -120), 120);
-      const float down = __uint_as_float(uint32_t(127 - e) << 23), up = __uint_as_float(uint32_t(127 + e) << 23);
-#pragma unroll
-      for (int i = 0; i < KW; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          qf[n][i][j] = Act<T>::kHalf ? w[2 * i + j] : pack_half2(Act<T>::lo(w[2 * i + j]) * down, Act<T>::hi(w[2 * i + j]) * down);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) qscale[n][j] = p.sm_log2 * __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
-    }
-
-    const uint8_t* base = p.codes + (long long)bh * p.blocks * (2 * BLK * D);
-    const float2* scales = reinterpret_cast<const float2*>(p.scale) + (long long)bh * p.blocks;
-    const int hi8 = min(hi, closed);
-    uint32_t kr[4][2][KW];
-    float2 sc_next = make_float2(0.f, 0.f);
-    auto load_k = [&](int blk) {
-      const uint8_t* kp = base + (long long)blk * (2 * BLK * D) + g * D + c * (4 * KW);
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) load_words<KW>(kp + (16 * m + 8 * u) * D, kr[m][u]);
-      sc_next = __ldg(scales + blk);
-    };
-    int blk = lo + warp;
-    if (blk < hi8) load_k(blk);
-    for (; blk < hi8; blk += kWarps) {
-      const float2 sc = sc_next;
-      uint32_t vr[DT][2][4];
-      const uint8_t* vp = base + (long long)blk * (2 * BLK * D) + BLK * D + g * BLK + c * 16;
+      for (int j = 0; j < 2; ++j) { st.m[n][j] = -CUDART_INF_F; st.l[n][j] = 0.f; }
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) load_words<4>(vp + (16 * d + 8 * u) * BLK, vr[d][u]);
-      float s[4][NQ][4];
+        for (int i = 0; i < 4; ++i) st.o[n][d][i] = 0.f;
+    }
+  };
+  reset();
+  Cursor cur;
+  cur.seek(p, prefix, c0);
+  // does the CTA stay within one item?  Then its four warps are joined here and count as one part.
+  const int item_begin = c0 - cur.at, item_end = item_begin + cur.units;
+  const bool one_item = c1 <= item_end;
+  if (u0 < u1 && u0 != c0) cur.seek(p, prefix, u0);
+
+  if (u0 < u1) {
+    uint8_t* ring = smem + warp * (STAGES * STAGE);
+    // Lane 0 starts the copies of a stage; the lanes below 8 NQ add the query rows where an item begins.  Tokens of the unfinished block
+    // that do not exist are copied with the rest and not used.
+    if (lane == 0) {
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          uint32_t a0, a1, a2, a3;
-          codes_to_half(kr[m][0][i], a0, a2);
-          codes_to_half(kr[m][1][i], a1, a3);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) mma_f16(s[m][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+      for (int t = 0; t < STAGES; ++t) { mbar_init(&bars[warp][t][0], 1); mbar_init(&bars[warp][t][1], 1); }
+      mbar_fence_init();
+    }
+    __syncwarp();
+    Cursor ahead = cur;
+    int u_ahead = u0;
+    auto tail_of = [&](const Cursor& k) {
+      return static_cast<const uint8_t*>(p.tail) + (((long long)k.b * p.Hkv + k.h) * 2 + (k.closed & 1)) * (4 * BLK * D) + (k.at - k.closed) * (BLK * D);
+    };
+    auto copy_k = [&](int stage) {
+      __syncwarp();                      // every lane has read what the copies overwrite
+      if (u_ahead < u1) {
+        uint8_t* dst = ring + stage * STAGE;
+        uint64_t* bar = &bars[warp][stage][0];
+        const bool begins = u_ahead == u0 || ahead.at == 0, finished = ahead.at < ahead.closed;
+        if (lane == 0) {
+          mbar_expect_tx(bar, BLK * D + (finished ? kCacheHead : 0) + (begins ? ROWS * D * 2 : 0));
+          if (finished) {
+            bulk_copy(dst, p.records + (((long long)ahead.b * p.Hkv + ahead.h) * p.blocks + ahead.at) * record_bytes(D), kCacheHead + BLK * D, bar);
+          } else {
+            bulk_copy(dst + KEYS, tail_of(ahead), BLK * D, bar);
+          }
+        }
+        if (begins) {
+          __syncwarp();                  // the bytes are expected before any arrive
+          if (lane < ROWS) {
+            const int r = ahead.tile * ROWS + lane;
+            const int t = r < rows ? r / p.group : 0, head = ahead.h * p.group + (r < rows ? r % p.group : 0);
+            bulk_copy(dst + QUERIES + lane * (D * 2), static_cast<const T*>(p.q) + ahead.b * p.sb + head * p.sh + t * p.st, D * 2, bar);
+          }
         }
       }
-      if (blk + kWarps < hi8) load_k(blk + kWarps);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float f = qscale[n][j] * sc.x;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) { s[m][n][j] *= f; s[m][n][j + 2] *= f; }
+    };
+    auto copy_v = [&](int stage) {       // then the cursor moves on
+      __syncwarp();
+      if (u_ahead < u1) {
+        if (lane == 0) {
+          uint64_t* bar = &bars[warp][stage][1];
+          mbar_expect_tx(bar, BLK * D);
+          const uint8_t* src = ahead.at < ahead.closed
+                                   ? p.records + (((long long)ahead.b * p.Hkv + ahead.h) * p.blocks + ahead.at) * record_bytes(D) + kCacheHead + BLK * D
+                                   : tail_of(ahead) + 2 * BLK * D;
+          bulk_copy(ring + stage * STAGE + VALUES, src, BLK * D, bar);
         }
-      const bool masked = blk * BLK + BLK > start;           // blocks of the step itself: rows see different lengths
-      if (masked) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (blk * BLK + 16 * m + g + 8 * (i >> 1) > limit[n][i & 1]) s[m][n][i] = -CUDART_INF_F;
+        ++u_ahead;
+        if (u_ahead < u1) ahead.next(p);
       }
-      update_max<D, NQ>(st, s);
-      uint32_t pf[4][NQ][2];
+    };
+    bool lost = false;                   // a copy did not come in time: the rest is not waited for, the host sees the status
+    auto arrive = [&](int stage, int which, uint32_t parity) {
+      if (!lost && !wait_copy(&bars[warp][stage][which], parity)) {
+        lost = true;
+        if (lane == 0) atomicMax(p.status, int(STATUS_WAIT_TIMEOUT));
+      }
+    };
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+    for (int t = 0; t < STAGES; ++t) { copy_k(t); copy_v(t); }
+
+    uint32_t qf[NQ][KW][2];              // fp16 query fragments, scaled: column g of every tile, dims 4 KW c ... of the head
+    float qscale[NQ][2];                 // log2(e) / sqrt(D) times the power of two taken out, for the columns 2c, 2c + 1
+    int limit[NQ][2];                    // last position that a column sees
+    int start = 0, fresh = 0;
+    int stage = 0;
+    uint32_t parity = 0;
+    for (int u = u0; u < u1; ++u) {
+      const uint8_t* here = ring + stage * STAGE;
+      arrive(stage, 0, parity);
+      if (u == u0 || cur.at == 0) {
+        const int2 span = span_of(p, cur.b);
+        start = span.x; fresh = span.y;
+        const int row0 = cur.tile * ROWS;
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-          pf[m][n][0] = transpose8x8(pack_half2(s[m][n][0], s[m][n][1]));
-          pf[m][n][1] = transpose8x8(pack_half2(s[m][n][2], s[m][n][3]));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = row0 + n * 8 + 2 * c + j;
+            limit[n][j] = r < fresh * p.group ? start + r / p.group : -1;
+          }
+          uint32_t w[2 * KW];
+          read_words<2 * KW>(here + QUERIES + (n * 8 + g) * (D * 2) + c * (2 * KB), w);
+          float amax = 0.f;
+          if (!Act<T>::kHalf) {
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i) amax = fmaxf(amax, fmaxf(fabsf(Act<T>::lo(w[i])), fabsf(Act<T>::hi(w[i]))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          }
+          // exponent of the largest value (fp16 queries stay as they are); kept within what 2^-e and 2^e can express
+          int e = Act<T>::kHalf ? 0 : int(__float_as_uint(amax) >> 23) - 127;
+          e = min(max(e, -120), 120);
+          const float down = __uint_as_float(uint32_t(127 - e) << 23), up = __uint_as_float(uint32_t(127 + e) << 23);
+#pragma unroll
+          for (int i = 0; i < KW; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              qf[n][i][j] = Act<T>::kHalf ? w[2 * i + j] : pack_half2(Act<T>::lo(w[2 * i + j]) * down, Act<T>::hi(w[2 * i + j]) * down);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) qscale[n][j] = p.sm_log2 * __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
         }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        float acc[NQ][4];
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+      }
+      if (cur.at < cur.closed) {
+        const int base = cur.at * BLK;
+        const uint8_t* kst = here + KEYS + g * D + c * KB;
+        const uint8_t* vst = here + VALUES + g * BLK + c * 16;
+        const float2 sc = *reinterpret_cast<const float2*>(here);
+        float s[4][NQ][4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          uint32_t a0, a1, a2, a3;
-          codes_to_half(vr[d][0][m], a0, a2);
-          codes_to_half(vr[d][1][m], a1, a3);
+          uint32_t kr[2][KW];
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) mma_f16(acc[n], a0, a1, a2, a3, pf[m][n][0], pf[m][n][1]);
-        }
+          for (int v = 0; v < 2; ++v) read_words<KW>(kst + (16 * m + 8 * v) * D, kr[v]);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+          for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)      // a block that a row does not see at all must not reach it through its scale
-            if (!masked || blk * BLK <= limit[n][i & 1]) st.o[n][d][i] = fmaf(acc[n][i], sc.y, st.o[n][d][i]);
-      }
-    }
-
-    // ---- the unfinished block, in the activation type ----
-    if (blk == closed && blk < hi) {
-      const T* tk = static_cast<const T*>(p.tail) + ((long long)bh * 2 + (blk & 1)) * (2 * BLK * D);
-      const T* tv = tk + BLK * D;
-      const int valid = total - blk * BLK;                   // what lies behind is not read
-      uint32_t qa[NQ][2 * KW];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) load_words<2 * KW>(qrow[n], qa[n]);
-      float s[4][NQ][4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        uint32_t a[2][2 * KW];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int tok = 16 * m + 8 * u + g;
-          if (tok < valid) {
-            load_words<2 * KW>(tk + tok * D + c * (4 * KW), a[u]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 2 * KW; ++i) a[u][i] = 0;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
+            for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
 #pragma unroll
           for (int i = 0; i < KW; ++i) {
-            const uint32_t f[4] = {a[0][2 * i], a[1][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]};
-            Act<T>::mma(s[m][n], f, qa[n][2 * i], qa[n][2 * i + 1]);
-          }
+            uint32_t a0, a1, a2, a3;
+            codes_to_half(kr[0][i], a0, a2);
+            codes_to_half(kr[1][i], a1, a3);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool seen = blk * BLK + 16 * m + g + 8 * (i >> 1) <= limit[n][i & 1];
-            s[m][n][i] = seen ? s[m][n][i] * p.sm_log2 : -CUDART_INF_F;
+            for (int n = 0; n < NQ; ++n) mma_f16(s[m][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
           }
         }
-      }
-      update_max<D, NQ>(st, s);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (16 * m >= valid) break;
-        uint32_t ph[NQ][2], pl[NQ][2];
+        copy_k(stage);
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float x = s[m][n][2 * u], y = s[m][n][2 * u + 1];
-            if (Act<T>::kHalf) {
-              ph[n][u] = transpose8x8(pack_half2(x, y));
-            } else {
-              const uint32_t hi2 = pack_bf162(x, y);
-              ph[n][u] = transpose8x8(hi2);
-              pl[n][u] = transpose8x8(pack_bf162(x - Act<T>::lo(hi2), y - Act<T>::hi(hi2)));
-            }
+          for (int j = 0; j < 2; ++j) {
+            const float f = qscale[n][j] * sc.x;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) { s[m][n][j] *= f; s[m][n][j + 2] *= f; }
           }
-        const int left = valid - 16 * m - 2 * c;             // tokens 16 m + 2c + {0, 1, 8, 9} of this lane that exist
-        const uint32_t keep0 = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
-        const uint32_t keep1 = left >= 10 ? 0xFFFFFFFFu : left == 9 ? 0xFFFFu : 0u;
+        const bool masked = base + BLK > start;              // blocks of the step itself: rows see different lengths
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (base + 16 * m + g + 8 * (i >> 1) > limit[n][i & 1]) s[m][n][i] = -CUDART_INF_F;
+        }
+        update_max<D, NQ, 4>(st, s);
+        uint32_t pf[4][NQ][2];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            pf[m][n][0] = transpose8x8(pack_half2(s[m][n][0], s[m][n][1]));
+            pf[m][n][1] = transpose8x8(pack_half2(s[m][n][2], s[m][n][3]));
+          }
+        arrive(stage, 1, parity);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          uint32_t f[4];
+          uint32_t vr[2][4];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint2 w = *reinterpret_cast<const uint2*>(tv + (16 * d + 8 * u + g) * BLK + c * 16 + m * 4);
-            f[u] = w.x & keep0;
-            f[u + 2] = w.y & keep1;
+          for (int v = 0; v < 2; ++v) read_words<4>(vst + (16 * d + 8 * v) * BLK, vr[v]);
+          float acc[NQ][4];
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half(vr[0][m], a0, a2);
+            codes_to_half(vr[1][m], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mma_f16(acc[n], a0, a1, a2, a3, pf[m][n][0], pf[m][n][1]);
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)    // a block that a row does not see at all must not reach it through its scale
+              if (!masked || base <= limit[n][i & 1]) st.o[n][d][i] = fmaf(acc[n][i], sc.y, st.o[n][d][i]);
+        }
+        copy_v(stage);
+      } else {                             // ---- half of the unfinished block, in the activation type ----
+        const int base = cur.closed * BLK + (cur.at - cur.closed) * 32;
+        const int valid = start + fresh - base;              // tokens that exist
+        float s[2][NQ][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          uint32_t a[2][2 * KW];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            read_words<2 * KW>(here + KEYS + (16 * m + 8 * v + g) * (D * 2) + c * (2 * KB), a[v]);
+            const uint32_t keep = 16 * m + 8 * v + g < valid ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+            for (int i = 0; i < 2 * KW; ++i) a[v][i] &= keep;
           }
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
-            Act<T>::mma(st.o[n][d], f, ph[n][0], ph[n][1]);
-            if (!Act<T>::kHalf) Act<T>::mma(st.o[n][d], f, pl[n][0], pl[n][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+              const uint32_t f[4] = {a[0][2 * i], a[1][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]};
+              Act<T>::mma(s[m][n], f, Act<T>::from_half2(qf[n][i][0]), Act<T>::from_half2(qf[n][i][1]));   // eight bits: exact
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool seen = base + 16 * m + g + 8 * (i >> 1) <= limit[n][i & 1];
+              s[m][n][i] = seen ? s[m][n][i] * qscale[n][i & 1] : -CUDART_INF_F;
+            }
           }
         }
+        copy_k(stage);
+        update_max<D, NQ, 2>(st, s);
+        arrive(stage, 1, parity);
+        uint32_t ph[2][NQ][2], pl[2][NQ][2], keep[2][2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              const float x = s[m][n][2 * v], y = s[m][n][2 * v + 1];
+              if (Act<T>::kHalf) {
+                ph[m][n][v] = transpose8x8(pack_half2(x, y));
+              } else {
+                const uint32_t hi2 = pack_bf162(x, y);
+                ph[m][n][v] = transpose8x8(hi2);
+                pl[m][n][v] = transpose8x8(pack_bf162(x - Act<T>::lo(hi2), y - Act<T>::hi(hi2)));
+              }
+            }
+          const int left = valid - 16 * m - 2 * c;           // tokens 16 m + 2c + {0, 1, 8, 9} of this lane that exist
+          keep[m][0] = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
+          keep[m][1] = left >= 10 ? 0xFFFFFFFFu : left == 9 ? 0xFFFFu : 0u;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          uint32_t w[2][4];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) read_words<4>(here + VALUES + (16 * d + 8 * v + g) * 64 + c * 16, w[v]);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t f[4] = {w[0][2 * m] & keep[m][0], w[1][2 * m] & keep[m][0], w[0][2 * m + 1] & keep[m][1], w[1][2 * m + 1] & keep[m][1]};
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+              Act<T>::mma(st.o[n][d], f, ph[m][n][0], ph[m][n][1]);
+              if (!Act<T>::kHalf) Act<T>::mma(st.o[n][d], f, pl[m][n][0], pl[m][n][1]);
+            }
+          }
+        }
+        copy_v(stage);
       }
+      if (++stage == STAGES) { stage = 0; parity ^= 1; }
+
+      const bool ends = cur.at + 1 == cur.units;
+      if (!one_item && (ends || u + 1 == u1)) {
+        // ---- the warp is done with this item: its output if the item was not cut, else its part ----
+        const bool whole = ends && u - cur.at >= u0;
+        const int row0 = cur.tile * ROWS;
+        float* dst = p.part + (2 * ((long long)blockIdx.x * kWarps + warp) + (u - cur.at >= u0 ? 1 : 0)) * (ROWS * (D + 2));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float l = st.l[n][j];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            const int r = n * 8 + 2 * c + j, row = row0 + r;
+            if (row >= fresh * p.group) continue;
+            const int t = row / p.group, head = cur.h * p.group + row % p.group;
+            T* out = static_cast<T*>(p.o) + (((long long)cur.b * p.T + t) * p.Hq + head) * D;
+            float* part = dst + r * (D + 2);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int dim = 16 * d + g + 8 * i;
+                if (whole) out[dim] = Act<T>::from(st.o[n][d][j + 2 * i] / l);
+                else part[dim] = st.o[n][d][j + 2 * i];
+              }
+            if (!whole && g == 0) { part[D] = st.m[n][j]; part[D + 1] = l; }
+          }
+        reset();
+      }
+      if (u + 1 < u1) cur.next(p);
+    }
+    if (lost) {                          // copies may still be on their way: give them time before the memory changes hands
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000000ull) __nanosleep(1000);
     }
   }
+  if (!one_item) return;
 
   // ---- join the warps ----
+  __syncthreads();                       // the rings are read; their memory takes the outputs
+  if (u0 == u1) cur.seek(p, prefix, c0);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
 #pragma unroll
@@ -383,12 +599,14 @@ cached_attention_kernel(const Params p) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o_sm[warp][(16 * d + g + 8 * (i >> 1)) * OP + n * 8 + 2 * c + (i & 1)] = st.o[n][d][i];
+      for (int i = 0; i < 4; ++i) o_sm[warp * (D * OP) + (16 * d + g + 8 * (i >> 1)) * OP + n * 8 + 2 * c + (i & 1)] = st.o[n][d][i];
   }
   __syncthreads();
+  const int live = span_of(p, cur.b).y * p.group, row0 = cur.tile * ROWS;
+  const bool whole = c0 == item_begin && c1 == item_end;
   for (int i = threadIdx.x; i < ROWS * D; i += kWarps * 32) {
     const int r = i / D, d = i % D, row = row0 + r;
-    if (row >= rows) break;
+    if (row >= live) break;
     float m = -CUDART_INF_F;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml_sm[w][r][0]);
@@ -398,125 +616,205 @@ cached_attention_kernel(const Params p) {
     for (int w = 0; w < kWarps; ++w) {
       const float a = exp2f(ml_sm[w][r][0] - base);
       l = fmaf(ml_sm[w][r][1], a, l);
-      o = fmaf(o_sm[w][d * OP + r], a, o);
+      o = fmaf(o_sm[w * (D * OP) + d * OP + r], a, o);
     }
-    if (p.splits == 1) {
-      const int t = row / p.group, head = h * p.group + row % p.group;
-      static_cast<T*>(p.o)[(((long long)b * p.T + t) * p.Hq + head) * D + d] = Act<T>::from(t < fresh ? o / l : 0.f);
+    if (whole) {
+      const int t = row / p.group, head = cur.h * p.group + row % p.group;
+      static_cast<T*>(p.o)[(((long long)cur.b * p.T + t) * p.Hq + head) * D + d] = Act<T>::from(o / l);
     } else {
-      float* dst = p.part + (((long long)item * p.splits + split) * ROWS + r) * (D + 2);
+      float* dst = p.part + (2 * (long long)blockIdx.x * kWarps * ROWS + r) * (D + 2);
       dst[d] = o;
       if (d == 0) { dst[D] = m; dst[D + 1] = l; }
     }
   }
 }
 
-// Joins the splits of one row: one warp a row, splits in order.
+// Joins the parts of one row, a CTA a row, and zeroes the rows of padding; rows of items that were not cut are there already.
+// The weight of every part first, then the eight warps add the outputs of every eighth part, and the eight sums in order.
+constexpr int kJoinThreads = 256;
 template <typename T, int D>
-__global__ void __launch_bounds__(128)
-join_splits_kernel(const Params p, int rows_per_tile, long long total_rows) {
-  const long long gr = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (gr >= total_rows) return;
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kJoinThreads)
+join_parts_kernel(const Params p, int rows_per_tile) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* prefix = reinterpret_cast<int*>(smem);              // [B + 1]
+  int* slot = prefix + p.B + 1;                            // [parts]
+  float* weight = reinterpret_cast<float*>(slot + p.ctas + 2 * kWarps);
+  __shared__ float red[kJoinThreads / 32], o_sm[kJoinThreads / 32][D];
+  __shared__ int scratch[kJoinThreads / 32];
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.group * p.T;
-  const int row = int(gr % rows);
-  const long long bh = gr / rows;
-  const int h = int(bh % p.Hkv), b = int(bh / p.Hkv);
-  const long long item = bh * p.row_tiles + row / rows_per_tile;
-  const float* src = p.part + (item * p.splits * rows_per_tile + row % rows_per_tile) * (D + 2);
-  const long long pitch = (long long)rows_per_tile * (D + 2);
-  const int capacity = p.blocks * BLK;
-  const int start = min(max(p.start[b], 0), capacity);
-  const int fresh = min(start + min(max(p.count[b], 0), p.T), capacity) - start;
+  const int row = int(blockIdx.x % unsigned(rows));
+  const int bh = int(blockIdx.x / unsigned(rows));
+  const int h = bh % p.Hkv, b = bh / p.Hkv;
   const int t = row / p.group, head = h * p.group + row % p.group;
+  T* out = static_cast<T*>(p.o) + (((long long)b * p.T + t) * p.Hq + head) * D;
+  const int2 span = span_of(p, b);
+  if (t >= span.y) {
+    for (int d = threadIdx.x; d < D; d += kJoinThreads) out[d] = Act<T>::from(0.f);
+    return;
+  }
+  count_units<kJoinThreads>(p, prefix, scratch);
+  const int N = prefix[p.B];
+  const int begin = prefix[b] + (h * p.row_tiles + row / rows_per_tile) * units_of(span), end = begin + units_of(span);
+  const int i0 = owner(N, begin, p.ctas), i1 = owner(N, end - 1, p.ctas);
+  // candidates: the warps of the first and of the last CTA, and one part of every CTA between (those lie within the item)
+  const int between = max(i1 - i0 - 1, 0), candidates = kWarps + (i1 > i0 ? between + kWarps : 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // everything above read only what the caller wrote
+  bool whole = false;
   float m = -CUDART_INF_F;
-  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, src[s * pitch + D]);
+  const float* src = p.part + (long long)(row % rows_per_tile) * (D + 2);
+  const long long pitch = (long long)rows_per_tile * (D + 2);
+  for (int k = threadIdx.x; k < candidates; k += kJoinThreads) {
+    const int i = k < kWarps ? i0 : k < kWarps + between ? i0 + 1 + k - kWarps : i1;
+    const int w = k < kWarps ? k : k < kWarps + between ? 0 : k - kWarps - between;
+    const int c0 = cut(N, i, p.ctas), c1 = cut(N, i + 1, p.ctas);
+    int at = -1;
+    if (c0 >= begin && c1 <= end) {                        // within the item: its warps are one part
+      if (w == 0 && c0 < c1) at = 2 * i * kWarps;
+      whole |= c0 == begin && c1 == end;
+    } else {
+      const int x0 = c0 + cut(c1 - c0, w, kWarps), x1 = c0 + cut(c1 - c0, w + 1, kWarps);
+      if (x0 < end && x1 > begin && x0 < x1) {
+        at = 2 * (i * kWarps + w) + (x0 <= begin ? 1 : 0);
+        whole |= x0 <= begin && x1 >= end;
+      }
+    }
+    slot[k] = at;
+    if (at >= 0) m = fmaxf(m, src[at * pitch + D]);
+  }
+  if (__syncthreads_or(whole)) return;                     // its owner has written the output
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, red[w]);
   const float base = m == -CUDART_INF_F ? 0.f : m;
-  float l = 0.f, o[D / 32];
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j) o[j] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float a = exp2f(src[s * pitch + D] - base);
-    l = fmaf(src[s * pitch + D + 1], a, l);
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) o[j] = fmaf(src[s * pitch + j * 32 + lane], a, o[j]);
+  __syncthreads();
+  float l = 0.f;
+  for (int k = threadIdx.x; k < candidates; k += kJoinThreads) {
+    float a = 0.f;
+    if (slot[k] >= 0) {
+      a = exp2f(src[slot[k] * pitch + D] - base);
+      l = fmaf(src[slot[k] * pitch + D + 1], a, l);
+    }
+    weight[k] = a;
   }
-  T* dst = static_cast<T*>(p.o) + (((long long)b * p.T + t) * p.Hq + head) * D;
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) dst[j * 32 + lane] = Act<T>::from(t < fresh ? o[j] / l : 0.f);
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (lane == 0) red[warp] = l;
+  __syncthreads();
+  float o[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) o[j] = 0.f;
+#pragma unroll 4
+  for (int k = warp; k < candidates; k += kJoinThreads / 32) {
+    if (slot[k] < 0) continue;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[j] = fmaf(src[slot[k] * pitch + j * 32 + lane], weight[k], o[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) o_sm[warp][j * 32 + lane] = o[j];
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += kJoinThreads) {
+    float sum = 0.f, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) { sum += o_sm[w][d]; total += red[w]; }
+    out[d] = Act<T>::from(sum / total);
+  }
 }
 
 struct Plan {
-  int nq, row_tiles, splits;
-  long long items;
+  int nq, row_tiles, ctas;
 };
 
-// Query rows in tiles of 8, 16 or 32 (16 at D = 128, where the accumulators of 32 would not fit in registers), and as many splits
-// of the cache as fill the machine with four CTAs an SM, while each warp of a split still has a block of its own.
-// The capacity decides, not the lengths, which only the device knows.
+// Query rows in tiles of 8, 16 or 32 (16 at D = 128, where the accumulators of 32 would not fit in registers); as many CTAs as are
+// resident at once, or as there can be units for.  The capacity decides, not the lengths, which only the device knows.
 Plan plan_for(int B, int Hkv, int Hq, int T, int D, int blocks) {
   Plan pl;
   const int rows = Hq / Hkv * T, most = D == 128 ? 2 : 4;
   pl.nq = rows <= 8 ? 1 : rows <= 16 ? 2 : most;
   pl.row_tiles = (rows + 8 * pl.nq - 1) / (8 * pl.nq);
-  pl.items = (long long)B * Hkv * pl.row_tiles;
-  const long long want = ((long long)device_sm_count() * 4 + pl.items - 1) / pl.items;
-  const long long fit = (blocks + kWarps - 1) / kWarps;
-  const long long s = want < fit ? want : fit;
-  pl.splits = int(s < 1 ? 1 : s);
+  const long long units = (long long)B * Hkv * pl.row_tiles * blocks;
+  // the third ring of a CTA leaves little room for the counts of many sequences
+  const int resident = B <= 160 ? ctas_per_sm(pl.nq) : 2;
+  const long long slots = (long long)device_sm_count() * resident;
+  pl.ctas = int(units < slots ? units : slots);
   return pl;
 }
 
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool> (&ready)[64]) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (ready[dev]) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) ready[dev] = true;
+  return err;
+}
+
 template <typename T, int D, int NQ>
-cudaError_t launch_typed(const Params& p, const Plan& pl, int B, cudaStream_t stream) {
-  // the grid's y and z extents hold at most 65,535 each
-  const long long y = pl.items < 32768 ? pl.items : 1;
-  long long gy = y, gz = 1;
-  if (pl.items >= 32768) {
-    gy = (long long)p.Hkv * p.row_tiles;
-    gz = B;
-    if (gy > 65535 || gz > 65535) return cudaErrorInvalidConfiguration;
-  }
-  cached_attention_kernel<T, D, NQ><<<dim3(unsigned(p.splits), unsigned(gy), unsigned(gz)), kWarps * 32, 0, stream>>>(p);
+cudaError_t launch_typed(const Params& p, cudaStream_t stream) {
+  static std::atomic<bool> ready[64];
+  const int bytes = shared_bytes(D, NQ);
+  cudaError_t err = allow_shared(cached_attention_kernel<T, D, NQ>, bytes + (kBatchMax + 1) * 4, ready);
+  if (err != cudaSuccess) return err;
+  const long long rows = (long long)p.B * p.Hkv * p.group * p.T;
+  if (rows > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  cached_attention_kernel<T, D, NQ><<<unsigned(p.ctas), kWarps * 32, bytes + (p.B + 1) * 4, stream>>>(p);
   ++g_launch_count;
-  if (p.splits > 1) {
-    const long long rows = (long long)B * p.Hkv * p.group * p.T;
-    join_splits_kernel<T, D><<<unsigned((rows + 3) / 4), 128, 0, stream>>>(p, 8 * NQ, rows);
-    ++g_launch_count;
-  }
-  return cudaGetLastError();
+  if ((err = cudaGetLastError()) != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = size_t(p.B + 1 + 2 * (p.ctas + 2 * kWarps)) * 4;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, D>, p, 8 * NQ);
+  ++g_launch_count;
+  return err;
 }
 
 template <typename T, int D>
-cudaError_t launch_dim(const Params& p, const Plan& pl, int B, cudaStream_t stream) {
-  if (pl.nq == 1) return launch_typed<T, D, 1>(p, pl, B, stream);
-  if (pl.nq == 2) return launch_typed<T, D, 2>(p, pl, B, stream);
-  if constexpr (D != 128) return launch_typed<T, D, 4>(p, pl, B, stream);
+cudaError_t launch_dim(const Params& p, const Plan& pl, cudaStream_t stream) {
+  if (pl.nq == 1) return launch_typed<T, D, 1>(p, stream);
+  if (pl.nq == 2) return launch_typed<T, D, 2>(p, stream);
+  if constexpr (D != 128) return launch_typed<T, D, 4>(p, stream);
   return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
+bool cached_attention_fits(int B, int Hkv, int Hq, int T, int D, int blocks) {
+  const Plan pl = plan_for(B, Hkv, Hq, T, D, blocks);
+  return B <= kBatchMax && (long long)B * Hkv * pl.row_tiles * blocks <= (1ll << 30);
+}
+
 size_t cached_attention_workspace_floats(int B, int Hkv, int Hq, int T, int D, int blocks) {
   const Plan pl = plan_for(B, Hkv, Hq, T, D, blocks);
-  return pl.splits == 1 ? 0 : size_t(pl.items) * pl.splits * (8 * pl.nq) * (D + 2);
+  return size_t(2) * pl.ctas * kWarps * (8 * pl.nq) * (D + 2);
 }
 
 cudaError_t launch_cached_attention(const CachedAttentionArgs& a) {
   const CacheView& c = a.cache;
+  if (a.workspace == nullptr || !cached_attention_fits(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks)) return cudaErrorInvalidValue;
   const Plan pl = plan_for(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks);
-  if (pl.splits > 1 && a.workspace == nullptr) return cudaErrorInvalidValue;
   Params p;
-  p.codes = c.codes; p.scale = c.scale; p.tail = c.tail; p.start = c.start; p.count = c.count;
-  p.Hkv = c.Hkv; p.blocks = c.blocks; p.Hq = a.Hq; p.T = a.T; p.group = a.Hq / c.Hkv;
-  p.row_tiles = pl.row_tiles; p.splits = pl.splits;
+  p.records = c.records; p.tail = c.tail; p.start = c.start; p.count = c.count;
+  p.B = c.B; p.Hkv = c.Hkv; p.blocks = c.blocks; p.Hq = a.Hq; p.T = a.T; p.group = a.Hq / c.Hkv;
+  p.row_tiles = pl.row_tiles; p.ctas = pl.ctas;
   p.q = a.q.p; p.sb = a.q.sb; p.sh = a.q.sh; p.st = a.q.st;
-  p.o = a.o; p.part = a.workspace; p.sm_log2 = a.scale * kLog2e;
-  if (c.D == 32) return c.fp16 ? launch_dim<__half, 32>(p, pl, c.B, a.stream) : launch_dim<__nv_bfloat16, 32>(p, pl, c.B, a.stream);
-  if (c.D == 64) return c.fp16 ? launch_dim<__half, 64>(p, pl, c.B, a.stream) : launch_dim<__nv_bfloat16, 64>(p, pl, c.B, a.stream);
-  if (c.D == 128) return c.fp16 ? launch_dim<__half, 128>(p, pl, c.B, a.stream) : launch_dim<__nv_bfloat16, 128>(p, pl, c.B, a.stream);
+  p.o = a.o; p.part = a.workspace; p.sm_log2 = a.scale * kLog2e; p.status = a.status;
+  if (c.D == 32) return c.fp16 ? launch_dim<__half, 32>(p, pl, a.stream) : launch_dim<__nv_bfloat16, 32>(p, pl, a.stream);
+  if (c.D == 64) return c.fp16 ? launch_dim<__half, 64>(p, pl, a.stream) : launch_dim<__nv_bfloat16, 64>(p, pl, a.stream);
+  if (c.D == 128) return c.fp16 ? launch_dim<__half, 128>(p, pl, a.stream) : launch_dim<__nv_bfloat16, 128>(p, pl, a.stream);
   return cudaErrorInvalidValue;
 }
 

@@ -10,19 +10,23 @@ namespace mts {
 // ---- the cache of one layer -----------------------------------------------------------------------------------------
 // Tokens of a (sequence, K/V head) are grouped in blocks of kCacheBlock.  A finished block is held in 8 bits, the unfinished
 // one in the activation type, so that a value is rounded to 8 bits once, whatever calls brought the tokens.
-//   codes [B, Hkv, blocks, 2, 64 * D] uint8: excess-128 codes, K as [token][dim], V as [dim][slot of the token]
-//   scale [B, Hkv, blocks, 2] fp32: value = (code - 128) * scale
-//   tail  [B, Hkv, 2, 2, 64 * D] activation type: block j is at index j & 1, laid out as the codes are
-// The slot of token 16 m + u of a V row is cache_slot(16 m + u): the four tokens that one lane of an m16n8k16 product needs per
-// step are adjacent, and the sixteen that it needs per block are one 16-byte load.
+//   records [B, Hkv, blocks, 16 + 2 * 64 * D] bytes: the fp32 scales of K and V (and 8 bytes of padding), then excess-128 codes, K as
+//                    [token][dim], V as [dim][cache_slot(token)];  value = (code - 128) * scale
+//   tail    [B, Hkv, 2, 2, 64 * D] activation type: block j is at index j & 1; K as [token][dim], V as tail_slot(dim, token)
+// One copy of adjacent bytes brings the keys of a block with its scales, one its values; a half of the unfinished block (32 tokens in
+// 16 bits) is as many bytes.  In a row of V the tokens that one lane of an m16n8k16 product needs are adjacent: four of every 16.
 constexpr int kCacheBlock = 64;
+constexpr int kCacheHead = 16;           // bytes before the codes of a record
 __host__ __device__ constexpr int cache_slot(int token) {
   return ((token & 7) >> 1) * 16 + (token >> 4) * 4 + ((token >> 3) & 1) * 2 + (token & 1);
 }
+__host__ __device__ constexpr int tail_slot(int D, int dim, int token) {      // halves of 32 tokens one after the other
+  return ((token >> 5) * D + dim) * 32 + ((token & 7) >> 1) * 8 + ((token >> 4) & 1) * 4 + ((token >> 3) & 1) * 2 + (token & 1);
+}
+__host__ __device__ constexpr int record_bytes(int D) { return kCacheHead + 2 * kCacheBlock * D; }
 
 struct CacheView {
-  uint8_t* codes;
-  float* scale;
+  uint8_t* records;
   void* tail;
   const int* start;      // [B] tokens before this step
   const int* count;      // [B] new tokens of this step
@@ -48,9 +52,11 @@ struct CachedAttentionArgs {
   void* o;               // [B, T, Hq, D] storage
   int Hq, T;
   float scale;
-  float* workspace;      // cached_attention_workspace_floats(...) floats; may be null when that is 0
+  float* workspace;      // cached_attention_workspace_floats(...) floats
+  int* status;           // raised to STATUS_WAIT_TIMEOUT by a wait that gives up
   cudaStream_t stream;
 };
+bool cached_attention_fits(int B, int Hkv, int Hq, int T, int D, int blocks);
 size_t cached_attention_workspace_floats(int B, int Hkv, int Hq, int T, int D, int blocks);
 cudaError_t launch_cached_attention(const CachedAttentionArgs& a);
 

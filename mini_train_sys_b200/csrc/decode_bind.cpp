@@ -8,6 +8,7 @@
 namespace {
 
 using torch::Tensor;
+namespace py = pybind11;
 
 bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 
@@ -20,129 +21,133 @@ void check_ints(const Tensor& t, int64_t n, const Tensor& like, const char* name
   TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == n, name, " must be contiguous int32 with one entry per sequence");
 }
 
-// codes [B, Hkv, blocks, 2, 64 * D], scale [B, Hkv, blocks, 2], tail [B, Hkv, 2, 2, 64 * D]
-mts::CacheView cache_view(const Tensor& codes, const Tensor& scale, const Tensor& tail, const Tensor& start, const Tensor& count) {
-  TORCH_CHECK(codes.is_cuda() && codes.dim() == 5 && codes.scalar_type() == at::kByte && codes.is_contiguous() && aligned16(codes) &&
-                  codes.size(3) == 2 && codes.size(4) % mts::kCacheBlock == 0, "cache codes must be contiguous uint8 [B, Hkv, blocks, 2, 64 * D]");
-  const int64_t B = codes.size(0), H = codes.size(1), N = codes.size(2), D = codes.size(4) / mts::kCacheBlock;
-  TORCH_CHECK(D == 32 || D == 64 || D == 128, "cache head dimension must be 32, 64 or 128");
-  TORCH_CHECK(B > 0 && H > 0 && N > 0 && B <= 65535 && H <= 65535 && N <= (1 << 24), "unsupported cache extents");
-  check_same_device(scale, codes, "cache scale");
-  TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.dim() == 4 && scale.size(0) == B && scale.size(1) == H &&
-                  scale.size(2) == N && scale.size(3) == 2 && aligned16(scale), "cache scale must be contiguous fp32 [B, Hkv, blocks, 2]");
-  check_same_device(tail, codes, "cache tail");
-  TORCH_CHECK((tail.scalar_type() == at::kBFloat16 || tail.scalar_type() == at::kHalf) && tail.is_contiguous() && aligned16(tail) &&
-                  tail.dim() == 5 && tail.size(0) == B && tail.size(1) == H && tail.size(2) == 2 && tail.size(3) == 2 &&
-                  tail.size(4) == mts::kCacheBlock * D, "cache tail must be contiguous bf16 or fp16 [B, Hkv, 2, 2, 64 * D]");
-  check_ints(start, B, codes, "start");
-  check_ints(count, B, codes, "count");
+// One layer of a cache, checked once: records [B, Hkv, blocks, 16 + 128 D] bytes, tail [B, Hkv, 2, 2, 64 D], lengths and counts [B].
+// The operators answer None for inputs that they do not cover; the caller then takes its plain path, which also words the errors.
+struct KvLayer {
+  Tensor records, tail, start, count;
   mts::CacheView c;
-  c.codes = codes.data_ptr<uint8_t>(); c.scale = scale.data_ptr<float>(); c.tail = tail.data_ptr();
-  c.start = start.data_ptr<int>(); c.count = count.data_ptr<int>();
-  c.B = int(B); c.Hkv = int(H); c.blocks = int(N); c.D = int(D);
-  c.fp16 = tail.scalar_type() == at::kHalf;
-  return c;
-}
+  int* status;
 
-mts::Strided rows_of(const Tensor& t, const Tensor& tail, int64_t B, int64_t H, int64_t T, int64_t D, const char* name) {
-  check_same_device(t, tail, name);
-  TORCH_CHECK(t.scalar_type() == tail.scalar_type(), name, " must have the cache's activation type");
-  TORCH_CHECK(t.dim() == 4 && t.size(0) == B && t.size(1) == H && t.size(2) == T && t.size(3) == D, name, " must be [B, heads, T, D]");
-  TORCH_CHECK(t.stride(3) == 1 && aligned16(t), name, " must have a contiguous, 16-byte aligned last dimension");
-  for (int i = 0; i < 3; ++i)
-    TORCH_CHECK(t.size(i) == 1 || t.stride(i) % 8 == 0, name, " rows must be 16-byte aligned");
-  return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
-}
+  KvLayer(Tensor records_, Tensor tail_, Tensor start_, Tensor count_, Tensor status_)
+      : records(std::move(records_)), tail(std::move(tail_)), start(std::move(start_)), count(std::move(count_)), status_word_(std::move(status_)) {
+    TORCH_CHECK(tail.is_cuda() && tail.dim() == 5 && tail.is_contiguous() && aligned16(tail) && tail.size(2) == 2 && tail.size(3) == 2 &&
+                    (tail.scalar_type() == at::kBFloat16 || tail.scalar_type() == at::kHalf) && tail.size(4) % mts::kCacheBlock == 0,
+                "cache tail must be contiguous bf16 or fp16 [B, Hkv, 2, 2, 64 * D]");
+    const int64_t B = tail.size(0), H = tail.size(1), D = tail.size(4) / mts::kCacheBlock;
+    TORCH_CHECK(D == 32 || D == 64 || D == 128, "cache head dimension must be 32, 64 or 128");
+    check_same_device(records, tail, "cache records");
+    TORCH_CHECK(records.scalar_type() == at::kByte && records.dim() == 4 && records.is_contiguous() && aligned16(records) && records.size(0) == B &&
+                    records.size(1) == H && records.size(3) == mts::record_bytes(int(D)), "cache records must be contiguous uint8 [B, Hkv, blocks, 16 + 128 * D]");
+    TORCH_CHECK(B > 0 && H > 0 && records.size(2) > 0 && B <= 65535 && H <= 65535 && records.size(2) <= (1 << 24), "unsupported cache extents");
+    check_ints(start, B, tail, "lengths");
+    check_ints(count, B, tail, "counts");
+    check_ints(status_word_, 4, tail, "status");
+    c.records = records.data_ptr<uint8_t>(); c.tail = tail.data_ptr();
+    c.start = start.data_ptr<int>(); c.count = count.data_ptr<int>();
+    c.B = int(B); c.Hkv = int(H); c.blocks = int(records.size(2)); c.D = int(D);
+    c.fp16 = tail.scalar_type() == at::kHalf;
+    status = status_word_.data_ptr<int>();
+  }
 
-c10::optional<Tensor> kv_append(Tensor codes, Tensor scale, Tensor tail, const Tensor& start, const Tensor& count, const Tensor& k, const Tensor& v,
-                                const c10::optional<Tensor>& q, const c10::optional<Tensor>& cosv, const c10::optional<Tensor>& sinv) {
-  const mts::CacheView c = cache_view(codes, scale, tail, start, count);
-  TORCH_CHECK(k.dim() == 4 && k.size(2) > 0 && k.size(2) <= (1 << 30), "k must be [B, heads, T, D] with at least one token");
-  const int64_t T = k.size(2);
-  const mts::Strided kr = rows_of(k, tail, c.B, c.Hkv, T, c.D, "k"), vr = rows_of(v, tail, c.B, c.Hkv, T, c.D, "v");
-  const bool rotate = cosv.has_value() && cosv->defined();
-  TORCH_CHECK(rotate == (sinv.has_value() && sinv->defined()), "cos and sin come together");
-  if (rotate)
-    for (const Tensor* t : {&*cosv, &*sinv}) {
-      check_same_device(*t, codes, "rotary table");
-      TORCH_CHECK(t->scalar_type() == tail.scalar_type() && t->dim() == 2 && t->size(1) == c.D && t->size(0) == cosv->size(0) &&
-                      t->size(0) <= (1 << 30) && t->is_contiguous() && aligned16(*t), "rotary tables must be contiguous [positions, D] in the activation type");
+  // [B, heads, T, D] rows of the cache's type that can be read 16 bytes at a time, without a gradient to be kept
+  bool covers(const Tensor& t, int64_t heads, int64_t T) const {
+    if (t.dim() != 4 || t.scalar_type() != tail.scalar_type() || t.device() != tail.device()) return false;
+    if (t.size(0) != c.B || t.size(1) != heads || t.size(2) != T || t.size(3) != c.D || t.stride(3) != 1 || !aligned16(t)) return false;
+    for (int i = 0; i < 3; ++i)
+      if (t.size(i) != 1 && t.stride(i) % 8 != 0) return false;
+    return !(t.requires_grad() && at::GradMode::is_enabled());
+  }
+
+  // `padded`: tokens of the open step (0: none is open); `reach`: positions that the rotary tables have to hold.  True, or the rotated q.
+  py::object append(const Tensor& k, const Tensor& v, const c10::optional<Tensor>& q, const c10::optional<Tensor>& cosv,
+                    const c10::optional<Tensor>& sinv, int64_t padded, int64_t reach) const {
+    if (padded <= 0 || padded > (1 << 30) || !covers(k, c.Hkv, padded) || !covers(v, c.Hkv, padded)) return py::none();
+    const bool rotate = cosv.has_value();
+    if (rotate != sinv.has_value()) return py::none();
+    if (rotate)
+      for (const Tensor* t : {&*cosv, &*sinv})
+        if (t->device() != tail.device() || t->scalar_type() != tail.scalar_type() || t->dim() != 2 || t->size(1) != c.D || t->size(0) != cosv->size(0) ||
+            t->size(0) < reach || t->size(0) > (1 << 30) || !t->is_contiguous() || !aligned16(*t))
+          return py::none();
+    int64_t Hq = 0;
+    if (q.has_value()) {
+      if (q->dim() != 4) return py::none();
+      Hq = q->size(1);
+      if (Hq <= 0 || Hq > 65535 || Hq % c.Hkv != 0 || !covers(*q, Hq, padded)) return py::none();
     }
-  c10::cuda::CUDAGuard guard(codes.device());
-  mts::Strided qr{nullptr, 0, 0, 0};
-  Tensor out;
-  int64_t Hq = 0;
-  if (q.has_value() && q->defined()) {
-    TORCH_CHECK(q->dim() == 4 && q->size(1) > 0 && q->size(1) <= 65535, "q must be [B, heads, T, D]");
-    Hq = q->size(1);
-    qr = rows_of(*q, tail, c.B, Hq, T, c.D, "q");
-    out = torch::empty({c.B, T, Hq, c.D}, q->options()).transpose(1, 2);
+    c10::cuda::CUDAGuard guard(tail.device());
+    mts::Strided qr{nullptr, 0, 0, 0};
+    Tensor out;
+    if (q.has_value()) {
+      qr = rows_of(*q);
+      out = at::empty({c.B, padded, Hq, c.D}, q->options()).transpose(1, 2);
+    }
+    const cudaError_t e = mts::launch_kv_append(c, qr, int(Hq), rows_of(k), rows_of(v), out.defined() ? out.data_ptr() : nullptr,
+                                                rotate ? cosv->data_ptr() : nullptr, rotate ? sinv->data_ptr() : nullptr,
+                                                rotate ? int(cosv->size(0)) : 0, int(padded), at::cuda::getCurrentCUDAStream().stream());
+    TORCH_CHECK(e == cudaSuccess, "kv_append failed: ", cudaGetErrorString(e));
+    if (!out.defined()) return py::bool_(true);
+    return py::cast(out);
   }
-  const cudaError_t e = mts::launch_kv_append(c, qr, int(Hq), kr, vr, out.defined() ? out.data_ptr() : nullptr, rotate ? cosv->data_ptr() : nullptr,
-                                              rotate ? sinv->data_ptr() : nullptr, rotate ? int(cosv->size(0)) : 0, int(T),
-                                              at::cuda::getCurrentCUDAStream().stream());
-  TORCH_CHECK(e == cudaSuccess, "kv_append failed: ", cudaGetErrorString(e));
-  if (!out.defined()) return c10::nullopt;
-  return out;
-}
 
-std::vector<Tensor> kv_read(const Tensor& codes, const Tensor& scale, const Tensor& tail, const Tensor& start, const Tensor& count,
-                            const Tensor& first, int64_t n) {
-  const mts::CacheView c = cache_view(codes, scale, tail, start, count);
-  check_ints(first, c.B, codes, "first");
-  TORCH_CHECK(n >= 0 && n <= (1 << 30), "the number of positions must not be negative");
-  c10::cuda::CUDAGuard guard(codes.device());
-  Tensor k = torch::empty({c.B, c.Hkv, n, c.D}, codes.options().dtype(torch::kFloat)), v = torch::empty_like(k);
-  if (n > 0) {
-    const cudaError_t e = mts::launch_kv_read(c, first.data_ptr<int>(), int(n), k.data_ptr<float>(), v.data_ptr<float>(),
-                                              at::cuda::getCurrentCUDAStream().stream());
-    TORCH_CHECK(e == cudaSuccess, "kv_read failed: ", cudaGetErrorString(e));
+  py::object read(const Tensor& first, int64_t n) const {
+    if (n < 0 || n > (1 << 30) || first.device() != tail.device() || first.scalar_type() != at::kInt || first.dim() != 1 || first.size(0) != c.B ||
+        !first.is_contiguous())
+      return py::none();
+    c10::cuda::CUDAGuard guard(tail.device());
+    Tensor k = at::empty({c.B, c.Hkv, n, c.D}, tail.options().dtype(at::kFloat)), v = at::empty_like(k);
+    if (n > 0) {
+      const cudaError_t e = mts::launch_kv_read(c, first.data_ptr<int>(), int(n), k.data_ptr<float>(), v.data_ptr<float>(),
+                                                at::cuda::getCurrentCUDAStream().stream());
+      TORCH_CHECK(e == cudaSuccess, "kv_read failed: ", cudaGetErrorString(e));
+    }
+    return py::make_tuple(k, v);
   }
-  return {k, v};
-}
 
-Tensor cached_attention(const Tensor& codes, const Tensor& scale, const Tensor& tail, const Tensor& start, const Tensor& count, const Tensor& q,
-                        double softmax_scale) {
-  mts::CachedAttentionArgs a;
-  a.cache = cache_view(codes, scale, tail, start, count);
-  TORCH_CHECK(q.dim() == 4 && q.size(1) > 0 && q.size(1) % a.cache.Hkv == 0 && q.size(2) > 0, "q must be [B, heads, T, D] with a multiple of the cache's heads");
-  TORCH_CHECK(q.size(1) / a.cache.Hkv * q.size(2) <= (1 << 24), "too many query rows");
-  a.Hq = int(q.size(1)); a.T = int(q.size(2));
-  a.q = rows_of(q, tail, a.cache.B, a.Hq, a.T, a.cache.D, "q");
-  a.scale = float(softmax_scale);
-  c10::cuda::CUDAGuard guard(codes.device());
-  Tensor o = torch::empty({a.cache.B, a.T, a.Hq, a.cache.D}, q.options()).transpose(1, 2);
-  a.o = o.data_ptr();
-  const size_t floats = mts::cached_attention_workspace_floats(a.cache.B, a.cache.Hkv, a.Hq, a.T, a.cache.D, a.cache.blocks);
-  Tensor ws;
-  if (floats > 0) ws = torch::empty({int64_t(floats)}, codes.options().dtype(torch::kFloat));
-  a.workspace = floats > 0 ? ws.data_ptr<float>() : nullptr;
-  a.stream = at::cuda::getCurrentCUDAStream().stream();
-  const cudaError_t e = mts::launch_cached_attention(a);
-  TORCH_CHECK(e == cudaSuccess, "cached_attention failed: ", cudaGetErrorString(e));
-  return o;
-}
-
-Tensor moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_up, const Tensor& down, int64_t top_k, bool normalize) {
-  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.stride(1) == 1 && aligned16(x) &&
-                  (x.size(0) == 1 || x.stride(0) % 8 == 0), "x must be bf16 [T, H] with 16-byte aligned rows");
-  const int64_t T = x.size(0), H = x.size(1), E = router.size(0);
-  TORCH_CHECK(T <= mts::kMoeTokensMax && H > 0 && H % 8 == 0 && H <= (1 << 20), "moe_tokens takes up to 64 tokens and a hidden size that is a multiple of 8");
-  check_same_device(router, x, "router weight");
-  TORCH_CHECK(router.dim() == 2 && router.size(1) == H && router.is_contiguous() && aligned16(router) &&
-                  (router.scalar_type() == at::kFloat || router.scalar_type() == at::kBFloat16), "router weight must be contiguous fp32 or bf16 [E, H]");
-  TORCH_CHECK(E >= 1 && E <= 64 && top_k >= 1 && top_k <= 8 && top_k <= E, "moe_tokens takes up to 64 experts and top-8");
-  for (const Tensor* w : {&gate_up, &down}) {
-    check_same_device(*w, x, "expert weight");
-    TORCH_CHECK(w->scalar_type() == at::kBFloat16 && w->is_contiguous() && aligned16(*w) && w->dim() == 3 && w->size(0) == E, "expert weights must be contiguous bf16 [E, ., .]");
+  py::object attend(const Tensor& q, int64_t padded, double softmax_scale) const {
+    if (padded <= 0 || q.dim() != 4) return py::none();
+    const int64_t Hq = q.size(1);
+    if (Hq <= 0 || Hq % c.Hkv != 0 || Hq / c.Hkv * padded > (1 << 24) || !covers(q, Hq, padded)) return py::none();
+    if (!mts::cached_attention_fits(c.B, c.Hkv, int(Hq), int(padded), c.D, c.blocks)) return py::none();
+    c10::cuda::CUDAGuard guard(tail.device());
+    mts::CachedAttentionArgs a;
+    a.cache = c;
+    a.Hq = int(Hq); a.T = int(padded);
+    a.q = rows_of(q);
+    a.scale = float(softmax_scale);
+    Tensor o = at::empty({c.B, a.T, Hq, c.D}, q.options()).transpose(1, 2);
+    a.o = o.data_ptr();
+    const size_t floats = mts::cached_attention_workspace_floats(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks);
+    Tensor ws = at::empty({int64_t(floats)}, tail.options().dtype(at::kFloat));
+    a.workspace = ws.data_ptr<float>();
+    a.status = status;
+    a.stream = at::cuda::getCurrentCUDAStream().stream();
+    const cudaError_t e = mts::launch_cached_attention(a);
+    TORCH_CHECK(e == cudaSuccess, "cached_attention failed: ", cudaGetErrorString(e));
+    return py::cast(o);
   }
-  const int64_t I = down.size(2);
-  TORCH_CHECK(I > 0 && I % 8 == 0 && I <= (1 << 20) && down.size(1) == H && gate_up.size(1) == 2 * I && gate_up.size(2) == H,
-              "expert weights must be [E, 2 I, H] and [E, H, I] with I a multiple of 8");
+
+ private:
+  Tensor status_word_;
+  static mts::Strided rows_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+};
+
+// None for inputs that the kernels do not cover.
+py::object moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_up, const Tensor& down, int64_t top_k, bool normalize) {
+  if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() != 2 || router.dim() != 2 || gate_up.dim() != 3 || down.dim() != 3) return py::none();
+  const int64_t T = x.size(0), H = x.size(1), E = router.size(0), I = down.size(2);
+  if (T > mts::kMoeTokensMax || H <= 0 || H % 8 != 0 || H > (1 << 20) || x.stride(1) != 1 || !aligned16(x) || (T > 1 && x.stride(0) % 8 != 0)) return py::none();
+  if (E < 1 || E > 64 || top_k < 1 || top_k > 8 || top_k > E || I <= 0 || I % 8 != 0 || I > (1 << 20)) return py::none();
+  if (router.size(1) != H || (router.scalar_type() != at::kFloat && router.scalar_type() != at::kBFloat16)) return py::none();
+  if (gate_up.size(0) != E || gate_up.size(1) != 2 * I || gate_up.size(2) != H || down.size(0) != E || down.size(1) != H) return py::none();
+  if (gate_up.scalar_type() != at::kBFloat16 || down.scalar_type() != at::kBFloat16) return py::none();
+  for (const Tensor* w : {&router, &gate_up, &down})
+    if (w->device() != x.device() || !w->is_contiguous() || !aligned16(*w)) return py::none();
+  if (at::GradMode::is_enabled() && (x.requires_grad() || router.requires_grad() || gate_up.requires_grad() || down.requires_grad())) return py::none();
   c10::cuda::CUDAGuard guard(x.device());
-  Tensor y = torch::empty({T, H}, x.options());
-  if (T == 0) return y;
-  Tensor hidden = torch::empty({2, T * top_k, I}, x.options()), routes = torch::empty({T * top_k}, x.options().dtype(torch::kInt));
+  Tensor y = at::empty({T, H}, x.options());
+  if (T == 0) return py::cast(y);
+  Tensor hidden = at::empty({2, T * top_k, I}, x.options()), routes = at::empty({T * top_k}, x.options().dtype(at::kInt));
   mts::MoeTokensArgs a;
   a.x = x.data_ptr(); a.ldx = x.stride(0);
   a.router = router.data_ptr(); a.router_bf16 = router.scalar_type() == at::kBFloat16;
@@ -153,14 +158,16 @@ Tensor moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_up, 
   a.stream = at::cuda::getCurrentCUDAStream().stream();
   const cudaError_t e = mts::launch_moe_tokens(a);
   TORCH_CHECK(e == cudaSuccess, "moe_tokens failed: ", cudaGetErrorString(e));
-  return y;
+  return py::cast(y);
 }
 
 }  // namespace
 
 void bind_decode(pybind11::module_& m) {
-  m.def("kv_append", &kv_append);
-  m.def("kv_read", &kv_read);
-  m.def("cached_attention", &cached_attention);
+  py::class_<KvLayer>(m, "KvLayer")
+      .def(py::init<Tensor, Tensor, Tensor, Tensor, Tensor>())
+      .def("append", &KvLayer::append)
+      .def("read", &KvLayer::read)
+      .def("attend", &KvLayer::attend);
   m.def("moe_tokens", &moe_tokens);
 }

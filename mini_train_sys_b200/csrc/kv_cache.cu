@@ -140,11 +140,10 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
       } else if (closes && p < start) {
         klo[it].q = *reinterpret_cast<const uint4*>(tk + tok * D + vec * 8);
         khi[it].q = *reinterpret_cast<const uint4*>(tk + tok * D + D / 2 + vec * 8);
-        const int slot = cache_slot(tok);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          vlo[it].v[j] = tv[(vec * 8 + j) * BLK + slot];
-          vhi[it].v[j] = tv[(D / 2 + vec * 8 + j) * BLK + slot];
+          vlo[it].v[j] = tv[tail_slot(D, vec * 8 + j, tok)];
+          vhi[it].v[j] = tv[tail_slot(D, D / 2 + vec * 8 + j, tok)];
         }
       }
     }
@@ -157,11 +156,10 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
         if (tok >= BLK || p < start || p >= end) continue;
         *reinterpret_cast<uint4*>(tk + tok * D + vec * 8) = klo[it].q;
         *reinterpret_cast<uint4*>(tk + tok * D + D / 2 + vec * 8) = khi[it].q;
-        const int slot = cache_slot(tok);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          tv[(vec * 8 + j) * BLK + slot] = vlo[it].v[j];
-          tv[(D / 2 + vec * 8 + j) * BLK + slot] = vhi[it].v[j];
+          tv[tail_slot(D, vec * 8 + j, tok)] = vlo[it].v[j];
+          tv[tail_slot(D, D / 2 + vec * 8 + j, tok)] = vhi[it].v[j];
         }
       }
       continue;
@@ -184,10 +182,11 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
     const bool k_ok = ka < 0x7f800000u, v_ok = va < 0x7f800000u;
     const float kamax = __uint_as_float(ka), vamax = __uint_as_float(va);
     const float kinv = k_ok && ka != 0 ? __fdiv_rn(127.f, kamax) : 0.f, vinv = v_ok && va != 0 ? __fdiv_rn(127.f, vamax) : 0.f;
-    uint8_t* kc = c.codes + (((long long)bh * c.blocks + blk) * 2) * BLK * D;
+    uint8_t* record = c.records + ((long long)bh * c.blocks + blk) * record_bytes(D);
+    uint8_t* kc = record + kCacheHead;
     uint8_t* vc = kc + BLK * D;
     if (tid == 0) {
-      float* sc = c.scale + ((long long)bh * c.blocks + blk) * 2;
+      float* sc = reinterpret_cast<float*>(record);
       sc[0] = k_ok ? __fdiv_rn(kamax, 127.f) : CUDART_NAN_F;     // a block that holds a NaN or an infinity reads NaN
       sc[1] = v_ok ? __fdiv_rn(vamax, 127.f) : CUDART_NAN_F;
     }
@@ -236,11 +235,12 @@ kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restr
   const bool live = p >= 0 && p < total;
   const int blk = live ? int(p / BLK) : 0, at = live ? int(p % BLK) : 0;
   const bool open = blk == total / BLK;
-  const uint8_t* kc = c.codes + (((long long)bh * c.blocks + blk) * 2) * BLK * D;
+  const uint8_t* record = c.records + ((long long)bh * c.blocks + blk) * record_bytes(D);
+  const uint8_t* kc = record + kCacheHead;
   const T* tk = static_cast<const T*>(c.tail) + ((long long)bh * 2 + (blk & 1)) * 2 * BLK * D;
   float ks = 0.f, vs = 0.f;
   if (live && !open) {
-    const float* sc = c.scale + ((long long)bh * c.blocks + blk) * 2;
+    const float* sc = reinterpret_cast<const float*>(record);
     ks = sc[0];
     vs = sc[1];
   }
@@ -255,7 +255,7 @@ kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restr
       Vec8T<T> x;
       x.q = *reinterpret_cast<const uint4*>(tk + at * D + d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { kf[j] = to_f(x.v[j]); vf[j] = to_f(tk[BLK * D + (d + j) * BLK + slot]); }
+      for (int j = 0; j < 8; ++j) { kf[j] = to_f(x.v[j]); vf[j] = to_f(tk[BLK * D + tail_slot(D, d + j, at)]); }
     } else if (live) {
       const uint2 w = *reinterpret_cast<const uint2*>(kc + at * D + d);
 #pragma unroll

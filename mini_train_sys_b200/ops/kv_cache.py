@@ -19,7 +19,9 @@ from __future__ import annotations
 import torch
 
 BLOCK = 64
-HEAD_DIMS = (32, 64, 128)      # of the native kernels
+HEAD = 16                      # bytes of a record before its codes
+# where a row of values keeps a token: finished blocks, and each half of the unfinished one
+_HALF_SLOT = [((t & 7) >> 1) * 8 + (t >> 4) * 4 + ((t >> 3) & 1) * 2 + (t & 1) for t in range(BLOCK // 2)]
 _SLOT = [((t & 7) >> 1) * 16 + (t >> 4) * 4 + ((t >> 3) & 1) * 2 + (t & 1) for t in range(BLOCK)]
 
 
@@ -36,18 +38,34 @@ class QuantizedKVCache:
         self.layers, self.batch, self.kv_heads, self.head_dim = layers, batch, kv_heads, head_dim
         self.blocks = -(-capacity // BLOCK)
         self.capacity = self.blocks * BLOCK
-        self.dtype, self.device = dtype, torch.device(device)
+        self.dtype = dtype
         lead = (layers, batch, kv_heads)
-        self.codes = torch.full((*lead, self.blocks, 2, BLOCK * head_dim), 128, dtype=torch.uint8, device=device)
-        self.scale = torch.zeros(*lead, self.blocks, 2, dtype=torch.float32, device=device)
+        # a finished block: the fp32 scales of its keys and values, 8 bytes of padding, the codes of its keys and of its values
+        self.records = torch.full((*lead, self.blocks, HEAD + 2 * BLOCK * head_dim), 128, dtype=torch.uint8, device=device)
+        self.records[..., :HEAD] = 0
         self.tail = torch.zeros(*lead, 2, 2, BLOCK * head_dim, dtype=dtype, device=device)
+        self.device = self.records.device
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)     # tokens before the step
         self.counts = torch.zeros(batch, dtype=torch.int32, device=device)      # new tokens of the step
         self.held = 0                   # upper bound of the lengths, known without asking the device
         self.padded: int | None = None  # padded number of new tokens of the open step
 
+        self.native: dict[int, object] = {}     # layers as the native backend holds them
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """``[layers, B, heads, blocks, 2, 64 * D]`` view of the codes (128 stands for zero)."""
+
+        return self.records[..., HEAD:].unflatten(-1, (2, BLOCK * self.head_dim))
+
+    @property
+    def scale(self) -> torch.Tensor:
+        """``[layers, B, heads, blocks, 2]`` view of the scales of keys and values."""
+
+        return self.records[..., :8].view(torch.float32)
+
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.codes, self.scale, self.tail, self.lengths, self.counts))
+        return sum(t.numel() * t.element_size() for t in (self.records, self.tail, self.lengths, self.counts))
 
     def begin(self, count: torch.Tensor | None = None, *, padded: int = 1) -> None:
         """Open a step of up to ``padded`` new tokens per sequence: ``count[b]`` of them, or all of them where it is None."""
@@ -89,10 +107,10 @@ class QuantizedKVCache:
         self.counts.zero_()
         self.held, self.padded = 0, None
 
-    def layer(self, index: int) -> tuple[torch.Tensor, ...]:
+    def check_layer(self, index: int) -> int:
         if not 0 <= index < self.layers:
             raise IndexError(f"cache layer {index} of {self.layers}")
-        return self.codes[index], self.scale[index], self.tail[index], self.lengths, self.counts
+        return index
 
 
 def check_rows(cache: QuantizedKVCache, name: str, x: torch.Tensor, heads: int | None = None, tokens: int | None = None) -> None:
@@ -104,8 +122,8 @@ def check_rows(cache: QuantizedKVCache, name: str, x: torch.Tensor, heads: int |
         raise ValueError(f"{name} must have a multiple of {cache.kv_heads} heads, got {x.shape[1]}")
     if x.dtype != cache.dtype:
         raise ValueError(f"{name} must have the cache's activation type {cache.dtype}, got {x.dtype}")
-    if x.device != cache.codes.device:
-        raise ValueError(f"{name} must be on {cache.codes.device}, got {x.device}")
+    if x.device != cache.device:
+        raise ValueError(f"{name} must be on {cache.device}, got {x.device}")
     if tokens is not None and x.shape[2] != tokens:
         raise ValueError(f"{name} must hold the {tokens} padded tokens of the open step, got {x.shape[2]}")
     if torch.is_grad_enabled() and x.requires_grad:
@@ -137,7 +155,7 @@ def check_attention(cache, q) -> None:
 
 
 def check_read(cache, first, n) -> None:
-    if first.shape != (cache.batch,) or first.dtype != torch.int32 or first.device != cache.codes.device:
+    if first.shape != (cache.batch,) or first.dtype != torch.int32 or first.device != cache.device:
         raise ValueError("first must hold one int32 position per sequence, on the cache's device")
     if n < 0:
         raise ValueError("the number of positions must not be negative")
@@ -167,12 +185,27 @@ def quantize_block(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return (codes + 128).to(torch.uint8), scale[..., 0, 0]
 
 
-def _slots(device) -> torch.Tensor:
-    return torch.tensor(_SLOT, device=device)
+def _pack_values(rows: torch.Tensor, *, tail: bool) -> torch.Tensor:
+    """``[heads, 64, D]`` -> the order in which a record or the tail holds values."""
+
+    heads, _, dim = rows.shape
+    slots = torch.tensor(_HALF_SLOT if tail else _SLOT, device=rows.device)
+    parts = rows.view(heads, -1, len(slots), dim).transpose(2, 3)        # [heads, 1 or 2 halves, D, tokens]
+    out = torch.empty_like(parts, memory_format=torch.contiguous_format)
+    out[..., slots] = parts
+    return out.view(heads, -1)
+
+
+def _unpack_values(flat: torch.Tensor, dim: int, *, tail: bool) -> torch.Tensor:
+    """Inverse of ``_pack_values`` over the last dimension: ``[..., 64 D]`` -> ``[..., 64, D]``."""
+
+    slots = torch.tensor(_HALF_SLOT if tail else _SLOT, device=flat.device)
+    return flat.unflatten(-1, (-1, dim, len(slots)))[..., slots].transpose(-1, -2).flatten(-3, -2)
 
 
 def append_plain(cache: QuantizedKVCache, layer: int, k, v, q=None, cos=None, sin=None):
-    codes, scale, tail, lengths, counts = cache.layer(layer)
+    cache.check_layer(layer)
+    codes, scale, tail, lengths, counts = cache.codes[layer], cache.scale[layer], cache.tail[layer], cache.lengths, cache.counts
     new, dim, heads = k.shape[2], cache.head_dim, cache.kv_heads
     start = lengths.long().clamp(0, cache.capacity)
     t = torch.arange(new, device=k.device)
@@ -188,51 +221,46 @@ def append_plain(cache: QuantizedKVCache, layer: int, k, v, q=None, cos=None, si
         q_out = q
     if q_out is not None:
         q_out = torch.where(live[:, None, :, None], q_out, torch.zeros_like(q_out))
-    slots = _slots(k.device)
     for b in range(cache.batch):
         lo, hi = int(start[b]), int(start[b]) + int(live[b].sum())
         for blk in range(lo // BLOCK, -(-hi // BLOCK) if hi > lo else lo // BLOCK):
             base = blk * BLOCK
             first, last = max(lo, base), min(hi, base + BLOCK)
             held = tail[b, :, blk & 1]
-            blocks = torch.stack((held[:, 0].view(heads, BLOCK, dim), held[:, 1].view(heads, dim, BLOCK)[:, :, slots].transpose(1, 2)), 1).clone()
+            blocks = torch.stack((held[:, 0].view(heads, BLOCK, dim), _unpack_values(held[:, 1], dim, tail=True)), 1)
             blocks[:, 0, first - base:last - base] = k[b, :, first - lo:last - lo]
             blocks[:, 1, first - base:last - base] = v[b, :, first - lo:last - lo]
-            if last < base + BLOCK:
+            open_ = last < base + BLOCK
+            if open_:
                 dest, rows = held, blocks
             else:
                 rows, scales = quantize_block(blocks)
                 dest = codes[b, :, blk]
                 scale[b, :, blk] = scales
-            packed = torch.empty(heads, dim, BLOCK, dtype=rows.dtype, device=k.device)
-            packed[:, :, slots] = rows[:, 1].transpose(1, 2)
             dest[:, 0] = rows[:, 0].reshape(heads, -1)
-            dest[:, 1] = packed.reshape(heads, -1)
+            dest[:, 1] = _pack_values(rows[:, 1], tail=open_)
     return q_out
 
 
 def read_plain(cache: QuantizedKVCache, layer: int, first: torch.Tensor, n: int) -> tuple[torch.Tensor, torch.Tensor]:
-    codes, scale, tail, lengths, counts = cache.layer(layer)
-    total = (lengths.long().clamp(0, cache.capacity) + counts).clamp_max(cache.capacity)
-    dev = codes.device
+    cache.check_layer(layer)
+    dim, dev = cache.head_dim, cache.device
+    total = (cache.lengths.long().clamp(0, cache.capacity) + cache.counts).clamp_max(cache.capacity)
     pos = first.long()[:, None] + torch.arange(n, device=dev)
     live = (pos >= 0) & (pos < total[:, None])
-    safe = torch.where(live, pos, torch.zeros_like(pos))
-    blk, at = safe // BLOCK, safe % BLOCK
-    b = torch.arange(cache.batch, device=dev)[:, None]
-    slot = _slots(dev)[at]
-    shape = (cache.batch, cache.kv_heads, -1, 2)
-    open_ = (blk == (total // BLOCK)[:, None])[..., None, None]
+    pos = torch.where(live, pos, torch.zeros_like(pos))
+    last = total // BLOCK
+    which = torch.arange(cache.batch, device=dev)
+    tail = cache.tail[layer][which, :, last & 1]                          # [B, heads, 2, 64 D]
     out = []
-    for which in range(2):
-        def rows(buf, block_index, which=which):           # -> [B, n, heads, D]
-            if which == 0:
-                return buf.view(*buf.shape[:3], 2, BLOCK, cache.head_dim)[b, :, block_index, 0, at]
-            return buf.view(*buf.shape[:3], 2, cache.head_dim, BLOCK)[b, :, block_index, 1, :, slot]
-        finished = (rows(codes, blk).float() - 128.0) * scale.view(*shape[:2], cache.blocks, 2)[b, :, blk, which][..., None]
-        values = torch.where(open_, rows(tail, blk & 1).float(), finished)
-        values = torch.where(live[..., None, None], values, torch.zeros_like(values))
-        out.append(values.transpose(1, 2).contiguous())
+    for side in range(2):
+        codes, scale = cache.codes[layer][:, :, :, side], cache.scale[layer][:, :, :, side]
+        done = codes.unflatten(-1, (BLOCK, dim)) if side == 0 else _unpack_values(codes, dim, tail=False)
+        done = ((done.float() - 128.0) * scale[..., None, None]).flatten(2, 3)
+        open_ = tail[:, :, side].unflatten(-1, (BLOCK, dim)) if side == 0 else _unpack_values(tail[:, :, side], dim, tail=True)
+        index = pos[:, None, :, None].expand(-1, cache.kv_heads, -1, dim)
+        values = torch.where((pos // BLOCK == last[:, None])[:, None, :, None], open_.float().gather(2, index % BLOCK), done.gather(2, index))
+        out.append(torch.where(live[:, None, :, None], values, torch.zeros_like(values)))
     return out[0], out[1]
 
 

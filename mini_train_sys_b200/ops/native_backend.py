@@ -906,51 +906,60 @@ class NativeOpsBackend(TorchOpsBackend):
         return super().attention(q, k, v, is_causal=is_causal, dropout_p=dropout_p)
 
     # -- decoding step ------------------------------------------------------------------------
-    def _cache_ok(self, cache, *rows) -> bool:
-        return (cache.codes.is_cuda and cache.dtype in (torch.bfloat16, torch.float16) and cache.head_dim in kv_cache.HEAD_DIMS
-                and all(_rows16(t) for t in rows))
+    # The extension checks the inputs and answers None for what the kernels do not cover (other types, head dimensions or
+    # strides, and wrong arguments); the plain form then does the work or says what is wrong.
+    def _native_layer(self, cache, layer):
+        held = cache.native.get(layer)
+        if held is None and 0 <= layer < cache.layers and cache.records.is_cuda and cache.dtype in (torch.bfloat16, torch.float16) \
+                and cache.head_dim in (32, 64, 128):
+            held = ext().KvLayer(cache.records[layer], cache.tail[layer], cache.lengths, cache.counts, ext().status_tensor(cache.device.index))
+            cache.native[layer] = held
+        return held
 
     def kv_append(self, cache, layer, k, v, *, q=None, cos=None, sin=None):
-        kv_cache.check_append(cache, k, v, q, cos, sin)
-        ok = self._cache_ok(cache, k, v, *(() if q is None else (q,)))
-        ok = ok and (cos is None or (cos.is_contiguous() and sin.is_contiguous()))
-        if self._count("kv_append", ok):
-            return ext().kv_append(*cache.layer(layer), k, v, q, cos, sin)
-        return super().kv_append(cache, layer, k, v, q=q, cos=cos, sin=sin)
+        held = cache.native.get(layer) or self._native_layer(cache, layer)
+        if held is not None:
+            padded = cache.padded or 0
+            out = held.append(k, v, q, cos, sin, padded, cache.held + padded)
+            if out is not None:
+                self.dispatch["kv_append:native"] += 1
+                return None if out is True else out
+        out = super().kv_append(cache, layer, k, v, q=q, cos=cos, sin=sin)
+        self.dispatch["kv_append:fallback"] += 1
+        return out
 
     def kv_read(self, cache, layer, first, n):
-        kv_cache.check_read(cache, first, n)
-        if self._count("kv_read", self._cache_ok(cache) and first.is_contiguous()):
-            return tuple(ext().kv_read(*cache.layer(layer), first, n))
-        return super().kv_read(cache, layer, first, n)
+        held = cache.native.get(layer) or self._native_layer(cache, layer)
+        out = held.read(first, n) if held is not None else None
+        if out is not None:
+            self.dispatch["kv_read:native"] += 1
+            return out
+        out = super().kv_read(cache, layer, first, n)
+        self.dispatch["kv_read:fallback"] += 1
+        return out
 
     def cached_attention(self, q, cache, layer):
-        kv_cache.check_attention(cache, q)
-        if self._count("cached_attention", self._cache_ok(cache, q)):
-            return ext().cached_attention(*cache.layer(layer), q, scaled_dot_scale(cache.head_dim))
-        return super().cached_attention(q, cache, layer)
+        held = cache.native.get(layer) or self._native_layer(cache, layer)
+        out = held.attend(q, cache.padded or 0, scaled_dot_scale(cache.head_dim)) if held is not None else None
+        if out is not None:
+            self.dispatch["cached_attention:native"] += 1
+            return out
+        out = super().cached_attention(q, cache, layer)
+        self.dispatch["cached_attention:fallback"] += 1
+        return out
 
     def moe_tokens(self, x, router_weight, gate_up_proj, down_proj, top_k, *, normalize):
-        check_moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k)
-        n_exp, hidden, inter = down_proj.shape
-        weights = (router_weight, gate_up_proj, down_proj)
-        ok = (x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] <= MOE_TOKENS_MAX and hidden % 8 == 0 and inter % 8 == 0
-              and n_exp <= 64 and top_k <= 8 and x.stride(1) == 1 and x.data_ptr() % 16 == 0
-              and (x.shape[0] <= 1 or x.stride(0) % 8 == 0)
-              and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in weights)
-              and all(w.is_contiguous() and w.data_ptr() % 16 == 0 for w in weights))
-        if self._count("moe_tokens", ok):
-            return ext().moe_tokens(x, router_weight.detach(), bf16_weight(gate_up_proj), bf16_weight(down_proj), top_k, bool(normalize))
+        y = ext().moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k, normalize)
+        if y is None:
+            check_moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k)
+            if x.dtype == torch.bfloat16 and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in (gate_up_proj, down_proj)):
+                # fp32 parameters: their bf16 copies, as in the other operators
+                y = ext().moe_tokens(x, router_weight.detach(), bf16_weight(gate_up_proj), bf16_weight(down_proj), top_k, normalize)
+        if y is not None:
+            self.dispatch["moe_tokens:native"] += 1
+            return y
+        self.dispatch["moe_tokens:fallback"] += 1
         return super().moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k, normalize=normalize)
-
-
-MOE_TOKENS_MAX = 64     # of the few-token MoE kernels
-
-
-def _rows16(t: torch.Tensor) -> bool:
-    """``[B, heads, T, D]`` whose rows the kernels can read in 16-byte pieces."""
-
-    return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], t.stride()[:3]))
 
 
 def scaled_dot_scale(head_dim: int) -> float:
