@@ -6,14 +6,16 @@
 // share a K/V head, times the new tokens of the step).  Every warp has a ring of blocks of its own in shared memory, which bulk
 // copies fill (one for the keys of a block with its scales, one for its values), so the warps run without barriers and each
 // keeps 8 to 16 KB of the cache in flight.  A lane's 16 adjacent bytes are its K or V fragment of several steps (the V rows are
-// stored in that order); 4 bytes become two fp16 pairs in four instructions; both products run on m16n8k16 with the tokens (K) or
+// stored in that order); 4 bytes become two fp16 pairs, 1152 too large, in two instructions, and the sums start from what that adds
+// (-1152 times the sum of the query, or of the probabilities, which a product with ones gives); both products run on m16n8k16 with the tokens (K) or
 // the head's dims (V) as rows and eight query rows as columns.  The (sequence, head, row tile, block) units of
 // the whole batch are one list, cut into equal parts for the warps that fit on the machine: sequences of unlike lengths, and a
 // single long one, keep every SM busy, and a warp streams across the ends of sequences.  A second kernel joins the parts of
 // the (sequence, head, row tile) items that were cut.
 // What bounds it: reading the codes, 2 D bytes per token and K/V head.
 //
-// Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
+// Rounding: codes are exact in fp16 (and 1152 more than they are still exact; in fp32 sums it costs 2^-24 of 1152 sum p, for values of
+// about 40).  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
 // queries keep their eight bits in fp16.  Probabilities are rounded to fp16 (2^-11 of each, at a scale of 2^14 so that the
 // smallest kept one is 2^-38 of the largest); the sum of probabilities, the maximum and the output accumulators are fp32.  In
 // the unfinished block, whose values are bf16, a probability is the sum of two bf16 values.
@@ -22,19 +24,23 @@
 #include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
 
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 namespace mts {
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int BLK = kCacheBlock;
 constexpr int kWarps = 4;
-// Resident CTAs an SM: three rings of 64 KB fit; more than eight query rows need the registers of the third.
-__host__ __device__ constexpr int ctas_per_sm(int nq) { return nq == 1 ? 3 : 2; }
+// Resident CTAs an SM: what fits in registers (four with eight query rows) and, at D = 128, in shared memory.
+__host__ __device__ constexpr int ctas_per_sm(int D, int nq) { return nq > 1 ? 2 : D == 128 ? 3 : 4; }
 constexpr int kBatchMax = 2048;          // sequences: their units are counted in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kProbShift = 14.f;       // probabilities are held times 2^14
+constexpr uint32_t kOnes = 0x3C003C00u;  // a pair of fp16 ones
 
 struct Params {
   const uint8_t* records;
@@ -96,7 +102,7 @@ __device__ __forceinline__ int owner(int N, int u, int n) { return int(((long lo
 
 // A stage of a warp's ring: the head of a record (its scales), keys, values, and the query rows of an item that begins.  The codes are
 // 16 KB a warp at any head dimension.
-__host__ __device__ constexpr int ring_stages(int D) { return 128 / D; }
+__host__ __device__ constexpr int ring_stages(int D) { return D < 64 ? 2 : 1; }
 __host__ __device__ constexpr int stage_bytes(int D, int NQ) { return record_bytes(D) + 8 * NQ * D * 2; }
 __host__ __device__ constexpr int shared_bytes(int D, int NQ) {
   const int ring = kWarps * ring_stages(D) * stage_bytes(D, NQ), exchange = kWarps * D * (8 * NQ + 1) * 4;
@@ -127,6 +133,7 @@ __device__ __forceinline__ void read_words(const uint8_t* p, uint32_t (&w)[WORDS
 template <typename T> struct Act;
 template <> struct Act<__nv_bfloat16> {
   static constexpr bool kHalf = false;
+  static constexpr uint32_t kOnes = 0x3F803F80u;
   static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
   static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
@@ -140,6 +147,7 @@ template <> struct Act<__nv_bfloat16> {
 };
 template <> struct Act<__half> {
   static constexpr bool kHalf = true;
+  static constexpr uint32_t kOnes = 0x3C003C00u;
   static __device__ __forceinline__ float lo(uint32_t w) { return __low2float(*reinterpret_cast<const __half2*>(&w)); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __high2float(*reinterpret_cast<const __half2*>(&w)); }
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
@@ -153,47 +161,51 @@ template <> struct Act<__half> {
 // eight rows (the statistics are the same in the eight lanes that share c) and the dims g and g + 8 of every 16.
 template <int D, int NQ>
 struct State {
-  float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];
+  float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];              // l: the sum of the probabilities, complete in every lane
 };
 
-// Scores of 16 M tokens (log2 domain, -inf where masked) -> probabilities as fragments; rescales the state.
-// s[m][n][i]: token 16 m + g + 8 (i >> 1), query 2c + (i & 1) of tile n.
+__device__ __forceinline__ float exp2_fast(float x) {     // 2^x to 2 ulp; 0 below 2^-126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Scores of 16 M tokens, of which `f` times is the logit in the log2 domain (-inf where masked), to probabilities times 2^14;
+// rescales the state.  s[m][n][i]: token 16 m + g + 8 (i >> 1), query 2c + (i & 1) of tile n.
 template <int D, int NQ, int M>
-__device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[M][NQ][4]) {
+__device__ __forceinline__ void update_max(State<D, NQ>& st, float (&s)[M][NQ][4], const float (&f)[NQ][2]) {
   bool moved = false;
   float alpha[NQ][2];
 #pragma unroll
   for (int n = 0; n < NQ; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float mx = -CUDART_INF_F;
+      float mx = fmaxf(s[0][n][j], s[0][n][j + 2]);
 #pragma unroll
-      for (int m = 0; m < M; ++m) mx = fmaxf(mx, fmaxf(s[m][n][j], s[m][n][j + 2]));
+      for (int m = 1; m < M; ++m) mx = fmaxf(mx, fmaxf(s[m][n][j], s[m][n][j + 2]));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      mx = fmaxf(mx, st.m[n][j]);
+      mx = fmaxf(mx * f[n][j], st.m[n][j]);
       const float base = mx == -CUDART_INF_F ? 0.f : mx;     // a row that has seen nothing yet
-      alpha[n][j] = exp2f(st.m[n][j] - base);
+      alpha[n][j] = exp2_fast(st.m[n][j] - base);
       moved |= mx != st.m[n][j];
       st.m[n][j] = mx;
-      const float shift = base - kProbShift;
-      float sum = 0.f;
+      const float shift = kProbShift - base;
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s[m][n][j + 2 * i] = exp2f(s[m][n][j + 2 * i] - shift);
-          sum += s[m][n][j + 2 * i];
-        }
-      st.l[n][j] = st.l[n][j] * alpha[n][j] + sum;           // per lane: summed over the eight g at the end
+        for (int i = 0; i < 2; ++i) s[m][n][j + 2 * i] = exp2_fast(fmaf(s[m][n][j + 2 * i], f[n][j], shift));
     }
   if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) st.l[n][j] *= alpha[n][j];
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[n][d][i] *= alpha[n][i & 1];
+    }
   }
 }
 
@@ -240,8 +252,9 @@ struct Cursor {
   }
 };
 
-template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NQ))
+// CLUSTER: the CTAs of a cluster share one item, else the CTAs of the grid share the list of units.
+template <typename T, int D, int NQ, bool CLUSTER>
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NQ))
 cached_attention_kernel(const Params p) {
   constexpr int KW = D / 16;             // K words per lane and token = steps of 16 dims
   constexpr int DT = D / 16;             // tiles of 16 dims of the output
@@ -258,11 +271,25 @@ cached_attention_kernel(const Params p) {
   float* o_sm = reinterpret_cast<float*>(smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");    // the joining kernel may be set up; it waits for this one's end
-  count_units<kWarps * 32>(p, prefix, scratch);
-  const int N = prefix[p.B];
-  const int c0 = cut(N, blockIdx.x, p.ctas), c1 = cut(N, blockIdx.x + 1, p.ctas);
-  if (c0 == c1) return;
+  Cursor cur;
+  int c0, c1;                            // units of this CTA
+  if constexpr (CLUSTER) {
+    const int shares = int(cg::this_cluster().num_blocks()), item = blockIdx.x / shares, share = blockIdx.x % shares;
+    cur.tile = item % p.row_tiles;
+    cur.h = item / p.row_tiles % p.Hkv;
+    cur.enter(p, item / p.row_tiles / p.Hkv);
+    c0 = cut(cur.units, share, shares);
+    c1 = cut(cur.units, share + 1, shares);
+    cur.at = c0;
+  } else {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may be set up; it waits for this one's end
+    count_units<kWarps * 32>(p, prefix, scratch);
+    const int N = prefix[p.B];
+    c0 = cut(N, blockIdx.x, p.ctas);
+    c1 = cut(N, blockIdx.x + 1, p.ctas);
+    if (c0 == c1) return;
+    cur.seek(p, prefix, c0);
+  }
   const int u0 = c0 + cut(c1 - c0, warp, kWarps), u1 = c0 + cut(c1 - c0, warp + 1, kWarps);
   const int rows = p.group * p.T;
 
@@ -279,12 +306,11 @@ cached_attention_kernel(const Params p) {
     }
   };
   reset();
-  Cursor cur;
-  cur.seek(p, prefix, c0);
   // does the CTA stay within one item?  Then its four warps are joined here and count as one part.
   const int item_begin = c0 - cur.at, item_end = item_begin + cur.units;
-  const bool one_item = c1 <= item_end;
-  if (u0 < u1 && u0 != c0) cur.seek(p, prefix, u0);
+  const bool one_item = CLUSTER || c1 <= item_end;
+  if constexpr (CLUSTER) cur.at = u0;
+  else if (u0 < u1 && u0 != c0) cur.seek(p, prefix, u0);
 
   if (u0 < u1) {
     uint8_t* ring = smem + warp * (STAGES * STAGE);
@@ -352,6 +378,7 @@ cached_attention_kernel(const Params p) {
 
     uint32_t qf[NQ][KW][2];              // fp16 query fragments, scaled: column g of every tile, dims 4 KW c ... of the head
     float qscale[NQ][2];                 // log2(e) / sqrt(D) times the power of two taken out, for the columns 2c, 2c + 1
+    float qbias[NQ][2];                  // -1152 times the sum of the scaled query
     int limit[NQ][2];                    // last position that a column sees
     int start = 0, fresh = 0;
     int stage = 0;
@@ -390,6 +417,11 @@ cached_attention_kernel(const Params p) {
               qf[n][i][j] = Act<T>::kHalf ? w[2 * i + j] : pack_half2(Act<T>::lo(w[2 * i + j]) * down, Act<T>::hi(w[2 * i + j]) * down);
 #pragma unroll
           for (int j = 0; j < 2; ++j) qscale[n][j] = p.sm_log2 * __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < KW; ++i) mma_f16(sum, kOnes, kOnes, kOnes, kOnes, qf[n][i][0], qf[n][i][1]);
+          qbias[n][0] = -kCodeBias * sum[0];
+          qbias[n][1] = -kCodeBias * sum[1];
         }
       }
       if (cur.at < cur.closed) {
@@ -399,43 +431,48 @@ cached_attention_kernel(const Params p) {
         const float2 sc = *reinterpret_cast<const float2*>(here);
         float s[4][NQ][4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          uint32_t kr[2][KW];
+        for (int m0 = 0; m0 < 4; m0 += 2) {                  // two token tiles at a time: two chains of products
+          uint32_t kr[2][2][KW];
 #pragma unroll
-          for (int v = 0; v < 2; ++v) read_words<KW>(kst + (16 * m + 8 * v) * D, kr[v]);
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+            for (int v = 0; v < 2; ++v) read_words<KW>(kst + (16 * (m0 + m) + 8 * v) * D, kr[m][v]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[m][n][i] = 0.f;
+          for (int i = 0; i < KW; ++i)
 #pragma unroll
-          for (int i = 0; i < KW; ++i) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_half(kr[0][i], a0, a2);
-            codes_to_half(kr[1][i], a1, a3);
+            for (int m = 0; m < 2; ++m) {
+              uint32_t a0, a1, a2, a3;
+              codes_to_half(kr[m][0][i], a0, a2);
+              codes_to_half(kr[m][1][i], a1, a3);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) mma_f16(s[m][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
-          }
+              for (int n = 0; n < NQ; ++n) {
+                const float from[4] = {qbias[n][0], qbias[n][1], qbias[n][0], qbias[n][1]};
+                if (i == 0) mma_f16_from(s[m0 + m][n], from, a0, a1, a2, a3, qf[n][0][0], qf[n][0][1]);
+                else mma_f16(s[m0 + m][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+              }
+            }
         }
         copy_k(stage);
+        float f[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float f = qscale[n][j] * sc.x;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) { s[m][n][j] *= f; s[m][n][j + 2] *= f; }
-          }
+          for (int j = 0; j < 2; ++j) f[n][j] = qscale[n][j] * sc.x;
         const bool masked = base + BLK > start;              // blocks of the step itself: rows see different lengths
         if (masked) {
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+          for (int n = 0; n < NQ; ++n) {
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (base + 16 * m + g + 8 * (i >> 1) > limit[n][i & 1]) s[m][n][i] = -CUDART_INF_F;
+              for (int i = 0; i < 4; ++i) {
+                const bool seen = base + 16 * m + g + 8 * (i >> 1) <= limit[n][i & 1];
+                s[m][n][i] = seen ? s[m][n][i] * f[n][i & 1] : -CUDART_INF_F;
+              }
+            f[n][0] = f[n][1] = 1.f;                         // a scale of 0 would make a NaN of -inf
+          }
         }
-        update_max<D, NQ, 4>(st, s);
+        update_max<D, NQ, 4>(st, s, f);
         uint32_t pf[4][NQ][2];
 #pragma unroll
         for (int m = 0; m < 4; ++m)
@@ -444,30 +481,46 @@ cached_attention_kernel(const Params p) {
             pf[m][n][0] = transpose8x8(pack_half2(s[m][n][0], s[m][n][1]));
             pf[m][n][1] = transpose8x8(pack_half2(s[m][n][2], s[m][n][3]));
           }
+        float vbias[NQ][4];                                  // -1152 times the sum of the rounded probabilities
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int m = 0; m < 4; ++m) mma_f16(sum, kOnes, kOnes, kOnes, kOnes, pf[m][n][0], pf[m][n][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vbias[n][i] = -kCodeBias * sum[i & 1];
+          st.l[n][0] += sum[0];
+          st.l[n][1] += sum[1];
+        }
         arrive(stage, 1, parity);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          uint32_t vr[2][4];
+        for (int d0 = 0; d0 < DT; d0 += 2) {
+          uint32_t vr[2][2][4];
 #pragma unroll
-          for (int v = 0; v < 2; ++v) read_words<4>(vst + (16 * d + 8 * v) * BLK, vr[v]);
-          float acc[NQ][4];
+          for (int d = 0; d < 2; ++d)
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+            for (int v = 0; v < 2; ++v) read_words<4>(vst + (16 * (d0 + d) + 8 * v) * BLK, vr[d][v]);
+          float acc[2][NQ][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+          for (int m = 0; m < 4; ++m)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_half(vr[0][m], a0, a2);
-            codes_to_half(vr[1][m], a1, a3);
+            for (int d = 0; d < 2; ++d) {
+              uint32_t a0, a1, a2, a3;
+              codes_to_half(vr[d][0][m], a0, a2);
+              codes_to_half(vr[d][1][m], a1, a3);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) mma_f16(acc[n], a0, a1, a2, a3, pf[m][n][0], pf[m][n][1]);
-          }
+              for (int n = 0; n < NQ; ++n) {
+                if (m == 0) mma_f16_from(acc[d][n], vbias[n], a0, a1, a2, a3, pf[0][n][0], pf[0][n][1]);
+                else mma_f16(acc[d][n], a0, a1, a2, a3, pf[m][n][0], pf[m][n][1]);
+              }
+            }
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+          for (int d = 0; d < 2; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)    // a block that a row does not see at all must not reach it through its scale
-              if (!masked || base <= limit[n][i & 1]) st.o[n][d][i] = fmaf(acc[n][i], sc.y, st.o[n][d][i]);
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)  // a block that a row does not see at all must not reach it through its scale
+                if (!masked || base <= limit[n][i & 1]) st.o[n][d0 + d][i] = fmaf(acc[d][n][i], sc.y, st.o[n][d0 + d][i]);
         }
         copy_v(stage);
       } else {                             // ---- half of the unfinished block, in the activation type ----
@@ -501,7 +554,10 @@ cached_attention_kernel(const Params p) {
           }
         }
         copy_k(stage);
-        update_max<D, NQ, 2>(st, s);
+        float one[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) one[n][0] = one[n][1] = 1.f;
+        update_max<D, NQ, 2>(st, s, one);
         arrive(stage, 1, parity);
         uint32_t ph[2][NQ][2], pl[2][NQ][2], keep[2][2];
 #pragma unroll
@@ -522,6 +578,19 @@ cached_attention_kernel(const Params p) {
           const int left = valid - 16 * m - 2 * c;           // tokens 16 m + 2c + {0, 1, 8, 9} of this lane that exist
           keep[m][0] = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
           keep[m][1] = left >= 10 ? 0xFFFFFFFFu : left == 9 ? 0xFFFFu : 0u;
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            constexpr uint32_t ones = Act<T>::kOnes;
+            const uint32_t f[4] = {ones, ones, ones, ones};
+            Act<T>::mma(sum, f, ph[m][n][0], ph[m][n][1]);
+            if (!Act<T>::kHalf) Act<T>::mma(sum, f, pl[m][n][0], pl[m][n][1]);
+          }
+          st.l[n][0] += sum[0];
+          st.l[n][1] += sum[1];
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -552,9 +621,7 @@ cached_attention_kernel(const Params p) {
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float l = st.l[n][j];
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            const float l = st.l[n][j];
             const int r = n * 8 + 2 * c + j, row = row0 + r;
             if (row >= fresh * p.group) continue;
             const int t = row / p.group, head = cur.h * p.group + row % p.group;
@@ -583,17 +650,13 @@ cached_attention_kernel(const Params p) {
 
   // ---- join the warps ----
   __syncthreads();                       // the rings are read; their memory takes the outputs
-  if (u0 == u1) cur.seek(p, prefix, c0);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float l = st.l[n][j];
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
       if (g == 0) {
         ml_sm[warp][n * 8 + 2 * c + j][0] = st.m[n][j];
-        ml_sm[warp][n * 8 + 2 * c + j][1] = l;
+        ml_sm[warp][n * 8 + 2 * c + j][1] = st.l[n][j];
       }
     }
 #pragma unroll
@@ -604,6 +667,7 @@ cached_attention_kernel(const Params p) {
   __syncthreads();
   const int live = span_of(p, cur.b).y * p.group, row0 = cur.tile * ROWS;
   const bool whole = c0 == item_begin && c1 == item_end;
+  float* result = reinterpret_cast<float*>(smem + shared_bytes(D, NQ));                  // [ROWS][D + 2] of this CTA, where the counts would be
   for (int i = threadIdx.x; i < ROWS * D; i += kWarps * 32) {
     const int r = i / D, d = i % D, row = row0 + r;
     if (row >= live) break;
@@ -618,7 +682,11 @@ cached_attention_kernel(const Params p) {
       l = fmaf(ml_sm[w][r][1], a, l);
       o = fmaf(o_sm[w * (D * OP) + d * OP + r], a, o);
     }
-    if (whole) {
+    if (CLUSTER) {
+      float* dst = result + r * (D + 2);
+      dst[d] = o;
+      if (d == 0) { dst[D] = m; dst[D + 1] = l; }
+    } else if (whole) {
       const int t = row / p.group, head = cur.h * p.group + row % p.group;
       static_cast<T*>(p.o)[(((long long)cur.b * p.T + t) * p.Hq + head) * D + d] = Act<T>::from(o / l);
     } else {
@@ -626,6 +694,30 @@ cached_attention_kernel(const Params p) {
       dst[d] = o;
       if (d == 0) { dst[D] = m; dst[D + 1] = l; }
     }
+  }
+  if constexpr (CLUSTER) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int shares = int(cluster.num_blocks());
+    cluster.sync();
+    for (int i = int(cluster.block_rank()) * (kWarps * 32) + threadIdx.x; i < ROWS * D; i += shares * kWarps * 32) {
+      const int r = i / D, d = i % D, row = row0 + r;
+      if (row >= rows) break;
+      const int t = row / p.group, head = cur.h * p.group + row % p.group;
+      float l = 0.f, o = 0.f;
+      if (row < live) {
+        float m = -CUDART_INF_F;
+        for (int k = 0; k < shares; ++k) m = fmaxf(m, cluster.map_shared_rank(result, k)[r * (D + 2) + D]);
+        const float base = m == -CUDART_INF_F ? 0.f : m;
+        for (int k = 0; k < shares; ++k) {
+          const float* part = cluster.map_shared_rank(result, k) + r * (D + 2);
+          const float a = exp2f(part[D] - base);
+          l = fmaf(part[D + 1], a, l);
+          o = fmaf(part[d], a, o);
+        }
+      }
+      static_cast<T*>(p.o)[(((long long)cur.b * p.T + t) * p.Hq + head) * D + d] = Act<T>::from(row < live ? o / l : 0.f);
+    }
+    cluster.sync();                      // nobody leaves while its result may still be read
   }
 }
 
@@ -651,6 +743,7 @@ join_parts_kernel(const Params p, int rows_per_tile) {
   T* out = static_cast<T*>(p.o) + (((long long)b * p.T + t) * p.Hq + head) * D;
   const int2 span = span_of(p, b);
   if (t >= span.y) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");     // this grid's end has to mean the other's end too
     for (int d = threadIdx.x; d < D; d += kJoinThreads) out[d] = Act<T>::from(0.f);
     return;
   }
@@ -708,11 +801,11 @@ join_parts_kernel(const Params p, int rows_per_tile) {
   float o[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) o[j] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = warp; k < candidates; k += kJoinThreads / 32) {
-    if (slot[k] < 0) continue;
+    const int at = slot[k];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) o[j] = fmaf(src[slot[k] * pitch + j * 32 + lane], weight[k], o[j]);
+    for (int j = 0; j < PER; ++j) o[j] = fmaf(at >= 0 ? src[at * pitch + j * 32 + lane] : 0.f, weight[k], o[j]);
   }
 #pragma unroll
   for (int j = 0; j < PER; ++j) o_sm[warp][j * 32 + lane] = o[j];
@@ -726,21 +819,25 @@ join_parts_kernel(const Params p, int rows_per_tile) {
 }
 
 struct Plan {
-  int nq, row_tiles, ctas;
+  int nq, row_tiles, ctas, cluster;      // cluster: 0 for the list of units
 };
 
-// Query rows in tiles of 8, 16 or 32 (16 at D = 128, where the accumulators of 32 would not fit in registers); as many CTAs as are
-// resident at once, or as there can be units for.  The capacity decides, not the lengths, which only the device knows.
+// Query rows in tiles of 8 to 32 (16 at D = 128, where the accumulators of 32 would not fit in registers).  Where a cluster of up to
+// eight CTAs has at most two blocks a warp and all clusters fit on the machine, an item is the work of one cluster, which joins its
+// parts through distributed shared memory: one launch, no counting of units.  Otherwise as many CTAs as are resident at once, or as
+// there can be units for.  The capacity decides, not the lengths, which only the device knows.
 Plan plan_for(int B, int Hkv, int Hq, int T, int D, int blocks) {
   Plan pl;
   const int rows = Hq / Hkv * T, most = D == 128 ? 2 : 4;
-  pl.nq = rows <= 8 ? 1 : rows <= 16 ? 2 : most;
+  pl.nq = (rows + 7) / 8 < most ? (rows + 7) / 8 : most;
   pl.row_tiles = (rows + 8 * pl.nq - 1) / (8 * pl.nq);
   const long long units = (long long)B * Hkv * pl.row_tiles * blocks;
-  // the third ring of a CTA leaves little room for the counts of many sequences
-  const int resident = B <= 160 ? ctas_per_sm(pl.nq) : 2;
-  const long long slots = (long long)device_sm_count() * resident;
-  pl.ctas = int(units < slots ? units : slots);
+  const long long slots = (long long)device_sm_count() * ctas_per_sm(D, pl.nq), items = units / blocks;
+  int cluster = 1;
+  while (cluster < 8 && cluster * kWarps < blocks) cluster *= 2;
+  while (cluster > 1 && items * cluster > slots) cluster /= 2;
+  pl.cluster = blocks <= 2 * kWarps * cluster && items * cluster <= slots ? cluster : 0;
+  pl.ctas = int(pl.cluster > 0 ? items * cluster : units < slots ? units : slots);
   return pl;
 }
 
@@ -757,36 +854,50 @@ cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool> (&ready)[64]) {
 }
 
 template <typename T, int D, int NQ>
-cudaError_t launch_typed(const Params& p, cudaStream_t stream) {
-  static std::atomic<bool> ready[64];
+cudaError_t launch_typed(const Params& p, int cluster, cudaStream_t stream) {
   const int bytes = shared_bytes(D, NQ);
-  cudaError_t err = allow_shared(cached_attention_kernel<T, D, NQ>, bytes + (kBatchMax + 1) * 4, ready);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.ctas));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cluster > 0) {
+    static std::atomic<bool> ready[64];
+    cfg.dynamicSmemBytes = size_t(bytes) + 8 * NQ * (D + 2) * 4;
+    const cudaError_t err = allow_shared(cached_attention_kernel<T, D, NQ, true>, int(cfg.dynamicSmemBytes), ready);
+    if (err != cudaSuccess) return err;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    ++g_launch_count;
+    return cudaLaunchKernelEx(&cfg, cached_attention_kernel<T, D, NQ, true>, p);
+  }
+  static std::atomic<bool> ready[64];
+  cudaError_t err = allow_shared(cached_attention_kernel<T, D, NQ, false>, bytes + (kBatchMax + 1) * 4, ready);
   if (err != cudaSuccess) return err;
   const long long rows = (long long)p.B * p.Hkv * p.group * p.T;
   if (rows > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  cached_attention_kernel<T, D, NQ><<<unsigned(p.ctas), kWarps * 32, bytes + (p.B + 1) * 4, stream>>>(p);
+  cfg.dynamicSmemBytes = size_t(bytes) + (p.B + 1) * 4;
+  cfg.numAttrs = 0;
   ++g_launch_count;
-  if ((err = cudaGetLastError()) != cudaSuccess) return err;
-  cudaLaunchConfig_t cfg = {};
+  if ((err = cudaLaunchKernelEx(&cfg, cached_attention_kernel<T, D, NQ, false>, p)) != cudaSuccess) return err;
   cfg.gridDim = dim3(unsigned(rows));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = size_t(p.B + 1 + 2 * (p.ctas + 2 * kWarps)) * 4;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 1;
-  err = cudaLaunchKernelEx(&cfg, join_parts_kernel<T, D>, p, 8 * NQ);
   ++g_launch_count;
-  return err;
+  return cudaLaunchKernelEx(&cfg, join_parts_kernel<T, D>, p, 8 * NQ);
 }
 
 template <typename T, int D>
 cudaError_t launch_dim(const Params& p, const Plan& pl, cudaStream_t stream) {
-  if (pl.nq == 1) return launch_typed<T, D, 1>(p, stream);
-  if (pl.nq == 2) return launch_typed<T, D, 2>(p, stream);
-  if constexpr (D != 128) return launch_typed<T, D, 4>(p, stream);
+  if (pl.nq == 1) return launch_typed<T, D, 1>(p, pl.cluster, stream);
+  if (pl.nq == 2) return launch_typed<T, D, 2>(p, pl.cluster, stream);
+  if constexpr (D != 128) return pl.nq == 3 ? launch_typed<T, D, 3>(p, pl.cluster, stream) : launch_typed<T, D, 4>(p, pl.cluster, stream);
   return cudaErrorInvalidValue;
 }
 
@@ -799,13 +910,14 @@ bool cached_attention_fits(int B, int Hkv, int Hq, int T, int D, int blocks) {
 
 size_t cached_attention_workspace_floats(int B, int Hkv, int Hq, int T, int D, int blocks) {
   const Plan pl = plan_for(B, Hkv, Hq, T, D, blocks);
-  return size_t(2) * pl.ctas * kWarps * (8 * pl.nq) * (D + 2);
+  return pl.cluster > 0 ? 0 : size_t(2) * pl.ctas * kWarps * (8 * pl.nq) * (D + 2);
 }
 
 cudaError_t launch_cached_attention(const CachedAttentionArgs& a) {
   const CacheView& c = a.cache;
-  if (a.workspace == nullptr || !cached_attention_fits(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks)) return cudaErrorInvalidValue;
+  if (!cached_attention_fits(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks)) return cudaErrorInvalidValue;
   const Plan pl = plan_for(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks);
+  if (pl.cluster == 0 && a.workspace == nullptr) return cudaErrorInvalidValue;
   Params p;
   p.records = c.records; p.tail = c.tail; p.start = c.start; p.count = c.count;
   p.B = c.B; p.Hkv = c.Hkv; p.blocks = c.blocks; p.Hq = a.Hq; p.T = a.T; p.group = a.Hq / c.Hkv;

@@ -52,7 +52,7 @@ struct CachedAttentionArgs {
   void* o;               // [B, T, Hq, D] storage
   int Hq, T;
   float scale;
-  float* workspace;      // cached_attention_workspace_floats(...) floats
+  float* workspace;      // cached_attention_workspace_floats(...) floats; null when that is 0
   int* status;           // raised to STATUS_WAIT_TIMEOUT by a wait that gives up
   cudaStream_t stream;
 };

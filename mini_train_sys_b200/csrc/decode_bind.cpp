@@ -118,8 +118,9 @@ struct KvLayer {
     Tensor o = at::empty({c.B, a.T, Hq, c.D}, q.options()).transpose(1, 2);
     a.o = o.data_ptr();
     const size_t floats = mts::cached_attention_workspace_floats(c.B, c.Hkv, a.Hq, a.T, c.D, c.blocks);
-    Tensor ws = at::empty({int64_t(floats)}, tail.options().dtype(at::kFloat));
-    a.workspace = ws.data_ptr<float>();
+    Tensor ws;
+    if (floats > 0) ws = at::empty({int64_t(floats)}, tail.options().dtype(at::kFloat));
+    a.workspace = floats > 0 ? ws.data_ptr<float>() : nullptr;
     a.status = status;
     a.stream = at::cuda::getCurrentCUDAStream().stream();
     const cudaError_t e = mts::launch_cached_attention(a);
