@@ -70,12 +70,13 @@ struct MoeTokensArgs {
   const void* gate_up;   // [E, 2 I, H] bf16
   const void* down;      // [E, H, I] bf16
   void* y;               // [T, H] bf16, contiguous
-  void* hidden;          // workspace: [2, T * K, I] bf16
-  int* routes;           // workspace: [T * K] expert of every route
+  void* workspace;       // moe_tokens_workspace_bytes(...), 256-byte aligned
+  int* status;           // raised to STATUS_WAIT_TIMEOUT by a wait that gives up
   int T, E, K, H, I;
   bool normalize;
   cudaStream_t stream;
 };
+size_t moe_tokens_workspace_bytes(int T, int K, int H, int I);
 cudaError_t launch_moe_tokens(const MoeTokensArgs& a);
 
 }  // namespace mts

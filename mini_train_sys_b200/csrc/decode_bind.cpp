@@ -134,7 +134,8 @@ struct KvLayer {
 };
 
 // None for inputs that the kernels do not cover.
-py::object moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_up, const Tensor& down, int64_t top_k, bool normalize) {
+py::object moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_up, const Tensor& down, int64_t top_k, bool normalize,
+                      const Tensor& status) {
   if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() != 2 || router.dim() != 2 || gate_up.dim() != 3 || down.dim() != 3) return py::none();
   const int64_t T = x.size(0), H = x.size(1), E = router.size(0), I = down.size(2);
   if (T > mts::kMoeTokensMax || H <= 0 || H % 8 != 0 || H > (1 << 20) || x.stride(1) != 1 || !aligned16(x) || (T > 1 && x.stride(0) % 8 != 0)) return py::none();
@@ -148,12 +149,13 @@ py::object moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_
   c10::cuda::CUDAGuard guard(x.device());
   Tensor y = at::empty({T, H}, x.options());
   if (T == 0) return py::cast(y);
-  Tensor hidden = at::empty({2, T * top_k, I}, x.options()), routes = at::empty({T * top_k}, x.options().dtype(at::kInt));
+  check_ints(status, 4, x, "status");
+  Tensor ws = at::empty({int64_t(mts::moe_tokens_workspace_bytes(int(T), int(top_k), int(H), int(I)))}, x.options().dtype(at::kByte));
   mts::MoeTokensArgs a;
   a.x = x.data_ptr(); a.ldx = x.stride(0);
   a.router = router.data_ptr(); a.router_bf16 = router.scalar_type() == at::kBFloat16;
   a.gate_up = gate_up.data_ptr(); a.down = down.data_ptr(); a.y = y.data_ptr();
-  a.hidden = hidden.data_ptr(); a.routes = routes.data_ptr<int>();
+  a.workspace = ws.data_ptr(); a.status = status.data_ptr<int>();
   a.T = int(T); a.E = int(E); a.K = int(top_k); a.H = int(H); a.I = int(I);
   a.normalize = normalize;
   a.stream = at::cuda::getCurrentCUDAStream().stream();

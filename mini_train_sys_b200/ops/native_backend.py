@@ -948,13 +948,17 @@ class NativeOpsBackend(TorchOpsBackend):
         self.dispatch["cached_attention:fallback"] += 1
         return out
 
+    def _status(self, x):
+        return ext().status_tensor(x.device.index) if x.is_cuda else None
+
     def moe_tokens(self, x, router_weight, gate_up_proj, down_proj, top_k, *, normalize):
-        y = ext().moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k, normalize)
+        status = self._status(x)
+        y = ext().moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k, normalize, status) if status is not None else None
         if y is None:
             check_moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k)
-            if x.dtype == torch.bfloat16 and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in (gate_up_proj, down_proj)):
+            if status is not None and x.dtype == torch.bfloat16 and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in (gate_up_proj, down_proj)):
                 # fp32 parameters: their bf16 copies, as in the other operators
-                y = ext().moe_tokens(x, router_weight.detach(), bf16_weight(gate_up_proj), bf16_weight(down_proj), top_k, normalize)
+                y = ext().moe_tokens(x, router_weight.detach(), bf16_weight(gate_up_proj), bf16_weight(down_proj), top_k, normalize, status)
         if y is not None:
             self.dispatch["moe_tokens:native"] += 1
             return y
