@@ -22,6 +22,7 @@
 #include "decode.cuh"
 #include "ops.cuh"
 #include "mma_sync.cuh"
+#include "parts.cuh"
 #include "ptx_sm100.cuh"
 
 #include <cooperative_groups.h>
@@ -95,10 +96,6 @@ __device__ __forceinline__ void count_units(const Params& p, int* prefix, int* s
     __syncthreads();
   }
 }
-
-// The list of N units in equal parts: part i of n begins at unit cut(N, i, n), and unit u is in part owner(N, u, n).
-__device__ __forceinline__ int cut(int N, int i, int n) { return int((long long)N * i / n); }
-__device__ __forceinline__ int owner(int N, int u, int n) { return int(((long long)(u + 1) * n - 1) / N); }
 
 // A stage of a warp's ring: the head of a record (its scales), keys, values, and the query rows of an item that begins.  The codes are
 // 16 KB a warp at any head dimension.
@@ -278,19 +275,20 @@ cached_attention_kernel(const Params p) {
     cur.tile = item % p.row_tiles;
     cur.h = item / p.row_tiles % p.Hkv;
     cur.enter(p, item / p.row_tiles / p.Hkv);
-    c0 = cut(cur.units, share, shares);
-    c1 = cut(cur.units, share + 1, shares);
+    const Parts parts(cur.units, shares);
+    c0 = parts.begin(share);
+    c1 = parts.begin(share + 1);
     cur.at = c0;
   } else {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining kernel may be set up; it waits for this one's end
     count_units<kWarps * 32>(p, prefix, scratch);
-    const int N = prefix[p.B];
-    c0 = cut(N, blockIdx.x, p.ctas);
-    c1 = cut(N, blockIdx.x + 1, p.ctas);
+    const Parts parts(prefix[p.B], p.ctas);
+    c0 = parts.begin(blockIdx.x);
+    c1 = parts.begin(blockIdx.x + 1);
     if (c0 == c1) return;
     cur.seek(p, prefix, c0);
   }
-  const int u0 = c0 + cut(c1 - c0, warp, kWarps), u1 = c0 + cut(c1 - c0, warp + 1, kWarps);
+  const int u0 = c0 + part_begin<kWarps>(c1 - c0, warp), u1 = c0 + part_begin<kWarps>(c1 - c0, warp + 1);
   const int rows = p.group * p.T;
 
   State<D, NQ> st;
@@ -748,9 +746,9 @@ join_parts_kernel(const Params p, int rows_per_tile) {
     return;
   }
   count_units<kJoinThreads>(p, prefix, scratch);
-  const int N = prefix[p.B];
+  const Parts parts(prefix[p.B], p.ctas);
   const int begin = prefix[b] + (h * p.row_tiles + row / rows_per_tile) * units_of(span), end = begin + units_of(span);
-  const int i0 = owner(N, begin, p.ctas), i1 = owner(N, end - 1, p.ctas);
+  const int i0 = parts.owner(begin), i1 = parts.owner(end - 1);
   // candidates: the warps of the first and of the last CTA, and one part of every CTA between (those lie within the item)
   const int between = max(i1 - i0 - 1, 0), candidates = kWarps + (i1 > i0 ? between + kWarps : 0);
   asm volatile("griddepcontrol.wait;" ::: "memory");       // everything above read only what the caller wrote
@@ -761,13 +759,13 @@ join_parts_kernel(const Params p, int rows_per_tile) {
   for (int k = threadIdx.x; k < candidates; k += kJoinThreads) {
     const int i = k < kWarps ? i0 : k < kWarps + between ? i0 + 1 + k - kWarps : i1;
     const int w = k < kWarps ? k : k < kWarps + between ? 0 : k - kWarps - between;
-    const int c0 = cut(N, i, p.ctas), c1 = cut(N, i + 1, p.ctas);
+    const int c0 = parts.begin(i), c1 = parts.begin(i + 1);
     int at = -1;
     if (c0 >= begin && c1 <= end) {                        // within the item: its warps are one part
       if (w == 0 && c0 < c1) at = 2 * i * kWarps;
       whole |= c0 == begin && c1 == end;
     } else {
-      const int x0 = c0 + cut(c1 - c0, w, kWarps), x1 = c0 + cut(c1 - c0, w + 1, kWarps);
+      const int x0 = c0 + part_begin<kWarps>(c1 - c0, w), x1 = c0 + part_begin<kWarps>(c1 - c0, w + 1);
       if (x0 < end && x1 > begin && x0 < x1) {
         at = 2 * (i * kWarps + w) + (x0 <= begin ? 1 : 0);
         whole |= x0 <= begin && x1 >= end;

@@ -5,13 +5,13 @@
 //
 // What bounds it: reading the weights of every expert that has a token, 6 H I bytes each, once.  Weight rows are the row operand of
 // m16n8k16 and the tokens of their expert the columns (8 at a time), so one pass over the weights serves up to 64 tokens.  Every warp
-// streams its own weight tiles through a ring in shared memory, 4 KB a TMA copy and 16 or 20 KB in flight a warp, across the ends of
-// items: 128 to 160 KB in flight an SM, and no barrier between warps inside a stream.
+// streams its own weight tiles through a ring in shared memory, 8 KB a TMA copy and 16 or 24 KB in flight a warp, across the ends of
+// items: 128 to 192 KB in flight an SM, and no barrier between warps inside a stream.
 //   1  every CTA (or cluster, where the router is large) routes all tokens for itself; then a warp takes (expert, 8 columns of the
 //      hidden layer) items: 8 gate rows and 8 up rows are one tile, so a lane ends up with both factors of its hidden values and
 //      applies SwiGLU in registers.  The hidden value is multiplied by the route's weight, so that the sums of the second
 //      kernel are over the experts already.
-//   2  the (32 output rows, expert, 64 columns) units of the down projections are one list, cut into equal parts for the CTAs; what
+//   2  the (32 output rows, expert, 128 columns) units of the down projections are one list, cut into equal parts for the CTAs; what
 //      a CTA has of a row tile is added in shared memory, and where a tile was cut its last CTA adds the parts, in order.
 //
 // Rounding: logits, softmax, sums and the hidden values are fp32 (the router's fp32 weight enters the tensor cores as the sum of three
@@ -19,6 +19,7 @@
 #include "decode.cuh"
 #include "ops.cuh"
 #include "mma_sync.cuh"
+#include "parts.cuh"
 #include "ptx_sm100.cuh"
 
 #include <cooperative_groups.h>
@@ -38,21 +39,25 @@ constexpr int kTopK = 8;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRoutes = kMoeTokensMax * kTopK;
-constexpr int kTile = 4096;              // bytes of a copy: 16 rows x 128 columns (gate and up), 32 x 64 (down)
-constexpr int kUpCols = 128, kUpRows = 8, kDownCols = 64, kDownRows = 32;
-constexpr int kStagesMax = 5;
+constexpr int kTile = 8192;              // bytes of a copy: 16 rows x 256 columns (8 gate, 8 up rows), 32 x 128 (down)
+constexpr int kUpCols = 256, kUpRows = 8, kDownCols = 128, kDownRows = 32;
+constexpr int kColumns = 32;             // tokens of an entry: four products of eight
+constexpr int kEntries = kExperts + kRoutes / kColumns;
 constexpr int kSumPitch = kDownRows + 1;
-// Five stages of ring a warp, four where the sums of more than 32 tokens need the room.
-__host__ __device__ constexpr int ring_stages(int T) { return T > 32 ? 4 : 5; }
-__host__ __device__ constexpr int ring_bytes(int T) { return kWarps * ring_stages(T) * kTile; }
+// Stages of a warp's ring in the first kernel, and in the second, whose sums need room too.
+constexpr int kUpStages = 3;
+__host__ __device__ constexpr int down_stages(int T) { return T <= 16 ? 3 : 2; }
+constexpr int kUpRing = kWarps * kUpStages * kTile;
 
-// Routes by expert: `order` holds the routes of expert e, ascending, at [first[e], first[e + 1]); `active` the experts with one.
+// The routes sorted by expert, and the entries that the weights are streamed for: an expert with at most kColumns of its tokens (one
+// with more has several and is read as often).
 struct Routing {
-  int expert[kRoutes];
-  int order[kRoutes];
+  int expert[kRoutes];         // of a route, as chosen
+  int order[kRoutes];          // routes by expert, ascending
+  int token[kRoutes];          // of the routes in order
   int first[kExperts + 1];
-  int active[kExperts];
-  int num_active;
+  int entry_expert[kEntries], entry_begin[kEntries], entry_tokens[kEntries];
+  int entries;
 };
 
 struct Params {
@@ -62,15 +67,12 @@ struct Params {
   int router_bf16;
   __nv_bfloat16* y;
   __nv_bfloat16* hidden;       // [2][T * K][I]: high and low part
-  Routing* routing;            // written by the first kernel for the second
+  int* routing;                // for the second kernel: the number of entries, three words of each, order and token of every route
   unsigned* arrived;           // [row tiles] parts of a row tile that are there; zeroed by the first kernel
   float* part;                 // [2 * CTAs][T][32]
   int* status;
   int T, E, K, H, I, normalize;
 };
-
-__device__ __forceinline__ int cut(int N, int i, int n) { return int((long long)N * i / n); }
-__device__ __forceinline__ int owner(int N, int u, int n) { return int(((long long)(u + 1) * n - 1) / N); }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -124,8 +126,8 @@ struct Ring {
   }
 };
 
-// first / order / active from expert[]: one warp an expert, so the order is that of the routes whatever the timing.
-__device__ __forceinline__ void sort_routes(Routing& r, int routes, int E) {
+// Order and entries from expert[]: one warp an expert, so the order is that of the routes whatever the timing.
+__device__ __forceinline__ void sort_routes(Routing& r, int routes, int E, int K) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int e = warp; e < E; e += kWarps) {
     int n = 0;
@@ -137,13 +139,19 @@ __device__ __forceinline__ void sort_routes(Routing& r, int routes, int E) {
   if (threadIdx.x == 0) {
     int at = 0, live = 0;
     r.first[0] = 0;
+#pragma unroll 1
     for (int e = 0; e < E; ++e) {
       const int n = r.first[e + 1];
-      if (n > 0) r.active[live++] = e;
+#pragma unroll 1
+      for (int i = 0; i < n; i += kColumns, ++live) {
+        r.entry_expert[live] = e;
+        r.entry_begin[live] = at + i;
+        r.entry_tokens[live] = min(n - i, kColumns);
+      }
       at += n;
       r.first[e + 1] = at;
     }
-    r.num_active = live;
+    r.entries = live;
   }
   __syncthreads();
   for (int e = warp; e < E; e += kWarps) {
@@ -151,7 +159,11 @@ __device__ __forceinline__ void sort_routes(Routing& r, int routes, int E) {
     for (int i0 = 0; i0 < routes; i0 += 32) {
       const bool mine = i0 + lane < routes && r.expert[i0 + lane] == e;
       const unsigned votes = __ballot_sync(0xffffffffu, mine);
-      if (mine) r.order[at + __popc(votes & ((1u << lane) - 1))] = i0 + lane;
+      if (mine) {
+        const int to = at + __popc(votes & ((1u << lane) - 1));
+        r.order[to] = i0 + lane;
+        r.token[to] = (i0 + lane) / K;
+      }
       at += __popc(votes);
     }
   }
@@ -207,73 +219,82 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t& h, uint32_t& 
   l = pack_bf162(a1 - __uint_as_float(m << 16), b1 - __uint_as_float(m & 0xFFFF0000u));
 }
 
-// Partial logits part[warp][e][t] of this CTA's share of the contraction: 32 columns a warp and step, experts in tiles of 16 as rows.
-template <int MT, int NT, int UNROLL>
+// Partial logits part[warp][e][t] of this CTA's share of the contraction: steps of 16 experts (rows) by 32 columns, eight tokens a
+// product.  One loop over (expert tile, columns) whose loads run a step ahead: the code is run once or twice a launch, so
+// what it costs is its latency and its own size in the instruction cache.
 __device__ __forceinline__ void router_products(const Params& p, float* part, int worker, int workers) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int E16 = (p.E + 15) & ~15, T8 = (p.T + 7) & ~7;
-  float acc[MT][NT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-#pragma unroll UNROLL
-  for (int q = worker; q * 32 < p.H; q += workers) {
+  float* mine = part + (threadIdx.x >> 5) * (E16 * T8);
+  float acc[8][4];
+  float4 w[2][2];
+  uint4 b[8];
+  auto load = [&](int m, int q) {
     const int k = q * 32 + c * 8;
-    const bool in = k < p.H;
-    uint4 b[NT];
+    const bool in = m < E16 && k < p.H;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      b[j] = make_uint4(0, 0, 0, 0);
-      if (in && j * 8 < p.T) b[j] = __ldg(reinterpret_cast<const uint4*>(p.x + min(j * 8 + g, p.T - 1) * p.ldx + k));
+    for (int u = 0; u < 2; ++u) {
+      const long long at = (long long)min(m + g + 8 * u, p.E - 1) * p.H + k;
+      w[u][0] = w[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in && p.router_bf16) {
+        w[u][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const __nv_bfloat16*>(p.router) + at));      // eight bf16 values
+      } else if (in) {
+        w[u][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at));
+        w[u][1] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at) + 1);
+      }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m * 16 >= p.E) break;
-      uint32_t hi[2][4], mid[2][4], low[2][4];
+    for (int j = 0; j < 8; ++j) {
+      if (j * 8 >= p.T) break;
+      b[j] = in ? __ldg(reinterpret_cast<const uint4*>(p.x + min(j * 8 + g, p.T - 1) * p.ldx + k)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  int m = 0, q = worker;
+  load(m, q);
+#pragma unroll 1
+  while (m < E16) {
+    if (q == worker) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const long long at = (long long)min(m * 16 + g + 8 * u, p.E - 1) * p.H + k;
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+    }
+    uint32_t part3[3][2][4];           // high, middle, low
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float v[8] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w, w[u][1].x, w[u][1].y, w[u][1].z, w[u][1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         if (p.router_bf16) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (in) w = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.router) + at));
-          hi[u][0] = w.x; hi[u][1] = w.y; hi[u][2] = w.z; hi[u][3] = w.w;
+          part3[0][u][i] = __float_as_uint(v[i]);
+          part3[1][u][i] = part3[2][u][i] = 0u;
         } else {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
-          if (in) {
-            v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at));
-            w = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at) + 1);
-          }
-          split3(v.x, v.y, hi[u][0], mid[u][0], low[u][0]);
-          split3(v.z, v.w, hi[u][1], mid[u][1], low[u][1]);
-          split3(w.x, w.y, hi[u][2], mid[u][2], low[u][2]);
-          split3(w.z, w.w, hi[u][3], mid[u][3], low[u][3]);
+          split3(v[2 * i], v[2 * i + 1], part3[0][u][i], part3[1][u][i], part3[2][u][i]);
         }
       }
+    }
+    uint4 x[8];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if (j * 8 >= p.T) break;
-        if (!p.router_bf16) {          // the small parts first
-          mma_bf16(acc[m][j], low[0][0], low[1][0], low[0][1], low[1][1], b[j].x, b[j].y);
-          mma_bf16(acc[m][j], low[0][2], low[1][2], low[0][3], low[1][3], b[j].z, b[j].w);
-          mma_bf16(acc[m][j], mid[0][0], mid[1][0], mid[0][1], mid[1][1], b[j].x, b[j].y);
-          mma_bf16(acc[m][j], mid[0][2], mid[1][2], mid[0][3], mid[1][3], b[j].z, b[j].w);
-        }
-        mma_bf16(acc[m][j], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b[j].x, b[j].y);
-        mma_bf16(acc[m][j], hi[0][2], hi[1][2], hi[0][3], hi[1][3], b[j].z, b[j].w);
+    for (int j = 0; j < 8; ++j) x[j] = b[j];
+    const int m_now = m;
+    q += workers;
+    const bool last = q * 32 >= p.H;
+    if (last) { q = worker; m += 16; }
+    load(m, q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j * 8 >= p.T) break;
+#pragma unroll
+      for (int i = 2; i >= 0; --i) {   // the small parts first
+        mma_bf16(acc[j], part3[i][0][0], part3[i][1][0], part3[i][0][1], part3[i][1][1], x[j].x, x[j].y);
+        mma_bf16(acc[j], part3[i][0][2], part3[i][1][2], part3[i][0][3], part3[i][1][3], x[j].z, x[j].w);
+      }
+      if (last) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[(m_now + g + 8 * (i >> 1)) * T8 + j * 8 + 2 * c + (i & 1)] = acc[j][i];
       }
     }
   }
-  float* mine = part + (threadIdx.x >> 5) * (E16 * T8);
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (m * 16 < p.E && j * 8 < p.T) mine[(m * 16 + g + 8 * (i >> 1)) * T8 + j * 8 + 2 * c + (i & 1)] = acc[m][j][i];
 }
 
 // ---- kernel 1: routing, gate and up projection, SwiGLU ----
@@ -283,11 +304,11 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Routing r;
   __shared__ float weight[kRoutes];
-  __shared__ uint64_t bars[kWarps][kStagesMax];
+  __shared__ uint64_t bars[kWarps][kUpStages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int routes = p.T * p.K;
   float* part = reinterpret_cast<float*>(smem);            // partial logits, before the rings are used
-  float* logits = reinterpret_cast<float*>(smem + ring_bytes(p.T));                       // [T][E]
+  float* logits = reinterpret_cast<float*>(smem + kUpRing);                               // [T][E]
   const int E16 = (p.E + 15) & ~15, T8 = (p.T + 7) & ~7;
   int rank = 0, ranks = 1;
   if constexpr (CLUSTER) {
@@ -296,8 +317,7 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) tma_prefetch_desc(&weights);
-  if (p.E <= 16 && p.T <= 8) router_products<1, 1, 4>(p, part, rank * kWarps + warp, ranks * kWarps);
-  else router_products<4, 8, 1>(p, part, rank * kWarps + warp, ranks * kWarps);
+  router_products(p, part, rank * kWarps + warp, ranks * kWarps);
   __syncthreads();
   for (int i = threadIdx.x; i < p.T * p.E; i += kThreads) {
     const int t = i / p.E, e = i % p.E;
@@ -333,81 +353,139 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     choose_experts(p, logits, r, weight, 0, 1);
     __syncthreads();
   }
-  sort_routes(r, routes, p.E);
+  sort_routes(r, routes, p.E, p.K);
   if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < routes; i += kThreads) p.routing->order[i] = r.order[i];
-    for (int i = threadIdx.x; i <= p.E; i += kThreads) p.routing->first[i] = r.first[i];
-    for (int i = threadIdx.x; i < r.num_active; i += kThreads) p.routing->active[i] = r.active[i];
-    if (threadIdx.x == 0) p.routing->num_active = r.num_active;
+    if (threadIdx.x == 0) p.routing[0] = r.entries;
+    if (threadIdx.x < kEntries) p.routing[1 + threadIdx.x] = r.entry_expert[threadIdx.x] | (r.entry_tokens[threadIdx.x] << 8) | (r.entry_begin[threadIdx.x] << 16);
+    for (int i = threadIdx.x; i < routes; i += kThreads) p.routing[1 + kEntries + i] = r.order[i] | (r.token[i] << 16);
     for (int i = threadIdx.x; i < (p.H + kDownRows - 1) / kDownRows; i += kThreads) p.arrived[i] = 0u;
   }
 
   const int tiles = (p.I + kUpRows - 1) / kUpRows, steps = (p.H + kUpCols - 1) / kUpCols;
-  const int N = r.num_active * tiles;
-  const int c0 = cut(N, blockIdx.x, gridDim.x), c1 = cut(N, blockIdx.x + 1, gridDim.x);
-  const int i0 = c0 + cut(c1 - c0, warp, kWarps), i1 = c0 + cut(c1 - c0, warp + 1, kWarps);
+  const int N = r.entries * tiles;
+  const Parts parts(N, gridDim.x);
+  const int c0 = parts.begin(blockIdx.x), c1 = parts.begin(blockIdx.x + 1);
+  const int i0 = c0 + part_begin<kWarps>(c1 - c0, warp), i1 = c0 + part_begin<kWarps>(c1 - c0, warp + 1);
   if (i0 == i1) return;
   Ring ring;
-  ring.stages = ring_stages(p.T);
-  ring.base = smem + warp * ring.stages * kTile;
+  ring.stages = kUpStages;
+  ring.base = smem + warp * kUpStages * kTile;
   ring.bars = bars[warp];
   ring.status = p.status;
   ring.lane = lane;
   ring.init();
-  int ahead = i0, ahead_step = 0;
+  int left = (i1 - i0) * steps, ahead_step = 0, ahead_expert = i0 / tiles, ahead_tile = i0 % tiles;
+  int expert = ahead_expert, tile_at = ahead_tile;
   auto next_copy = [&]() {
-    if (ahead == i1) return;
-    ring.copy(&weights, ahead_step * kUpCols, ahead % tiles * kUpRows, 2 * r.active[ahead / tiles]);
-    if (++ahead_step == steps) { ahead_step = 0; ++ahead; }
+    if (left == 0) return;
+    --left;
+    ring.copy(&weights, ahead_step * kUpCols, ahead_tile * kUpRows, 2 * r.entry_expert[ahead_expert]);
+    if (++ahead_step == steps) {
+      ahead_step = 0;
+      if (++ahead_tile == tiles) { ahead_tile = 0; ++ahead_expert; }
+    }
   };
   fence_proxy_async_smem();              // the ring's memory held partial logits
   __syncwarp();
+#pragma unroll 1
   for (int s = 0; s < ring.stages; ++s) next_copy();
 
-  for (int item = i0; item < i1; ++item) {
-    const int e = r.active[item / tiles], row = item % tiles * kUpRows + g;
-    const int n0 = r.first[e], n = r.first[e + 1] - n0, nts = (n + 7) / 8;
-    float acc[8][4];
+  // The columns of the first eight tokens of a unit are loaded while the unit before is computed (two sets of registers in turn), those
+  // of more tokens in place.
+  struct Columns {
+    uint4 v[kUpCols / 32];
+  };
+  const __nv_bfloat16* first_row = nullptr;
+  int n0 = 0, n = 0;
+  auto row_of = [&](int begin, int tokens, int j) { return p.x + (long long)r.token[begin + min(j * 8 + g, tokens - 1)] * p.ldx + c * 8; };
+  auto enter = [&]() {                   // the entry that `expert` points to
+    n0 = r.entry_begin[expert];
+    n = r.entry_tokens[expert];
+    first_row = row_of(n0, n, 0);
+  };
+  auto load = [&](Columns& b, const __nv_bfloat16* row, int step) {
+    const __nv_bfloat16* src = row + step * kUpCols;
+    if ((step + 1) * kUpCols <= p.H) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+      for (int s = 0; s < kUpCols / 32; ++s) b.v[s] = __ldg(reinterpret_cast<const uint4*>(src + 32 * s));
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-    for (int step = 0; step < steps; ++step) {
-      const int k = step * kUpCols + c * 8;
-      uint4 b[4];
-      auto load_x = [&](int j) {
-        const __nv_bfloat16* src = p.x + (long long)(r.order[n0 + min(j * 8 + g, n - 1)] / p.K) * p.ldx + k;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) b[s] = k + 32 * s < p.H ? __ldg(reinterpret_cast<const uint4*>(src + 32 * s)) : make_uint4(0, 0, 0, 0);
-      };
-      load_x(0);
-      const uint8_t* tile = ring.wait() + g * (kUpCols * 2) + c * 16;
-      uint4 a[4][2];
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) a[s][u] = *reinterpret_cast<const uint4*>(tile + u * (kUpRows * kUpCols * 2) + s * 64);
-      ring.taken();
-      next_copy();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j >= nts) break;
-        if (j > 0) load_x(j);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          mma_bf16(acc[j], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b[s].x, b[s].y);
-          mma_bf16(acc[j], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b[s].z, b[s].w);
-        }
+      for (int s = 0; s < kUpCols / 32; ++s) {
+        b.v[s] = make_uint4(0, 0, 0, 0);
+        if (step * kUpCols + 32 * s + c * 8 < p.H) b.v[s] = __ldg(reinterpret_cast<const uint4*>(src + 32 * s));
       }
     }
-    if (row >= p.I) continue;
+  };
+  float acc[kColumns / 8][4], acc_odd[4];                  // the first product in two chains
+  int items = i1 - i0, step = 0, n0_item = 0, n_item = 0;
+  // one unit: its tile from the ring, its columns in `b`; the columns of the one behind it go to `other`
+  auto unit = [&](Columns& b, Columns& other) {
+    const uint8_t* tile = ring.wait() + g * (kUpCols * 2) + c * 16;
+    uint4 a[kUpCols / 32][2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int s = 0; s < kUpCols / 32; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) a[s][u] = *reinterpret_cast<const uint4*>(tile + u * (kUpRows * kUpCols * 2) + s * 64);
+    ring.taken();
+    next_copy();
+    if (step + 1 < steps) {
+      load(other, first_row, step + 1);
+    } else if (items > 1) {
+      if (++tile_at == tiles) { tile_at = 0; ++expert; enter(); }
+      load(other, first_row, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < kUpCols / 32; ++s) {
+      mma_bf16(acc[0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.v[s].x, b.v[s].y);
+      mma_bf16(acc_odd, a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.v[s].z, b.v[s].w);
+    }
+#pragma unroll
+    for (int j = 1; j < kColumns / 8; ++j) {
+      if (j * 8 >= n_item) break;
+      load(b, row_of(n0_item, n_item, j), step);
+#pragma unroll
+      for (int s = 0; s < kUpCols / 32; ++s) {
+        mma_bf16(acc[j], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.v[s].x, b.v[s].y);
+        mma_bf16(acc[j], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.v[s].z, b.v[s].w);
+      }
+    }
+    ++step;
+  };
+  Columns even, odd;
+  enter();
+  load(even, first_row, 0);
+#pragma unroll 1
+  for (; items > 0; --items) {
+    const int row = tile_at * kUpRows + g;
+    n0_item = n0;
+    n_item = n;
+    step = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc_odd[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kColumns / 8; ++j) acc[j][i] = 0.f;
+    }
+#pragma unroll 1
+    while (step + 1 < steps) {
+      unit(even, odd);
+      unit(odd, even);
+    }
+    if (step < steps) {
+      unit(even, odd);
+      even = odd;
+    }
+    // ---- the hidden values of the item ----
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[0][i] += acc_odd[i];
+#pragma unroll
+    for (int j = 0; j < kColumns / 8; ++j) {
+      if (j * 8 >= n_item) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int col = j * 8 + 2 * c + i;
-        if (col >= n) continue;
-        const int route = r.order[n0 + col];
+        if (col >= n_item || row >= p.I) continue;
+        const int route = r.order[n0_item + col];
         const float gate = acc[j][i], up = acc[j][i + 2];
         const float h = gate / (1.f + expf(-gate)) * up * weight[route];
         const __nv_bfloat16 high = __float2bfloat16_rn(h);
@@ -415,6 +493,7 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
         dst[0] = high;
         dst[(long long)routes * p.I] = __float2bfloat16_rn(h - __bfloat162float(high));
       }
+    }
   }
   ring.finish();
 }
@@ -424,117 +503,194 @@ __global__ void __launch_bounds__(kThreads)
 moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Routing r;
-  __shared__ uint64_t bars[kWarps][kStagesMax];
+  __shared__ uint64_t bars[kWarps][3];
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int routes = p.T * p.K, sum_size = p.T * kSumPitch;
-  float* sums = reinterpret_cast<float*>(smem + ring_bytes(p.T));                         // [warps][T][pitch]
+  float* sums = reinterpret_cast<float*>(smem + kWarps * down_stages(p.T) * kTile);       // [warps][T][pitch]
   for (int i = threadIdx.x; i < kWarps * sum_size; i += kThreads) sums[i] = 0.f;
   if (threadIdx.x == 0) tma_prefetch_desc(&weights);
   Ring ring;
-  ring.stages = ring_stages(p.T);
+  ring.stages = down_stages(p.T);
   ring.base = smem + warp * ring.stages * kTile;
   ring.bars = bars[warp];
   ring.status = p.status;
   ring.lane = lane;
   ring.init();
   asm volatile("griddepcontrol.wait;" ::: "memory");       // what follows reads what the first kernel wrote
-  for (int i = threadIdx.x; i < routes; i += kThreads) r.order[i] = __ldcg(&p.routing->order[i]);
-  for (int i = threadIdx.x; i <= p.E; i += kThreads) r.first[i] = __ldcg(&p.routing->first[i]);
-  const int live = __ldcg(&p.routing->num_active);
-  for (int i = threadIdx.x; i < live; i += kThreads) r.active[i] = __ldcg(&p.routing->active[i]);
+  {
+    constexpr int MOST = (1 + kEntries + kRoutes + kThreads - 1) / kThreads;
+    const int words = 1 + kEntries + routes;
+    int v[MOST];                         // all loads before the first use
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) v[i] = threadIdx.x + i * kThreads < words ? __ldcg(p.routing + threadIdx.x + i * kThreads) : 0;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      const int at = threadIdx.x + i * kThreads;
+      if (at == 0) {
+        r.entries = v[i];
+      } else if (at <= kEntries) {
+        r.entry_expert[at - 1] = v[i] & 0xFF;
+        r.entry_tokens[at - 1] = (v[i] >> 8) & 0xFF;
+        r.entry_begin[at - 1] = (v[i] >> 16) & 0xFFFF;
+      } else if (at < words) {
+        r.order[at - 1 - kEntries] = v[i] & 0xFFFF;
+        r.token[at - 1 - kEntries] = v[i] >> 16;
+      }
+    }
+  }
   __syncthreads();
+  const int live = r.entries;
 
   const int steps = (p.I + kDownCols - 1) / kDownCols, tiles = (p.H + kDownRows - 1) / kDownRows;
-  const int per_tile = live * steps, N = tiles * per_tile, parts = min(int(gridDim.x), N);
-  if (int(blockIdx.x) >= parts) return;
-  const int c0 = cut(N, blockIdx.x, parts), c1 = cut(N, blockIdx.x + 1, parts);
+  const int per_tile = live * steps, N = tiles * per_tile, ctas = min(int(gridDim.x), N);
+  if (int(blockIdx.x) >= ctas) return;
+  const Parts parts(N, ctas);
+  const int c0 = parts.begin(blockIdx.x), c1 = parts.begin(blockIdx.x + 1);
   // The units of this warp: its share of what the CTA has of each row tile, one after the other.
   struct Stream {
-    int tile, u, end;
+    int tile, u, end, expert, step;
   };
   auto enter = [&](Stream& s) {          // the first row tile from s.tile on that has units for this warp
     for (; s.tile * per_tile < c1; ++s.tile) {
       const int s0 = max(c0, s.tile * per_tile), s1 = min(c1, (s.tile + 1) * per_tile);
-      s.u = s0 + cut(s1 - s0, warp, kWarps);
-      s.end = s0 + cut(s1 - s0, warp + 1, kWarps);
-      if (s.u < s.end) return;
+      s.u = s0 + part_begin<kWarps>(s1 - s0, warp);
+      s.end = s0 + part_begin<kWarps>(s1 - s0, warp + 1);
+      if (s.u == s.end) continue;
+      s.expert = (s.u - s.tile * per_tile) / steps;
+      s.step = (s.u - s.tile * per_tile) % steps;
+      return;
     }
     s.u = s.end = 0;
   };
-  Stream ahead{c0 / per_tile, 0, 0};
+  Stream ahead{c0 / per_tile, 0, 0, 0, 0};
   enter(ahead);
   auto next_copy = [&]() {
     if (ahead.u == ahead.end) return;
-    const int rest = ahead.u - ahead.tile * per_tile;
-    ring.copy(&weights, rest % steps * kDownCols, ahead.tile * kDownRows, r.active[rest / steps]);
+    ring.copy(&weights, ahead.step * kDownCols, ahead.tile * kDownRows, r.entry_expert[ahead.expert]);
+    if (++ahead.step == steps) { ahead.step = 0; ++ahead.expert; }
     if (++ahead.u == ahead.end) { ++ahead.tile; enter(ahead); }
   };
+#pragma unroll 1
   for (int s = 0; s < ring.stages; ++s) next_copy();
 
+  // Hidden values of a unit, as the columns in the first kernel: [32 columns][high, low]
+  struct Columns {
+    uint4 v[kDownCols / 32][2];
+  };
+  const __nv_bfloat16* first_row = nullptr;
+  const long long low = (long long)routes * p.I;           // from a high part to its low part
+  int ai = 0, n0 = 0, n = 0;
+  auto row_of = [&](int begin, int tokens, int j) { return p.hidden + (long long)r.order[begin + min(j * 8 + g, tokens - 1)] * p.I + c * 8; };
+  auto enter_entry = [&]() {
+    n0 = r.entry_begin[ai];
+    n = r.entry_tokens[ai];
+    first_row = row_of(n0, n, 0);
+  };
+  auto load = [&](Columns& b, const __nv_bfloat16* row, int step) {
+    const __nv_bfloat16 *src = row + step * kDownCols, *src_low = src + low;
+    if ((step + 1) * kDownCols <= p.I) {
+#pragma unroll
+      for (int s = 0; s < kDownCols / 32; ++s) {
+        b.v[s][0] = *reinterpret_cast<const uint4*>(src + 32 * s);
+        b.v[s][1] = *reinterpret_cast<const uint4*>(src_low + 32 * s);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < kDownCols / 32; ++s) {
+        b.v[s][0] = b.v[s][1] = make_uint4(0, 0, 0, 0);
+        if (step * kDownCols + 32 * s + c * 8 < p.I) {
+          b.v[s][0] = *reinterpret_cast<const uint4*>(src + 32 * s);
+          b.v[s][1] = *reinterpret_cast<const uint4*>(src_low + 32 * s);
+        }
+      }
+    }
+  };
+  float acc[2][kColumns / 8][4];
+  auto multiply = [&](int j, const Columns& x, const uint4 (&a)[2][kDownCols / 32][2]) {
+#pragma unroll
+    for (int s = 0; s < kDownCols / 32; ++s)
+#pragma unroll
+      for (int v = 1; v >= 0; --v)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma_bf16(acc[m][j], a[m][s][0].x, a[m][s][1].x, a[m][s][0].y, a[m][s][1].y, x.v[s][v].x, x.v[s][v].y);
+          mma_bf16(acc[m][j], a[m][s][0].z, a[m][s][1].z, a[m][s][0].w, a[m][s][1].w, x.v[s][v].z, x.v[s][v].w);
+        }
+  };
   float* mine = sums + warp * sum_size;
+  int units = 0, step = 0, n0_now = 0, n_now = 0;
+  auto unit = [&](Columns& b, Columns& other) {
+    const uint8_t* at = ring.wait() + g * (kDownCols * 2) + c * 16;
+    uint4 a[2][kDownCols / 32][2];       // [row tile of 16][32 columns][rows g, g + 8]
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int s = 0; s < kDownCols / 32; ++s)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) a[m][s][v] = *reinterpret_cast<const uint4*>(at + (16 * m + 8 * v) * (kDownCols * 2) + s * 64);
+    ring.taken();
+    next_copy();
+    if (units > 1) {
+      if (step + 1 < steps) {
+        load(other, first_row, step + 1);
+      } else {
+        ++ai;
+        enter_entry();
+        load(other, first_row, 0);
+      }
+    }
+    multiply(0, b, a);
+#pragma unroll
+    for (int j = 1; j < kColumns / 8; ++j) {
+      if (j * 8 >= n_now) break;
+      load(b, row_of(n0_now, n_now, j), step);
+      multiply(j, b, a);
+    }
+    ++step;
+    --units;
+  };
+#pragma unroll 1
   for (int tile = c0 / per_tile; tile * per_tile < c1; ++tile) {
     const int s0 = max(c0, tile * per_tile), s1 = min(c1, (tile + 1) * per_tile);
-    int u = s0 + cut(s1 - s0, warp, kWarps);
-    const int end = s0 + cut(s1 - s0, warp + 1, kWarps);
-    while (u < end) {
-      const int rest = u - tile * per_tile, ai = rest / steps, e = r.active[ai];
-      const int step0 = rest % steps, step1 = min(steps, step0 + end - u);
-      u += step1 - step0;
-      const int n0 = r.first[e], n = r.first[e + 1] - n0, nts = (n + 7) / 8;
-      float acc[2][8][4];
+    const int u = s0 + part_begin<kWarps>(s1 - s0, warp);
+    units = s0 + part_begin<kWarps>(s1 - s0, warp + 1) - u;
+    Columns even, odd;
+    if (units > 0) {
+      ai = (u - tile * per_tile) / steps;
+      step = (u - tile * per_tile) % steps;
+      enter_entry();
+      load(even, first_row, step);
+    }
+#pragma unroll 1
+    while (units > 0) {                  // one entry of this row tile
+      n0_now = n0;
+      n_now = n;
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < kColumns / 8; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-      for (int step = step0; step < step1; ++step) {
-        const int k = step * kDownCols + c * 8;
-        uint4 b[2][2];
-        auto load_h = [&](int j) {
-          const __nv_bfloat16* src = p.hidden + (long long)r.order[n0 + min(j * 8 + g, n - 1)] * p.I + k;
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-              b[s][v] = k + 32 * s < p.I ? *reinterpret_cast<const uint4*>(src + (long long)v * routes * p.I + 32 * s) : make_uint4(0, 0, 0, 0);
-        };
-        load_h(0);
-        const uint8_t* at = ring.wait() + g * (kDownCols * 2) + c * 16;
-        uint4 a[2][2][2];                // [row tile of 16][32 columns][rows g, g + 8]
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int v = 0; v < 2; ++v) a[m][s][v] = *reinterpret_cast<const uint4*>(at + (16 * m + 8 * v) * (kDownCols * 2) + s * 64);
-        ring.taken();
-        next_copy();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j >= nts) break;
-          if (j > 0) load_h(j);
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int v = 1; v >= 0; --v)
-#pragma unroll
-              for (int m = 0; m < 2; ++m) {
-                mma_bf16(acc[m][j], a[m][s][0].x, a[m][s][1].x, a[m][s][0].y, a[m][s][1].y, b[s][v].x, b[s][v].y);
-                mma_bf16(acc[m][j], a[m][s][0].z, a[m][s][1].z, a[m][s][0].w, a[m][s][1].w, b[s][v].z, b[s][v].w);
-              }
-        }
+#pragma unroll 1
+      while (units > 1 && step + 1 < steps) {
+        unit(even, odd);
+        unit(odd, even);
       }
-      // an expert has a token at most once, so the lanes of a warp write different sums
+      if (units > 0 && step < steps) {
+        unit(even, odd);
+        even = odd;
+      }
+      step = 0;
+      // an entry has a token at most once, so the lanes of a warp write different sums
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j >= nts) break;
+      for (int j = 0; j < kColumns / 8; ++j) {
+        if (j * 8 >= n_now) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int col = j * 8 + 2 * c + i;
-          if (col >= n) continue;
-          float* dst = mine + r.order[n0 + col] / p.K * kSumPitch + g;
+          if (col >= n_now) continue;
+          float* dst = mine + r.token[n0_now + col] * kSumPitch + g;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             dst[16 * m] += acc[m][j][i];
@@ -560,7 +716,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
       else if (tile * kDownRows + row < p.H) p.y[(long long)t * p.H + tile * kDownRows + row] = __float2bfloat16_rn(v);
     }
     if (!whole) {
-      const int f = owner(N, tile * per_tile, parts), l = owner(N, (tile + 1) * per_tile - 1, parts);
+      const int f = parts.owner(tile * per_tile), l = parts.owner((tile + 1) * per_tile - 1);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -574,7 +730,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
           float v = 0.f;
 #pragma unroll 8
           for (int k = f; k <= l; ++k)
-            v += __ldcg(p.part + (2 * (long long)k + (cut(N, k, parts) <= tile * per_tile ? 1 : 0)) * p.T * kDownRows + i);
+            v += __ldcg(p.part + (2 * (long long)k + (parts.begin(k) <= tile * per_tile ? 1 : 0)) * p.T * kDownRows + i);
           if (row < p.H) p.y[(long long)t * p.H + row] = __float2bfloat16_rn(v);
         }
     }
@@ -603,10 +759,10 @@ bool encode_weights(CUtensorMap* map, const void* base, long long cols, long lon
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kCluster = 4;
+constexpr int kCluster = 2;
 
-size_t up_shared(int T, int E) { return size_t(ring_bytes(T)) + size_t(T) * E * 4; }
-size_t down_shared(int T) { return size_t(ring_bytes(T)) + size_t(kWarps) * T * kSumPitch * 4; }
+size_t up_shared(int T, int E) { return size_t(kUpRing) + size_t(T) * E * 4; }
+size_t down_shared(int T) { return size_t(kWarps) * down_stages(T) * kTile + size_t(kWarps) * T * kSumPitch * 4; }
 
 // What a launch needs to know of a device, found once.
 struct DeviceFacts {
@@ -618,8 +774,8 @@ DeviceFacts& facts(int dev) {
   static DeviceFacts all[64];
   DeviceFacts& f = all[dev];
   std::call_once(f.once, [&f] {
-    const int up = int(up_shared(kMoeTokensMax, kExperts) > up_shared(32, kExperts) ? up_shared(kMoeTokensMax, kExperts) : up_shared(32, kExperts));
-    const int down = int(down_shared(kMoeTokensMax) > down_shared(32) ? down_shared(kMoeTokensMax) : down_shared(32));
+    const int up = int(up_shared(kMoeTokensMax, kExperts));
+    const int down = int(down_shared(16) > down_shared(kMoeTokensMax) ? down_shared(16) : down_shared(kMoeTokensMax));
     f.sms = device_sm_count();
     if ((f.error = cudaFuncSetAttribute(moe_up_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, up)) != cudaSuccess) return;
     if ((f.error = cudaFuncSetAttribute(moe_up_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, up)) != cudaSuccess) return;
@@ -648,7 +804,7 @@ struct Workspace {                       // byte offsets of its parts
 Workspace workspace_of(int T, int K, int H, int I) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   Workspace w;
-  w.hidden = up(sizeof(Routing));
+  w.hidden = up(size_t(1 + kEntries + T * K) * 4);
   w.part = w.hidden + up(size_t(2) * T * K * I * 2);
   w.arrived = w.part + up(size_t(2) * device_sm_count() * T * kDownRows * 4);
   w.total = w.arrived + up(size_t((H + kDownRows - 1) / kDownRows) * 4);
@@ -679,7 +835,7 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   p.x = static_cast<const __nv_bfloat16*>(a.x); p.ldx = a.ldx;
   p.router = a.router; p.router_bf16 = a.router_bf16;
   p.y = static_cast<__nv_bfloat16*>(a.y);
-  p.routing = reinterpret_cast<Routing*>(ws);
+  p.routing = reinterpret_cast<int*>(ws);
   p.hidden = reinterpret_cast<__nv_bfloat16*>(ws + w.hidden);
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.arrived = reinterpret_cast<unsigned*>(ws + w.arrived);
@@ -695,7 +851,7 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   cfg.blockDim = dim3(kThreads);
   cfg.stream = a.stream;
   cfg.attrs = attr;
-  // What a CTA reads to route by itself (x and the router's weight, from L2); above 256 KB four CTAs share it.
+  // What a CTA reads to route by itself (x and the router's weight, from L2); above 256 KB two CTAs share it.
   const long long routing = (long long)a.E * a.H * (a.router_bf16 ? 2 : 4) + (long long)a.T * a.H * 2;
   cfg.dynamicSmemBytes = up_shared(a.T, a.E);
   ++g_launch_count;
