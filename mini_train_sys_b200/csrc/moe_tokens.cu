@@ -1,4 +1,4 @@
-// A whole mixture-of-experts layer for a few tokens in two kernels.
+// A whole mixture-of-experts layer for a few tokens in two kernels (three where the router is large).
 //
 //   p = softmax(x Wr^T);  the K largest (ties to the lower expert), optionally divided by their sum
 //   y = sum_k w_k Wd[e_k] (silu(Wg[e_k] x) * (Wu[e_k] x))
@@ -7,11 +7,12 @@
 // m16n8k16 and the tokens of their expert the columns (8 at a time), so one pass over the weights serves up to 64 tokens.  Every warp
 // streams its own weight tiles through a ring in shared memory, 8 KB a TMA copy and 16 or 24 KB in flight a warp, across the ends of
 // items: 128 to 192 KB in flight an SM, and no barrier between warps inside a stream.
-//   1  every CTA (or cluster, where the router is large) routes all tokens for itself; then a warp takes (expert, 8 columns of the
-//      hidden layer) items: 8 gate rows and 8 up rows are one tile, so a lane ends up with both factors of its hidden values and
-//      applies SwiGLU in registers.  The hidden value is multiplied by the route's weight, so that the sums of the second
-//      kernel are over the experts already.
-//   2  the (32 output rows, expert, 128 columns) units of the down projections are one list, cut into equal parts for the CTAs; what
+//   0  Routing reads x and the router's weight.  Up to 48 KB of them every CTA of the first kernel reads for itself (a launch costs
+//      more); above that one cluster of eight CTAs routes in a kernel of its own.
+//   1  A warp takes (entry, 8 columns of the hidden layer) items, an entry being an expert and its tokens: 8 gate rows and 8 up rows
+//      are one tile, so a lane ends up with both factors of its hidden values and applies SwiGLU in registers.  The hidden value
+//      is multiplied by the route's weight, so that the sums of the second kernel are over the experts already.
+//   2  The (32 output rows, expert, 128 columns) units of the down projections are one list, cut into equal parts for the CTAs; what
 //      a CTA has of a row tile is added in shared memory, and where a tile was cut its last CTA adds the parts, in order.
 //
 // Rounding: logits, softmax, sums and the hidden values are fp32 (the router's fp32 weight enters the tensor cores as the sum of three
@@ -55,10 +56,12 @@ struct Routing {
   int expert[kRoutes];         // of a route, as chosen
   int order[kRoutes];          // routes by expert, ascending
   int token[kRoutes];          // of the routes in order
-  int first[kExperts + 1];
+  int first[kExperts];         // place of an expert's first route
   int entry_expert[kEntries], entry_begin[kEntries], entry_tokens[kEntries];
   int entries;
+  float weight[kRoutes];       // of a route
 };
+constexpr int kChunks = kRoutes / 32;
 
 struct Params {
   const __nv_bfloat16* x;
@@ -67,7 +70,7 @@ struct Params {
   int router_bf16;
   __nv_bfloat16* y;
   __nv_bfloat16* hidden;       // [2][T * K][I]: high and low part
-  int* routing;                // for the second kernel: the number of entries, three words of each, order and token of every route
+  int* routing;                // published: number of entries, the entries, order and token of every route, weights (1 + kEntries + 2 T K words)
   unsigned* arrived;           // [row tiles] parts of a row tile that are there; zeroed by the first kernel
   float* part;                 // [2 * CTAs][T][32]
   int* status;
@@ -126,80 +129,99 @@ struct Ring {
   }
 };
 
-// Order and entries from expert[]: one warp an expert, so the order is that of the routes whatever the timing.
-__device__ __forceinline__ void sort_routes(Routing& r, int routes, int E, int K) {
+// Order, tokens and entries from expert[].  A route's place is the number of routes before it that go to its expert: those of its chunk
+// of 32 by a vote, those of the chunks before by a running sum, so that it does not depend on timing.
+__device__ __forceinline__ void sort_routes(Routing& r, int (*counts)[kExperts], int routes, int K) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = warp; e < E; e += kWarps) {
-    int n = 0;
-    for (int i = lane; i < routes; i += 32) n += r.expert[i] == e;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) r.first[e + 1] = n;
+  for (int i = threadIdx.x; i < kChunks * kExperts; i += kThreads) counts[i / kExperts][i % kExperts] = 0;
+  __syncthreads();
+  constexpr int MINE = kChunks / kWarps;
+  int expert[MINE], rank[MINE];
+#pragma unroll
+  for (int q = 0; q < MINE; ++q) {
+    const int chunk = warp + q * kWarps, i = chunk * 32 + lane;
+    expert[q] = -1;
+    rank[q] = 0;
+    if (chunk * 32 >= routes) continue;
+    if (i < routes) expert[q] = r.expert[i];
+    const unsigned same = __match_any_sync(0xffffffffu, expert[q]);
+    rank[q] = __popc(same & ((1u << lane) - 1));
+    if (expert[q] >= 0 && rank[q] == 0) counts[chunk][expert[q]] = __popc(same);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int at = 0, live = 0;
-    r.first[0] = 0;
-#pragma unroll 1
-    for (int e = 0; e < E; ++e) {
-      const int n = r.first[e + 1];
-#pragma unroll 1
-      for (int i = 0; i < n; i += kColumns, ++live) {
-        r.entry_expert[live] = e;
-        r.entry_begin[live] = at + i;
-        r.entry_tokens[live] = min(n - i, kColumns);
+  if (warp == 0) {
+    int n[2], before = 0, entries_before = 0;              // experts 2 lane, 2 lane + 1
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      n[j] = 0;
+      for (int chunk = 0; chunk * 32 < routes; ++chunk) {
+        const int here = counts[chunk][2 * lane + j];
+        counts[chunk][2 * lane + j] = n[j];
+        n[j] += here;
       }
-      at += n;
-      r.first[e + 1] = at;
     }
-    r.entries = live;
+    int sum = n[0] + n[1], parts = (n[0] + kColumns - 1) / kColumns + (n[1] + kColumns - 1) / kColumns;
+    before = sum;
+    entries_before = parts;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, off), v = __shfl_up_sync(0xffffffffu, entries_before, off);
+      if (lane >= off) { before += u; entries_before += v; }
+    }
+    if (lane == 31) r.entries = entries_before;
+    before -= sum;
+    entries_before -= parts;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      r.first[2 * lane + j] = before;
+      for (int i = 0; i < n[j]; i += kColumns, ++entries_before) {
+        r.entry_expert[entries_before] = 2 * lane + j;
+        r.entry_begin[entries_before] = before + i;
+        r.entry_tokens[entries_before] = min(n[j] - i, kColumns);
+      }
+      before += n[j];
+    }
   }
   __syncthreads();
-  for (int e = warp; e < E; e += kWarps) {
-    int at = r.first[e];
-    for (int i0 = 0; i0 < routes; i0 += 32) {
-      const bool mine = i0 + lane < routes && r.expert[i0 + lane] == e;
-      const unsigned votes = __ballot_sync(0xffffffffu, mine);
-      if (mine) {
-        const int to = at + __popc(votes & ((1u << lane) - 1));
-        r.order[to] = i0 + lane;
-        r.token[to] = (i0 + lane) / K;
-      }
-      at += __popc(votes);
-    }
+#pragma unroll
+  for (int q = 0; q < MINE; ++q) {
+    if (expert[q] < 0) continue;
+    const int chunk = warp + q * kWarps, i = chunk * 32 + lane, to = r.first[expert[q]] + counts[chunk][expert[q]] + rank[q];
+    r.order[to] = i;
+    r.token[to] = i / K;
   }
   __syncthreads();
 }
 
-// One warp a token: K rounds of arg-max over the logits (two experts a lane), then the softmax of the chosen ones.
+// One warp a token: K rounds of arg-max over the logits (two experts a lane), the first of which is the softmax's maximum.
 // The tokens of this CTA are rank, rank + ranks, ...
-__device__ __forceinline__ void choose_experts(const Params& p, const float* logits, Routing& r, float* weight, int rank, int ranks) {
+__device__ __forceinline__ void choose_experts(const Params& p, const float* logits, Routing& r, int rank, int ranks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
   for (int t = rank + ranks * warp; t < p.T; t += ranks * kWarps) {
-    float v[2];
-    unsigned key[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int e = lane + 32 * j;
-      v[j] = e < p.E ? logits[t * p.E + e] : -CUDART_INF_F;
-      const unsigned u = __float_as_uint(v[j]);
-      key[j] = e < p.E ? ((u & 0x80000000u) ? ~u : (u | 0x80000000u)) : 0u;        // unsigned order = float order
-      if (e < p.E && key[j] == 0u) key[j] = 1u;                                     // a negative NaN still beats "taken"
-    }
-    float mx = fmaxf(v[0], v[1]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    float sum = (lane < p.E ? expf(v[0] - mx) : 0.f) + (lane + 32 < p.E ? expf(v[1] - mx) : 0.f);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    float chosen = 0.f;                                    // lane k: the weight of choice k
+    const float v0 = lane < p.E ? logits[t * p.E + lane] : -CUDART_INF_F, v1 = lane + 32 < p.E ? logits[t * p.E + lane + 32] : -CUDART_INF_F;
+    auto key_of = [](float v) {                            // unsigned order = float order; 0 is "taken", which a negative NaN still beats
+      const unsigned u = __float_as_uint(v);
+      return max((u & 0x80000000u) ? ~u : (u | 0x80000000u), 1u);
+    };
+    unsigned k0 = lane < p.E ? key_of(v0) : 0u, k1 = lane + 32 < p.E ? key_of(v1) : 0u;
+    float chosen = 0.f, top = 0.f, sum = 1.f;              // lane k: the weight of choice k
     int which = 0;
+#pragma unroll 1
     for (int k = 0; k < p.K; ++k) {
-      const unsigned best = __reduce_max_sync(0xffffffffu, max(key[0], key[1]));
-      const unsigned low = __ballot_sync(0xffffffffu, key[0] == best), high = __ballot_sync(0xffffffffu, key[1] == best);
-      const int e = low != 0u ? __ffs(low) - 1 : 32 + __ffs(high) - 1;
-      const float l = __shfl_sync(0xffffffffu, e < 32 ? v[0] : v[1], e & 31);
-      if (lane == (e & 31)) key[e >> 5] = 0u;
-      if (lane == k) { chosen = expf(l - mx) / sum; which = e; }
+      const unsigned best = __reduce_max_sync(0xffffffffu, max(k0, k1));
+      const unsigned low = __ballot_sync(0xffffffffu, k0 == best), high = __ballot_sync(0xffffffffu, k1 == best);
+      const int e = low != 0u ? __ffs(low) - 1 : 31 + __ffs(high);
+      const float l = __shfl_sync(0xffffffffu, e < 32 ? v0 : v1, e & 31);
+      if (k == 0) {
+        top = l;
+        sum = (lane < p.E ? expf(v0 - top) : 0.f) + (lane + 32 < p.E ? expf(v1 - top) : 0.f);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      }
+      if (lane == e) k0 = 0u;
+      if (lane + 32 == e) k1 = 0u;
+      if (lane == k) { chosen = expf(l - top) / sum; which = e; }
     }
     if (p.normalize) {
       float total = lane < p.K ? chosen : 0.f;
@@ -207,7 +229,7 @@ __device__ __forceinline__ void choose_experts(const Params& p, const float* log
       for (int off = 4; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
       chosen = chosen / fmaxf(total, 1.1920929e-07f);
     }
-    if (lane < p.K) { r.expert[t * p.K + lane] = which; weight[t * p.K + lane] = chosen; }
+    if (lane < p.K) { r.expert[t * p.K + lane] = which; r.weight[t * p.K + lane] = chosen; }
   }
 }
 
@@ -297,28 +319,10 @@ __device__ __forceinline__ void router_products(const Params& p, float* part, in
   }
 }
 
-// ---- kernel 1: routing, gate and up projection, SwiGLU ----
-template <bool CLUSTER>
-__global__ void __launch_bounds__(kThreads)
-moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ Routing r;
-  __shared__ float weight[kRoutes];
-  __shared__ uint64_t bars[kWarps][kUpStages];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int routes = p.T * p.K;
-  float* part = reinterpret_cast<float*>(smem);            // partial logits, before the rings are used
-  float* logits = reinterpret_cast<float*>(smem + kUpRing);                               // [T][E]
+// What the CTA's warps have of the logits, added.
+__device__ __forceinline__ void add_logits(const Params& p, const float* part, float* logits) {
   const int E16 = (p.E + 15) & ~15, T8 = (p.T + 7) & ~7;
-  int rank = 0, ranks = 1;
-  if constexpr (CLUSTER) {
-    rank = int(cg::this_cluster().block_rank());
-    ranks = int(cg::this_cluster().num_blocks());
-  }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) tma_prefetch_desc(&weights);
-  router_products(p, part, rank * kWarps + warp, ranks * kWarps);
-  __syncthreads();
+#pragma unroll 1
   for (int i = threadIdx.x; i < p.T * p.E; i += kThreads) {
     const int t = i / p.E, e = i % p.E;
     float v = 0.f;
@@ -326,39 +330,123 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     for (int w = 0; w < kWarps; ++w) v += part[w * (E16 * T8) + e * T8 + t];
     logits[i] = v;
   }
-  if constexpr (CLUSTER) {
-    // every CTA adds the shares of its tokens, chooses for them and tells the others
-    cg::cluster_group cluster = cg::this_cluster();
-    float* full = part;
-    cluster.sync();
-    for (int i = threadIdx.x; i < p.T * p.E; i += kThreads) {
-      if (i / p.E % ranks != rank) continue;
-      float v = 0.f;
-      for (int k = 0; k < ranks; ++k) v += cluster.map_shared_rank(logits, k)[i];
-      full[i] = v;
-    }
-    __syncthreads();
-    choose_experts(p, full, r, weight, rank, ranks);
-    __syncthreads();
-    for (int i = threadIdx.x; i < routes; i += kThreads)
-      if (i / p.K % ranks == rank)
-        for (int k = 0; k < ranks; ++k)
-          if (k != rank) {
-            cluster.map_shared_rank(r.expert, k)[i] = r.expert[i];
-            cluster.map_shared_rank(weight, k)[i] = weight[i];
-          }
-    cluster.sync();
-  } else {
-    __syncthreads();
-    choose_experts(p, logits, r, weight, 0, 1);
-    __syncthreads();
+}
+
+__device__ __forceinline__ void publish(const Params& p, const Routing& r) {
+  const int routes = p.T * p.K;
+  if (threadIdx.x == 0) p.routing[0] = r.entries;
+  if (threadIdx.x < kEntries) p.routing[1 + threadIdx.x] = r.entry_expert[threadIdx.x] | (r.entry_tokens[threadIdx.x] << 8) | (r.entry_begin[threadIdx.x] << 16);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < routes; i += kThreads) {
+    p.routing[1 + kEntries + i] = r.order[i] | (r.token[i] << 16);
+    p.routing[1 + kEntries + routes + i] = __float_as_int(r.weight[i]);
   }
-  sort_routes(r, routes, p.E, p.K);
-  if (blockIdx.x == 0) {
-    if (threadIdx.x == 0) p.routing[0] = r.entries;
-    if (threadIdx.x < kEntries) p.routing[1 + threadIdx.x] = r.entry_expert[threadIdx.x] | (r.entry_tokens[threadIdx.x] << 8) | (r.entry_begin[threadIdx.x] << 16);
-    for (int i = threadIdx.x; i < routes; i += kThreads) p.routing[1 + kEntries + i] = r.order[i] | (r.token[i] << 16);
-    for (int i = threadIdx.x; i < (p.H + kDownRows - 1) / kDownRows; i += kThreads) p.arrived[i] = 0u;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < (p.H + kDownRows - 1) / kDownRows; i += kThreads) p.arrived[i] = 0u;
+}
+
+template <bool WEIGHTS>
+__device__ __forceinline__ void read_routing(const Params& p, Routing& r) {
+  const int routes = p.T * p.K, words = 1 + kEntries + (WEIGHTS ? 2 : 1) * routes;
+  constexpr int MOST = (1 + kEntries + (WEIGHTS ? 2 : 1) * kRoutes + kThreads - 1) / kThreads;
+  int v[MOST];                           // all loads before the first use
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) v[i] = threadIdx.x + i * kThreads < words ? __ldcg(p.routing + threadIdx.x + i * kThreads) : 0;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const int at = threadIdx.x + i * kThreads, route = at - 1 - kEntries;
+    if (at >= words) break;
+    if (at == 0) {
+      r.entries = v[i];
+    } else if (at <= kEntries) {
+      r.entry_expert[at - 1] = v[i] & 0xFF;
+      r.entry_tokens[at - 1] = (v[i] >> 8) & 0xFF;
+      r.entry_begin[at - 1] = (v[i] >> 16) & 0xFFFF;
+    } else if (route < routes) {
+      r.order[route] = v[i] & 0xFFFF;
+      r.token[route] = v[i] >> 16;
+    } else {
+      r.weight[route - routes] = __int_as_float(v[i]);
+    }
+  }
+  __syncthreads();
+}
+
+// ---- kernel 0, where the router is large: one cluster; its CTAs share the contraction, then the tokens ----
+constexpr int kRouteCluster = 8;
+__global__ void __launch_bounds__(kThreads)
+moe_route_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Routing r;
+  __shared__ int counts[kChunks][kExperts];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = int(cluster.block_rank()), warp = threadIdx.x >> 5;
+  float* logits = reinterpret_cast<float*>(smem);          // [T][E] of this CTA's columns
+  float* full = logits + p.T * p.E;
+  float* part = full + p.T * p.E;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  router_products(p, part, rank * kWarps + warp, kRouteCluster * kWarps);
+  __syncthreads();
+  add_logits(p, part, logits);
+  cluster.sync();
+  for (int i = threadIdx.x; i < p.T * p.E; i += kThreads) {
+    if (i / p.E % kRouteCluster != rank) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRouteCluster; ++k) v += cluster.map_shared_rank(logits, k)[i];
+    full[i] = v;
+  }
+  __syncthreads();
+  choose_experts(p, full, r, rank, kRouteCluster);
+  __syncthreads();
+  if (rank != 0) {
+    for (int i = threadIdx.x; i < p.T * p.K; i += kThreads)
+      if (i / p.K % kRouteCluster == rank) {
+        cluster.map_shared_rank(r.expert, 0)[i] = r.expert[i];
+        cluster.map_shared_rank(r.weight, 0)[i] = r.weight[i];
+      }
+  }
+  cluster.sync();
+  if (rank != 0) return;
+  sort_routes(r, counts, p.T * p.K, p.K);
+  publish(p, r);
+}
+
+// ---- kernel 1: gate and up projection, SwiGLU; ROUTED: kernel 0 has routed ----
+template <bool ROUTED>
+__global__ void __launch_bounds__(kThreads)
+moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Routing r;
+  __shared__ uint64_t bars[kWarps][kUpStages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int routes = p.T * p.K;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Ring ring;
+  ring.stages = kUpStages;
+  ring.base = smem + warp * kUpStages * kTile;
+  ring.bars = bars[warp];
+  ring.status = p.status;
+  ring.lane = lane;
+  ring.init();
+  if (threadIdx.x == 0) tma_prefetch_desc(&weights);
+  if constexpr (ROUTED) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    read_routing<true>(p, r);
+  } else {
+    __shared__ int counts[kChunks][kExperts];
+    float* part = reinterpret_cast<float*>(smem);          // partial logits, before the rings are used
+    float* logits = reinterpret_cast<float*>(smem + kUpRing);
+    router_products(p, part, warp, kWarps);
+    __syncthreads();
+    add_logits(p, part, logits);
+    __syncthreads();
+    choose_experts(p, logits, r, 0, 1);
+    __syncthreads();
+    sort_routes(r, counts, routes, p.K);
+    if (blockIdx.x == 0) publish(p, r);
+    fence_proxy_async_smem();            // the rings' memory held partial logits
+    __syncwarp();
   }
 
   const int tiles = (p.I + kUpRows - 1) / kUpRows, steps = (p.H + kUpCols - 1) / kUpCols;
@@ -367,13 +455,6 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   const int c0 = parts.begin(blockIdx.x), c1 = parts.begin(blockIdx.x + 1);
   const int i0 = c0 + part_begin<kWarps>(c1 - c0, warp), i1 = c0 + part_begin<kWarps>(c1 - c0, warp + 1);
   if (i0 == i1) return;
-  Ring ring;
-  ring.stages = kUpStages;
-  ring.base = smem + warp * kUpStages * kTile;
-  ring.bars = bars[warp];
-  ring.status = p.status;
-  ring.lane = lane;
-  ring.init();
   int left = (i1 - i0) * steps, ahead_step = 0, ahead_expert = i0 / tiles, ahead_tile = i0 % tiles;
   int expert = ahead_expert, tile_at = ahead_tile;
   auto next_copy = [&]() {
@@ -385,23 +466,12 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
       if (++ahead_tile == tiles) { ahead_tile = 0; ++ahead_expert; }
     }
   };
-  fence_proxy_async_smem();              // the ring's memory held partial logits
-  __syncwarp();
 #pragma unroll 1
   for (int s = 0; s < ring.stages; ++s) next_copy();
 
-  // The columns of the first eight tokens of a unit are loaded while the unit before is computed (two sets of registers in turn), those
-  // of more tokens in place.
+  // The columns of up to 16 tokens of a unit are loaded before its tile is waited for, those of more in place.
   struct Columns {
     uint4 v[kUpCols / 32];
-  };
-  const __nv_bfloat16* first_row = nullptr;
-  int n0 = 0, n = 0;
-  auto row_of = [&](int begin, int tokens, int j) { return p.x + (long long)r.token[begin + min(j * 8 + g, tokens - 1)] * p.ldx + c * 8; };
-  auto enter = [&]() {                   // the entry that `expert` points to
-    n0 = r.entry_begin[expert];
-    n = r.entry_tokens[expert];
-    first_row = row_of(n0, n, 0);
   };
   auto load = [&](Columns& b, const __nv_bfloat16* row, int step) {
     const __nv_bfloat16* src = row + step * kUpCols;
@@ -416,50 +486,14 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
       }
     }
   };
-  float acc[kColumns / 8][4], acc_odd[4];                  // the first product in two chains
-  int items = i1 - i0, step = 0, n0_item = 0, n_item = 0;
-  // one unit: its tile from the ring, its columns in `b`; the columns of the one behind it go to `other`
-  auto unit = [&](Columns& b, Columns& other) {
-    const uint8_t* tile = ring.wait() + g * (kUpCols * 2) + c * 16;
-    uint4 a[kUpCols / 32][2];
-#pragma unroll
-    for (int s = 0; s < kUpCols / 32; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) a[s][u] = *reinterpret_cast<const uint4*>(tile + u * (kUpRows * kUpCols * 2) + s * 64);
-    ring.taken();
-    next_copy();
-    if (step + 1 < steps) {
-      load(other, first_row, step + 1);
-    } else if (items > 1) {
-      if (++tile_at == tiles) { tile_at = 0; ++expert; enter(); }
-      load(other, first_row, 0);
-    }
-#pragma unroll
-    for (int s = 0; s < kUpCols / 32; ++s) {
-      mma_bf16(acc[0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.v[s].x, b.v[s].y);
-      mma_bf16(acc_odd, a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.v[s].z, b.v[s].w);
-    }
-#pragma unroll
-    for (int j = 1; j < kColumns / 8; ++j) {
-      if (j * 8 >= n_item) break;
-      load(b, row_of(n0_item, n_item, j), step);
-#pragma unroll
-      for (int s = 0; s < kUpCols / 32; ++s) {
-        mma_bf16(acc[j], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.v[s].x, b.v[s].y);
-        mma_bf16(acc[j], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.v[s].z, b.v[s].w);
-      }
-    }
-    ++step;
-  };
-  Columns even, odd;
-  enter();
-  load(even, first_row, 0);
 #pragma unroll 1
-  for (; items > 0; --items) {
-    const int row = tile_at * kUpRows + g;
-    n0_item = n0;
-    n_item = n;
-    step = 0;
+  for (int items = i1 - i0; items > 0; --items) {
+    const int row = tile_at * kUpRows + g, n0 = r.entry_begin[expert], n = r.entry_tokens[expert];
+    if (++tile_at == tiles) { tile_at = 0; ++expert; }
+    const __nv_bfloat16* rows[kColumns / 8];
+#pragma unroll
+    for (int j = 0; j < kColumns / 8; ++j) rows[j] = p.x + (long long)r.token[n0 + min(j * 8 + g, n - 1)] * p.ldx + c * 8;
+    float acc[kColumns / 8][4], acc_odd[4];                // the first product in two chains
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       acc_odd[i] = 0.f;
@@ -467,27 +501,47 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
       for (int j = 0; j < kColumns / 8; ++j) acc[j][i] = 0.f;
     }
 #pragma unroll 1
-    while (step + 1 < steps) {
-      unit(even, odd);
-      unit(odd, even);
-    }
-    if (step < steps) {
-      unit(even, odd);
-      even = odd;
+    for (int step = 0; step < steps; ++step) {
+      Columns b0, b1;
+      load(b0, rows[0], step);
+      if (n > 8) load(b1, rows[1], step);
+      const uint8_t* tile = ring.wait() + g * (kUpCols * 2) + c * 16;
+      uint4 a[kUpCols / 32][2];
+#pragma unroll
+      for (int s = 0; s < kUpCols / 32; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) a[s][u] = *reinterpret_cast<const uint4*>(tile + u * (kUpRows * kUpCols * 2) + s * 64);
+      ring.taken();
+      next_copy();
+#pragma unroll
+      for (int s = 0; s < kUpCols / 32; ++s) {
+        mma_bf16(acc[0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b0.v[s].x, b0.v[s].y);
+        mma_bf16(acc_odd, a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b0.v[s].z, b0.v[s].w);
+      }
+#pragma unroll
+      for (int j = 1; j < kColumns / 8; ++j) {
+        if (j * 8 >= n) break;
+        if (j > 1) load(b1, rows[j], step);
+#pragma unroll
+        for (int s = 0; s < kUpCols / 32; ++s) {
+          mma_bf16(acc[j], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b1.v[s].x, b1.v[s].y);
+          mma_bf16(acc[j], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b1.v[s].z, b1.v[s].w);
+        }
+      }
     }
     // ---- the hidden values of the item ----
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[0][i] += acc_odd[i];
 #pragma unroll
     for (int j = 0; j < kColumns / 8; ++j) {
-      if (j * 8 >= n_item) break;
+      if (j * 8 >= n) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int col = j * 8 + 2 * c + i;
-        if (col >= n_item || row >= p.I) continue;
-        const int route = r.order[n0_item + col];
+        if (col >= n || row >= p.I) continue;
+        const int route = r.order[n0 + col];
         const float gate = acc[j][i], up = acc[j][i + 2];
-        const float h = gate / (1.f + expf(-gate)) * up * weight[route];
+        const float h = gate / (1.f + expf(-gate)) * up * r.weight[route];
         const __nv_bfloat16 high = __float2bfloat16_rn(h);
         __nv_bfloat16* dst = p.hidden + (long long)route * p.I + row;
         dst[0] = high;
@@ -518,28 +572,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   ring.lane = lane;
   ring.init();
   asm volatile("griddepcontrol.wait;" ::: "memory");       // what follows reads what the first kernel wrote
-  {
-    constexpr int MOST = (1 + kEntries + kRoutes + kThreads - 1) / kThreads;
-    const int words = 1 + kEntries + routes;
-    int v[MOST];                         // all loads before the first use
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) v[i] = threadIdx.x + i * kThreads < words ? __ldcg(p.routing + threadIdx.x + i * kThreads) : 0;
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-      const int at = threadIdx.x + i * kThreads;
-      if (at == 0) {
-        r.entries = v[i];
-      } else if (at <= kEntries) {
-        r.entry_expert[at - 1] = v[i] & 0xFF;
-        r.entry_tokens[at - 1] = (v[i] >> 8) & 0xFF;
-        r.entry_begin[at - 1] = (v[i] >> 16) & 0xFFFF;
-      } else if (at < words) {
-        r.order[at - 1 - kEntries] = v[i] & 0xFFFF;
-        r.token[at - 1 - kEntries] = v[i] >> 16;
-      }
-    }
-  }
-  __syncthreads();
+  read_routing<false>(p, r);
   const int live = r.entries;
 
   const int steps = (p.I + kDownCols - 1) / kDownCols, tiles = (p.H + kDownRows - 1) / kDownRows;
@@ -578,15 +611,7 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   struct Columns {
     uint4 v[kDownCols / 32][2];
   };
-  const __nv_bfloat16* first_row = nullptr;
   const long long low = (long long)routes * p.I;           // from a high part to its low part
-  int ai = 0, n0 = 0, n = 0;
-  auto row_of = [&](int begin, int tokens, int j) { return p.hidden + (long long)r.order[begin + min(j * 8 + g, tokens - 1)] * p.I + c * 8; };
-  auto enter_entry = [&]() {
-    n0 = r.entry_begin[ai];
-    n = r.entry_tokens[ai];
-    first_row = row_of(n0, n, 0);
-  };
   auto load = [&](Columns& b, const __nv_bfloat16* row, int step) {
     const __nv_bfloat16 *src = row + step * kDownCols, *src_low = src + low;
     if ((step + 1) * kDownCols <= p.I) {
@@ -606,66 +631,20 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
       }
     }
   };
-  float acc[2][kColumns / 8][4];
-  auto multiply = [&](int j, const Columns& x, const uint4 (&a)[2][kDownCols / 32][2]) {
-#pragma unroll
-    for (int s = 0; s < kDownCols / 32; ++s)
-#pragma unroll
-      for (int v = 1; v >= 0; --v)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma_bf16(acc[m][j], a[m][s][0].x, a[m][s][1].x, a[m][s][0].y, a[m][s][1].y, x.v[s][v].x, x.v[s][v].y);
-          mma_bf16(acc[m][j], a[m][s][0].z, a[m][s][1].z, a[m][s][0].w, a[m][s][1].w, x.v[s][v].z, x.v[s][v].w);
-        }
-  };
   float* mine = sums + warp * sum_size;
-  int units = 0, step = 0, n0_now = 0, n_now = 0;
-  auto unit = [&](Columns& b, Columns& other) {
-    const uint8_t* at = ring.wait() + g * (kDownCols * 2) + c * 16;
-    uint4 a[2][kDownCols / 32][2];       // [row tile of 16][32 columns][rows g, g + 8]
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int s = 0; s < kDownCols / 32; ++s)
-#pragma unroll
-        for (int v = 0; v < 2; ++v) a[m][s][v] = *reinterpret_cast<const uint4*>(at + (16 * m + 8 * v) * (kDownCols * 2) + s * 64);
-    ring.taken();
-    next_copy();
-    if (units > 1) {
-      if (step + 1 < steps) {
-        load(other, first_row, step + 1);
-      } else {
-        ++ai;
-        enter_entry();
-        load(other, first_row, 0);
-      }
-    }
-    multiply(0, b, a);
-#pragma unroll
-    for (int j = 1; j < kColumns / 8; ++j) {
-      if (j * 8 >= n_now) break;
-      load(b, row_of(n0_now, n_now, j), step);
-      multiply(j, b, a);
-    }
-    ++step;
-    --units;
-  };
 #pragma unroll 1
   for (int tile = c0 / per_tile; tile * per_tile < c1; ++tile) {
     const int s0 = max(c0, tile * per_tile), s1 = min(c1, (tile + 1) * per_tile);
     const int u = s0 + part_begin<kWarps>(s1 - s0, warp);
-    units = s0 + part_begin<kWarps>(s1 - s0, warp + 1) - u;
-    Columns even, odd;
-    if (units > 0) {
-      ai = (u - tile * per_tile) / steps;
-      step = (u - tile * per_tile) % steps;
-      enter_entry();
-      load(even, first_row, step);
-    }
+    int units = s0 + part_begin<kWarps>(s1 - s0, warp + 1) - u;
+    int at_entry = (u - tile * per_tile) / steps, step = (u - tile * per_tile) % steps;
 #pragma unroll 1
-    while (units > 0) {                  // one entry of this row tile
-      n0_now = n0;
-      n_now = n;
+    for (; units > 0; ++at_entry) {      // one entry of this row tile
+      const int n0 = r.entry_begin[at_entry], n = r.entry_tokens[at_entry];
+      const __nv_bfloat16* rows[kColumns / 8];
+#pragma unroll
+      for (int j = 0; j < kColumns / 8; ++j) rows[j] = p.hidden + (long long)r.order[n0 + min(j * 8 + g, n - 1)] * p.I + c * 8;
+      float acc[2][kColumns / 8][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -673,24 +652,49 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
 #pragma unroll 1
-      while (units > 1 && step + 1 < steps) {
-        unit(even, odd);
-        unit(odd, even);
-      }
-      if (units > 0 && step < steps) {
-        unit(even, odd);
-        even = odd;
+      for (; units > 0 && step < steps; ++step, --units) {
+        Columns b0, b1;
+        load(b0, rows[0], step);
+        if (n > 8) load(b1, rows[1], step);
+        const uint8_t* at = ring.wait() + g * (kDownCols * 2) + c * 16;
+        uint4 a[2][kDownCols / 32][2];   // [row tile of 16][32 columns][rows g, g + 8]
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int s = 0; s < kDownCols / 32; ++s)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) a[m][s][v] = *reinterpret_cast<const uint4*>(at + (16 * m + 8 * v) * (kDownCols * 2) + s * 64);
+        ring.taken();
+        next_copy();
+        auto multiply = [&](int j, const Columns& x) {
+#pragma unroll
+          for (int s = 0; s < kDownCols / 32; ++s)
+#pragma unroll
+            for (int v = 1; v >= 0; --v)
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                mma_bf16(acc[m][j], a[m][s][0].x, a[m][s][1].x, a[m][s][0].y, a[m][s][1].y, x.v[s][v].x, x.v[s][v].y);
+                mma_bf16(acc[m][j], a[m][s][0].z, a[m][s][1].z, a[m][s][0].w, a[m][s][1].w, x.v[s][v].z, x.v[s][v].w);
+              }
+        };
+        multiply(0, b0);
+#pragma unroll
+        for (int j = 1; j < kColumns / 8; ++j) {
+          if (j * 8 >= n) break;
+          if (j > 1) load(b1, rows[j], step);
+          multiply(j, b1);
+        }
       }
       step = 0;
       // an entry has a token at most once, so the lanes of a warp write different sums
 #pragma unroll
       for (int j = 0; j < kColumns / 8; ++j) {
-        if (j * 8 >= n_now) break;
+        if (j * 8 >= n) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int col = j * 8 + 2 * c + i;
-          if (col >= n_now) continue;
-          float* dst = mine + r.token[n0_now + col] * kSumPitch + g;
+          if (col >= n) continue;
+          float* dst = mine + r.token[n0 + col] * kSumPitch + g;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             dst[16 * m] += acc[m][j][i];
@@ -759,43 +763,28 @@ bool encode_weights(CUtensorMap* map, const void* base, long long cols, long lon
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr int kCluster = 2;
+// Bytes of x and the router's weight up to which every CTA of the first kernel routes by itself.
+constexpr long long kRouteInPlace = 48 * 1024;
 
-size_t up_shared(int T, int E) { return size_t(kUpRing) + size_t(T) * E * 4; }
+size_t part_bytes(int T, int E) { return size_t(kWarps) * ((E + 15) / 16 * 16) * ((T + 7) / 8 * 8) * 4; }
+size_t route_shared(int T, int E) { return part_bytes(T, E) + size_t(2) * T * E * 4; }
+size_t up_shared(int T, int E, bool routed) { return size_t(kUpRing) + (routed ? 0 : size_t(T) * E * 4); }
 size_t down_shared(int T) { return size_t(kWarps) * down_stages(T) * kTile + size_t(kWarps) * T * kSumPitch * 4; }
 
-// What a launch needs to know of a device, found once.
-struct DeviceFacts {
-  std::once_flag once;
-  cudaError_t error = cudaSuccess;
-  int sms = 0, clustered = 0;            // CTAs of the first kernel that are resident at once in clusters
-};
-DeviceFacts& facts(int dev) {
-  static DeviceFacts all[64];
-  DeviceFacts& f = all[dev];
-  std::call_once(f.once, [&f] {
-    const int up = int(up_shared(kMoeTokensMax, kExperts));
-    const int down = int(down_shared(16) > down_shared(kMoeTokensMax) ? down_shared(16) : down_shared(kMoeTokensMax));
-    f.sms = device_sm_count();
-    if ((f.error = cudaFuncSetAttribute(moe_up_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, up)) != cudaSuccess) return;
-    if ((f.error = cudaFuncSetAttribute(moe_up_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, up)) != cudaSuccess) return;
-    if ((f.error = cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, down)) != cudaSuccess) return;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(f.sms / kCluster * kCluster));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = size_t(up);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int clusters = 0;
-    if ((f.error = cudaOccupancyMaxActiveClusters(&clusters, moe_up_kernel<true>, &cfg)) != cudaSuccess) return;
-    f.clustered = clusters * kCluster < f.sms ? clusters * kCluster : f.sms / kCluster * kCluster;
-    if (f.clustered < kCluster) f.error = cudaErrorInvalidConfiguration;
+// The kernels' shared memory, allowed once a device.
+cudaError_t prepare(int dev) {
+  static std::once_flag once[64];
+  static cudaError_t result[64];
+  std::call_once(once[dev], [dev] {
+    auto allow = [](auto kernel, size_t bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)); };
+    const size_t down = down_shared(16) > down_shared(kMoeTokensMax) ? down_shared(16) : down_shared(kMoeTokensMax);
+    cudaError_t e = allow(moe_route_kernel, route_shared(kMoeTokensMax, kExperts));
+    if (e == cudaSuccess) e = allow(moe_up_kernel<false>, up_shared(kMoeTokensMax, kExperts, false));
+    if (e == cudaSuccess) e = allow(moe_up_kernel<true>, up_shared(kMoeTokensMax, kExperts, true));
+    if (e == cudaSuccess) e = allow(moe_down_kernel, down);
+    result[dev] = e;
   });
-  return f;
+  return result[dev];
 }
 
 struct Workspace {                       // byte offsets of its parts
@@ -804,7 +793,7 @@ struct Workspace {                       // byte offsets of its parts
 Workspace workspace_of(int T, int K, int H, int I) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   Workspace w;
-  w.hidden = up(size_t(1 + kEntries + T * K) * 4);
+  w.hidden = up(size_t(1 + kEntries + 2 * T * K) * 4);
   w.part = w.hidden + up(size_t(2) * T * K * I * 2);
   w.arrived = w.part + up(size_t(2) * device_sm_count() * T * kDownRows * 4);
   w.total = w.arrived + up(size_t((H + kDownRows - 1) / kDownRows) * 4);
@@ -827,8 +816,8 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
     if ((err = cudaSetDevice(dev)) != cudaSuccess) return err;
     bound = dev;
   }
-  DeviceFacts& f = facts(dev);
-  if (f.error != cudaSuccess) return f.error;
+  if ((err = prepare(dev)) != cudaSuccess) return err;
+  const int sms = device_sm_count();
   const Workspace w = workspace_of(a.T, a.K, a.H, a.I);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   Params p;
@@ -851,26 +840,30 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   cfg.blockDim = dim3(kThreads);
   cfg.stream = a.stream;
   cfg.attrs = attr;
-  // What a CTA reads to route by itself (x and the router's weight, from L2); above 256 KB two CTAs share it.
-  const long long routing = (long long)a.E * a.H * (a.router_bf16 ? 2 : 4) + (long long)a.T * a.H * 2;
-  cfg.dynamicSmemBytes = up_shared(a.T, a.E);
-  ++g_launch_count;
-  if (routing > 256 * 1024) {
+  cfg.numAttrs = 0;
+  const bool routed = (long long)a.E * a.H * (a.router_bf16 ? 2 : 4) + (long long)a.T * a.H * 2 > kRouteInPlace;
+  if (routed) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.x = kRouteCluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3(unsigned(f.clustered));
-    err = cudaLaunchKernelEx(&cfg, moe_up_kernel<true>, up, p);
-  } else {
-    cfg.gridDim = dim3(unsigned(f.sms));
-    err = cudaLaunchKernelEx(&cfg, moe_up_kernel<false>, up, p);
+    cfg.gridDim = dim3(kRouteCluster);
+    cfg.dynamicSmemBytes = route_shared(a.T, a.E);
+    ++g_launch_count;
+    if ((err = cudaLaunchKernelEx(&cfg, moe_route_kernel, p)) != cudaSuccess) return err;
+    attr[0] = cudaLaunchAttribute{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
   }
+  cfg.gridDim = dim3(unsigned(sms));
+  cfg.dynamicSmemBytes = up_shared(a.T, a.E, routed);
+  ++g_launch_count;
+  err = routed ? cudaLaunchKernelEx(&cfg, moe_up_kernel<true>, up, p) : cudaLaunchKernelEx(&cfg, moe_up_kernel<false>, up, p);
   if (err != cudaSuccess) return err;
+  attr[0] = cudaLaunchAttribute{};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3(unsigned(f.sms));
   cfg.dynamicSmemBytes = down_shared(a.T);
   ++g_launch_count;
   return cudaLaunchKernelEx(&cfg, moe_down_kernel, down, p);
