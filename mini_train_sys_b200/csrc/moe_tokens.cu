@@ -48,7 +48,6 @@ constexpr int kSumPitch = kDownRows + 1;
 // Stages of a warp's ring in the first kernel, and in the second, whose sums need room too.
 constexpr int kUpStages = 3;
 __host__ __device__ constexpr int down_stages(int T) { return T <= 16 ? 3 : 2; }
-constexpr int kUpRing = kWarps * kUpStages * kTile;
 
 // The routes sorted by expert, and the entries that the weights are streamed for: an expert with at most kColumns of its tokens (one
 // with more has several and is read as often).
@@ -75,6 +74,7 @@ struct Params {
   float* part;                 // [2 * CTAs][T][32]
   int* status;
   int T, E, K, H, I, normalize;
+  int up_warps, down_warps;    // warps of a CTA that stream: no more than can have work, so that small problems leave shared memory free
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -133,6 +133,25 @@ struct Ring {
 // of 32 by a vote, those of the chunks before by a running sum, so that it does not depend on timing.
 __device__ __forceinline__ void sort_routes(Routing& r, int (*counts)[kExperts], int routes, int K) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (routes <= 32) {                    // one warp, by comparison
+    if (warp == 0) {
+      const int e = lane < routes ? r.expert[lane] : kExperts;
+      const unsigned same = __match_any_sync(0xffffffffu, e), below = (1u << lane) - 1;
+      const unsigned leaders = __ballot_sync(0xffffffffu, lane < routes && (same & below) == 0u);
+      int to = __popc(same & below), entry = 0;
+#pragma unroll 1
+      for (int j = 0; j < routes; ++j) {
+        const int other = __shfl_sync(0xffffffffu, e, j);
+        to += other < e;
+        entry += other < e && ((leaders >> j) & 1u);
+      }
+      if (lane < routes) { r.order[to] = lane; r.token[to] = lane / K; }
+      if ((leaders >> lane) & 1u) { r.entry_expert[entry] = e; r.entry_begin[entry] = to; r.entry_tokens[entry] = __popc(same); }
+      if (lane == 0) r.entries = __popc(leaders);
+    }
+    __syncthreads();
+    return;
+  }
   for (int i = threadIdx.x; i < kChunks * kExperts; i += kThreads) counts[i / kExperts][i % kExperts] = 0;
   __syncthreads();
   constexpr int MINE = kChunks / kWarps;
@@ -194,12 +213,21 @@ __device__ __forceinline__ void sort_routes(Routing& r, int (*counts)[kExperts],
 }
 
 // One warp a token: K rounds of arg-max over the logits (two experts a lane), the first of which is the softmax's maximum.
-// The tokens of this CTA are rank, rank + ranks, ...
-__device__ __forceinline__ void choose_experts(const Params& p, const float* logits, Routing& r, int rank, int ranks) {
+// A logit is the sum of `parts` values, the first at [e * se + t * st].  The tokens of this CTA are rank, rank + ranks, ...
+__device__ __forceinline__ void choose_experts(const Params& p, const float* logits, int parts, int pitch, int se, int st, Routing& r, int rank,
+                                               int ranks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll 1
   for (int t = rank + ranks * warp; t < p.T; t += ranks * kWarps) {
-    const float v0 = lane < p.E ? logits[t * p.E + lane] : -CUDART_INF_F, v1 = lane + 32 < p.E ? logits[t * p.E + lane + 32] : -CUDART_INF_F;
+    float v0 = 0.f, v1 = 0.f;
+#pragma unroll 8
+    for (int w = 0; w < parts; ++w) {
+      const float* at = logits + w * pitch + t * st;
+      if (lane < p.E) v0 += at[lane * se];
+      if (lane + 32 < p.E) v1 += at[(lane + 32) * se];
+    }
+    if (lane >= p.E) v0 = -CUDART_INF_F;
+    if (lane + 32 >= p.E) v1 = -CUDART_INF_F;
     auto key_of = [](float v) {                            // unsigned order = float order; 0 is "taken", which a negative NaN still beats
       const unsigned u = __float_as_uint(v);
       return max((u & 0x80000000u) ? ~u : (u | 0x80000000u), 1u);
@@ -319,6 +347,48 @@ __device__ __forceinline__ void router_products(const Params& p, float* part, in
   }
 }
 
+// The logits [t][e] of up to four tokens: a warp an expert, all loads of 1024 columns in flight, every sum in the same order.
+constexpr int kFewTokens = 4;
+__device__ __forceinline__ void router_few(const Params& p, float* logits) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int e = threadIdx.x >> 5; e < p.E; e += kWarps) {
+    float acc[kFewTokens] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int d = lane * 8; d < p.H; d += 256) {
+      float w[8];
+      if (p.router_bf16) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.router) + (long long)e * p.H + d));
+        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { w[2 * i] = __uint_as_float(v[i] << 16); w[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u); }
+      } else {
+        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + (long long)e * p.H + d);
+        const float4 a = __ldg(src), b = __ldg(src + 1);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+      }
+#pragma unroll
+      for (int t = 0; t < kFewTokens; ++t) {
+        if (t >= p.T) break;
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.ldx + d));
+        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[t] = fmaf(__uint_as_float(v[i] << 16), w[2 * i], acc[t]);
+          acc[t] = fmaf(__uint_as_float(v[i] & 0xFFFF0000u), w[2 * i + 1], acc[t]);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kFewTokens; ++t) {
+      if (t >= p.T) break;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], off);
+      if (lane == 0) logits[t * p.E + e] = acc[t];
+    }
+  }
+}
+
 // What the CTA's warps have of the logits, added.
 __device__ __forceinline__ void add_logits(const Params& p, const float* part, float* logits) {
   const int E16 = (p.E + 15) & ~15, T8 = (p.T + 7) & ~7;
@@ -397,7 +467,7 @@ moe_route_kernel(const Params p) {
     full[i] = v;
   }
   __syncthreads();
-  choose_experts(p, full, r, rank, kRouteCluster);
+  choose_experts(p, full, 1, 0, 1, p.E, r, rank, kRouteCluster);
   __syncthreads();
   if (rank != 0) {
     for (int i = threadIdx.x; i < p.T * p.K; i += kThreads)
@@ -436,16 +506,19 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   } else {
     __shared__ int counts[kChunks][kExperts];
     float* part = reinterpret_cast<float*>(smem);          // partial logits, before the rings are used
-    float* logits = reinterpret_cast<float*>(smem + kUpRing);
-    router_products(p, part, warp, kWarps);
-    __syncthreads();
-    add_logits(p, part, logits);
-    __syncthreads();
-    choose_experts(p, logits, r, 0, 1);
+    const int E16 = (p.E + 15) & ~15, T8 = (p.T + 7) & ~7;
+    if (p.T <= kFewTokens) {
+      router_few(p, part);
+      __syncthreads();
+      choose_experts(p, part, 1, 0, 1, p.E, r, 0, 1);
+    } else {
+      router_products(p, part, warp, kWarps);
+      __syncthreads();
+      choose_experts(p, part, kWarps, E16 * T8, T8, 1, r, 0, 1);
+    }
     __syncthreads();
     sort_routes(r, counts, routes, p.K);
-    if (blockIdx.x == 0) publish(p, r);
-    fence_proxy_async_smem();            // the rings' memory held partial logits
+    fence_proxy_async_smem();            // the rings' memory held the logits
     __syncwarp();
   }
 
@@ -453,8 +526,8 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   const int N = r.entries * tiles;
   const Parts parts(N, gridDim.x);
   const int c0 = parts.begin(blockIdx.x), c1 = parts.begin(blockIdx.x + 1);
-  const int i0 = c0 + part_begin<kWarps>(c1 - c0, warp), i1 = c0 + part_begin<kWarps>(c1 - c0, warp + 1);
-  if (i0 == i1) return;
+  const Parts shares(c1 - c0, p.up_warps);
+  const int i0 = c0 + shares.begin(min(warp, p.up_warps)), i1 = c0 + shares.begin(min(warp + 1, p.up_warps));
   int left = (i1 - i0) * steps, ahead_step = 0, ahead_expert = i0 / tiles, ahead_tile = i0 % tiles;
   int expert = ahead_expert, tile_at = ahead_tile;
   auto next_copy = [&]() {
@@ -468,6 +541,9 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   };
 #pragma unroll 1
   for (int s = 0; s < ring.stages; ++s) next_copy();
+  if constexpr (!ROUTED) {
+    if (blockIdx.x == 0) publish(p, r);
+  }
 
   // The columns of up to 16 tokens of a unit are loaded before its tile is waited for, those of more in place.
   struct Columns {
@@ -561,8 +637,9 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int routes = p.T * p.K, sum_size = p.T * kSumPitch;
-  float* sums = reinterpret_cast<float*>(smem + kWarps * down_stages(p.T) * kTile);       // [warps][T][pitch]
-  for (int i = threadIdx.x; i < kWarps * sum_size; i += kThreads) sums[i] = 0.f;
+  float* sums = reinterpret_cast<float*>(smem + p.down_warps * down_stages(p.T) * kTile); // [warps][T][pitch]
+#pragma unroll 1
+  for (int i = threadIdx.x; i < p.down_warps * sum_size; i += kThreads) sums[i] = 0.f;
   if (threadIdx.x == 0) tma_prefetch_desc(&weights);
   Ring ring;
   ring.stages = down_stages(p.T);
@@ -587,8 +664,9 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   auto enter = [&](Stream& s) {          // the first row tile from s.tile on that has units for this warp
     for (; s.tile * per_tile < c1; ++s.tile) {
       const int s0 = max(c0, s.tile * per_tile), s1 = min(c1, (s.tile + 1) * per_tile);
-      s.u = s0 + part_begin<kWarps>(s1 - s0, warp);
-      s.end = s0 + part_begin<kWarps>(s1 - s0, warp + 1);
+      const Parts shares(s1 - s0, p.down_warps);
+      s.u = s0 + shares.begin(min(warp, p.down_warps));
+      s.end = s0 + shares.begin(min(warp + 1, p.down_warps));
       if (s.u == s.end) continue;
       s.expert = (s.u - s.tile * per_tile) / steps;
       s.step = (s.u - s.tile * per_tile) % steps;
@@ -635,8 +713,9 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
 #pragma unroll 1
   for (int tile = c0 / per_tile; tile * per_tile < c1; ++tile) {
     const int s0 = max(c0, tile * per_tile), s1 = min(c1, (tile + 1) * per_tile);
-    const int u = s0 + part_begin<kWarps>(s1 - s0, warp);
-    int units = s0 + part_begin<kWarps>(s1 - s0, warp + 1) - u;
+    const Parts shares(s1 - s0, p.down_warps);
+    const int u = s0 + shares.begin(min(warp, p.down_warps));
+    int units = s0 + shares.begin(min(warp + 1, p.down_warps)) - u;
     int at_entry = (u - tile * per_tile) / steps, step = (u - tile * per_tile) % steps;
 #pragma unroll 1
     for (; units > 0; ++at_entry) {      // one entry of this row tile
@@ -707,17 +786,21 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     __syncthreads();
     const bool whole = s0 == tile * per_tile && s1 == (tile + 1) * per_tile;
     float* own = p.part + (2 * (long long)blockIdx.x + (s0 == tile * per_tile ? 1 : 0)) * p.T * kDownRows;
-    for (int i = threadIdx.x; i < p.T * kDownRows; i += kThreads) {
-      const int t = i / kDownRows, row = i % kDownRows;
-      float v = 0.f;
+    // four rows of a token a thread
+    auto store = [&](int i, const float (&v)[4]) {
+      const int t = i / kDownRows, row = tile * kDownRows + i % kDownRows;
+      if (row < p.H) *reinterpret_cast<uint2*>(p.y + (long long)t * p.H + row) = make_uint2(pack_bf162(v[0], v[1]), pack_bf162(v[2], v[3]));
+    };
+#pragma unroll 1
+    for (int i = threadIdx.x * 4; i < p.T * kDownRows; i += kThreads * 4) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      float* at = sums + i / kDownRows * kSumPitch + i % kDownRows;
+#pragma unroll 4
+      for (int w = 0; w < p.down_warps; ++w, at += sum_size)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        float* s = sums + w * sum_size + t * kSumPitch + row;
-        v += *s;
-        *s = 0.f;
-      }
-      if (!whole) own[i] = v;
-      else if (tile * kDownRows + row < p.H) p.y[(long long)t * p.H + tile * kDownRows + row] = __float2bfloat16_rn(v);
+        for (int k = 0; k < 4; ++k) { v[k] += at[k]; at[k] = 0.f; }
+      if (whole) store(i, v);
+      else *reinterpret_cast<float4*>(own + i) = make_float4(v[0], v[1], v[2], v[3]);
     }
     if (!whole) {
       const int f = parts.owner(tile * per_tile), l = parts.owner((tile + 1) * per_tile - 1);
@@ -728,15 +811,22 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
         __threadfence();
       }
       __syncthreads();
-      if (last)
-        for (int i = threadIdx.x; i < p.T * kDownRows; i += kThreads) {
-          const int t = i / kDownRows, row = tile * kDownRows + i % kDownRows;
-          float v = 0.f;
+      if (last) {
+        // the row tile begins in CTA f, whose second part it is; the others begin with it
+        const float* from = p.part + (2 * (long long)f + 1) * p.T * kDownRows;
+        const float* rest = p.part + 2 * (long long)(f + 1) * p.T * kDownRows;
+#pragma unroll 1
+        for (int i = threadIdx.x * 4; i < p.T * kDownRows; i += kThreads * 4) {
+          const float4 q = __ldcg(reinterpret_cast<const float4*>(from + i));
+          float v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll 8
-          for (int k = f; k <= l; ++k)
-            v += __ldcg(p.part + (2 * (long long)k + (parts.begin(k) <= tile * per_tile ? 1 : 0)) * p.T * kDownRows + i);
-          if (row < p.H) p.y[(long long)t * p.H + row] = __float2bfloat16_rn(v);
+          for (int k = 0; k < l - f; ++k) {
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(rest + 2 * (long long)k * p.T * kDownRows + i));
+            v[0] += o.x; v[1] += o.y; v[2] += o.z; v[3] += o.w;
+          }
+          store(i, v);
         }
+      }
     }
     __syncthreads();                     // the sums are zero again, `last` is read
   }
@@ -768,8 +858,11 @@ constexpr long long kRouteInPlace = 48 * 1024;
 
 size_t part_bytes(int T, int E) { return size_t(kWarps) * ((E + 15) / 16 * 16) * ((T + 7) / 8 * 8) * 4; }
 size_t route_shared(int T, int E) { return part_bytes(T, E) + size_t(2) * T * E * 4; }
-size_t up_shared(int T, int E, bool routed) { return size_t(kUpRing) + (routed ? 0 : size_t(T) * E * 4); }
-size_t down_shared(int T) { return size_t(kWarps) * down_stages(T) * kTile + size_t(kWarps) * T * kSumPitch * 4; }
+size_t up_shared(int T, int E, int warps, bool routed) {
+  const size_t ring = size_t(warps) * kUpStages * kTile, part = routed ? 0 : part_bytes(T, E);
+  return ring > part ? ring : part;
+}
+size_t down_shared(int T, int warps) { return size_t(warps) * (down_stages(T) * kTile + T * kSumPitch * 4); }
 
 // The kernels' shared memory, allowed once a device.
 cudaError_t prepare(int dev) {
@@ -777,10 +870,10 @@ cudaError_t prepare(int dev) {
   static cudaError_t result[64];
   std::call_once(once[dev], [dev] {
     auto allow = [](auto kernel, size_t bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)); };
-    const size_t down = down_shared(16) > down_shared(kMoeTokensMax) ? down_shared(16) : down_shared(kMoeTokensMax);
+    const size_t few = down_shared(16, kWarps), many = down_shared(kMoeTokensMax, kWarps), down = few > many ? few : many;
     cudaError_t e = allow(moe_route_kernel, route_shared(kMoeTokensMax, kExperts));
-    if (e == cudaSuccess) e = allow(moe_up_kernel<false>, up_shared(kMoeTokensMax, kExperts, false));
-    if (e == cudaSuccess) e = allow(moe_up_kernel<true>, up_shared(kMoeTokensMax, kExperts, true));
+    if (e == cudaSuccess) e = allow(moe_up_kernel<false>, up_shared(kMoeTokensMax, kExperts, kWarps, false));
+    if (e == cudaSuccess) e = allow(moe_up_kernel<true>, up_shared(kMoeTokensMax, kExperts, kWarps, true));
     if (e == cudaSuccess) e = allow(moe_down_kernel, down);
     result[dev] = e;
   });
@@ -818,6 +911,11 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   }
   if ((err = prepare(dev)) != cudaSuccess) return err;
   const int sms = device_sm_count();
+  // upper bounds of the items and units, hence of the warps that can have some
+  const long long entries = ((long long)a.T * a.K < a.E ? a.T * a.K : a.E) + a.T * a.K / kColumns;
+  const long long items = entries * ((a.I + kUpRows - 1) / kUpRows);
+  const long long units = entries * ((a.H + kDownRows - 1) / kDownRows) * ((a.I + kDownCols - 1) / kDownCols);
+  auto warps_for = [sms](long long n) { return n >= (long long)sms * kWarps ? kWarps : int((n + sms - 1) / sms); };
   const Workspace w = workspace_of(a.T, a.K, a.H, a.I);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   Params p;
@@ -830,6 +928,7 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   p.arrived = reinterpret_cast<unsigned*>(ws + w.arrived);
   p.status = a.status;
   p.T = a.T; p.E = a.E; p.K = a.K; p.H = a.H; p.I = a.I; p.normalize = a.normalize;
+  p.up_warps = warps_for(items); p.down_warps = warps_for(units);
   CUtensorMap up, down;
   if (!encode_weights(&up, a.gate_up, a.H, a.I, 2LL * a.E, kUpCols, kUpRows, 2) ||
       !encode_weights(&down, a.down, a.I, a.H, a.E, kDownCols, kDownRows, 1))
@@ -856,7 +955,7 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
   }
   cfg.gridDim = dim3(unsigned(sms));
-  cfg.dynamicSmemBytes = up_shared(a.T, a.E, routed);
+  cfg.dynamicSmemBytes = up_shared(a.T, a.E, p.up_warps, routed);
   ++g_launch_count;
   err = routed ? cudaLaunchKernelEx(&cfg, moe_up_kernel<true>, up, p) : cudaLaunchKernelEx(&cfg, moe_up_kernel<false>, up, p);
   if (err != cudaSuccess) return err;
@@ -864,7 +963,7 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  cfg.dynamicSmemBytes = down_shared(a.T);
+  cfg.dynamicSmemBytes = down_shared(a.T, p.down_warps);
   ++g_launch_count;
   return cudaLaunchKernelEx(&cfg, moe_down_kernel, down, p);
 }
