@@ -5,6 +5,7 @@
 // For 16-bit x the product 127 x is exact in fp32 and 127 x / a is either a half exactly or at least 2^-12 away from one, so
 // a correctly rounded quotient gives the code that exact arithmetic gives.
 #include "decode.cuh"
+#include "launch.cuh"
 #include "ops.cuh"
 #include "mma_sync.cuh"
 
@@ -62,33 +63,30 @@ constexpr int kAppendThreads = 256;
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads)
 kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __restrict__ q_out, const T* __restrict__ cosv,
-                 const T* __restrict__ sinv, int table_rows, int Tn, int kv_ctas, int blocks_per_head) {
+                 const T* __restrict__ sinv, int table_rows, int Tn, int kv_ctas, int q_ctas, int blocks_per_head) {
   constexpr int VEC = D / 16;                              // threads per token
   constexpr int ITER = (kCacheBlock * VEC + kAppendThreads - 1) / kAppendThreads;
   constexpr int BLK = kCacheBlock;
   const int tid = threadIdx.x;
-  if (int(blockIdx.x) >= kv_ctas) {                        // ---- q ----
-    const long long total = (long long)c.B * Hq * Tn * VEC;
-    for (long long i = (long long)(blockIdx.x - kv_ctas) * kAppendThreads + tid; i < total;
-         i += (long long)(gridDim.x - kv_ctas) * kAppendThreads) {
-      const int vec = int(i % VEC);
-      long long r = i / VEC;
-      const int h = int(r % Hq); r /= Hq;
-      const int t = int(r % Tn);
-      const int b = int(r / Tn);
-      T* dst = q_out + (((long long)b * Tn + t) * Hq + h) * D + vec * 8;
-      Vec8T<T> lo, hi;
-      lo.q = hi.q = make_uint4(0, 0, 0, 0);
-      const int p = c.start[b] + t;
-      if (t < c.count[b] && p >= 0 && p < c.blocks * BLK) {
-        const T* src = static_cast<const T*>(q.p) + b * q.sb + h * q.sh + t * q.st + vec * 8;
-        lo.q = *reinterpret_cast<const uint4*>(src);
-        hi.q = *reinterpret_cast<const uint4*>(src + D / 2);
-        if (cosv != nullptr && p < table_rows) rotate8(lo, hi, cosv + (long long)p * D + vec * 8, sinv + (long long)p * D + vec * 8);
-      }
-      *reinterpret_cast<uint4*>(dst) = lo.q;
-      *reinterpret_cast<uint4*>(dst + D / 2) = hi.q;
+  let_next_start();
+  wait_for_previous();
+  if (int(blockIdx.x) >= kv_ctas) {                        // ---- q: a CTA takes consecutive pieces of one sequence ----
+    const unsigned per_token = unsigned(Hq) * VEC, pieces = unsigned(Tn) * per_token;    // at most 2^31, checked by the launcher
+    const unsigned at = unsigned(blockIdx.x) - unsigned(kv_ctas), b = at / unsigned(q_ctas), piece = at % unsigned(q_ctas) * kAppendThreads + tid;
+    if (piece >= pieces) return;
+    const unsigned t = piece / per_token, rest = piece % per_token, h = rest / VEC, vec = rest % VEC;
+    T* dst = q_out + (((long long)b * Tn + t) * Hq + h) * D + vec * 8;
+    Vec8T<T> lo, hi;
+    lo.q = hi.q = make_uint4(0, 0, 0, 0);
+    const int p = c.start[b] + int(t);
+    if (int(t) < c.count[b] && p >= 0 && p < c.blocks * BLK) {
+      const T* src = static_cast<const T*>(q.p) + b * q.sb + h * q.sh + t * q.st + vec * 8;
+      lo.q = *reinterpret_cast<const uint4*>(src);
+      hi.q = *reinterpret_cast<const uint4*>(src + D / 2);
+      if (cosv != nullptr && p < table_rows) rotate8(lo, hi, cosv + (long long)p * D + vec * 8, sinv + (long long)p * D + vec * 8);
     }
+    *reinterpret_cast<uint4*>(dst) = lo.q;
+    *reinterpret_cast<uint4*>(dst + D / 2) = hi.q;
     return;
   }
 
@@ -218,56 +216,81 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
   }
 }
 
-// One CTA per 64 positions of a (sequence, K/V head); consecutive threads take consecutive positions, so that the bytes of one
-// V row are read together.
+// One CTA per 64 positions of a (sequence, K/V head), which lie in two blocks at most.  The values of a block are stored by dim, so
+// they pass through shared memory; then D / 8 consecutive threads write the dims of one token.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restrict__ ko, float* __restrict__ vo, int chunks) {
   constexpr int BLK = kCacheBlock;
+  constexpr int PITCH = BLK + 4;                           // bytes of a row of codes
+  constexpr int HALF_PITCH = BLK / 2 + 2;                  // values of a row of half the unfinished block
+  __shared__ __align__(16) uint8_t codes_sm[2][D * PITCH];
+  __shared__ __align__(16) T tail_sm[2 * D * HALF_PITCH];
+  let_next_start();
+  wait_for_previous();
   const int chunk = int(blockIdx.x) % chunks;
   const int bh = int(blockIdx.x) / chunks;
   const int b = bh / c.Hkv;
-  const int total = min(min(max(c.start[b], 0), c.blocks * BLK) + max(c.count[b], 0), c.blocks * BLK);
-  const int tok = threadIdx.x & 63;
-  const int i = chunk * 64 + tok;
-  if (i >= n) return;
-  const long long p = (long long)first[b] + i;
-  const bool live = p >= 0 && p < total;
-  const int blk = live ? int(p / BLK) : 0, at = live ? int(p % BLK) : 0;
-  const bool open = blk == total / BLK;
-  const uint8_t* record = c.records + ((long long)bh * c.blocks + blk) * record_bytes(D);
-  const uint8_t* kc = record + kCacheHead;
-  const T* tk = static_cast<const T*>(c.tail) + ((long long)bh * 2 + (blk & 1)) * 2 * BLK * D;
-  float ks = 0.f, vs = 0.f;
-  if (live && !open) {
-    const float* sc = reinterpret_cast<const float*>(record);
-    ks = sc[0];
-    vs = sc[1];
+  const int total = min(min(max(c.start[b], 0), c.blocks * BLK) + max(c.count[b], 0), c.blocks * BLK), closed = total / BLK;
+  const long long p0 = (long long)first[b] + chunk * 64;
+  const int lo = int(max(p0, 0ll) / BLK);                  // the two blocks
+  const uint8_t* record0 = c.records + ((long long)bh * c.blocks + lo) * record_bytes(D);
+  const T* tail = static_cast<const T*>(c.tail) + ((long long)bh * 2 + (closed & 1)) * 2 * BLK * D;
+  const bool reaches = p0 + 64 > 0 && p0 < total;          // else only zeros are written
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (!reaches || lo + j > closed || (lo + j) * (long long)BLK >= total) continue;
+    if (lo + j < closed) {
+      const uint8_t* vc = record0 + j * record_bytes(D) + kCacheHead + BLK * D;
+      for (int i = threadIdx.x; i < D * BLK / 16; i += 256) {
+        const uint4 w = *reinterpret_cast<const uint4*>(vc + i * 16);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(&codes_sm[j][i / 4 * PITCH + i % 4 * 16]);
+        dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
+      }
+    } else {
+      for (int i = threadIdx.x; i < D * BLK / 8; i += 256) {
+        const uint4 w = *reinterpret_cast<const uint4*>(tail + BLK * D + i * 8);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(&tail_sm[i / 4 * HALF_PITCH + i % 4 * 8]);
+        dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
+      }
+    }
   }
-  const int slot = cache_slot(at);
-  float* kd = ko + ((long long)bh * n + i) * D;
-  float* vd = vo + ((long long)bh * n + i) * D;
-  for (int d = (threadIdx.x >> 6) * 8; d < D; d += 32) {
+  __syncthreads();
+  constexpr int VEC = D / 8;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < 64 * VEC; i += 256) {
+    const int tok = i / VEC, d = i % VEC * 8, at_out = chunk * 64 + tok;
+    if (at_out >= n) break;
+    const long long p = p0 + tok;
     float kf[8], vf[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) kf[j] = vf[j] = 0.f;
-    if (live && open) {
-      Vec8T<T> x;
-      x.q = *reinterpret_cast<const uint4*>(tk + at * D + d);
+    if (p >= 0 && p < total) {
+      const int blk = int(p / BLK), at = int(p % BLK);
+      if (blk < closed) {
+        const uint8_t* record = record0 + (blk - lo) * record_bytes(D);
+        const float2 sc = *reinterpret_cast<const float2*>(record);
+        const uint2 w = *reinterpret_cast<const uint2*>(record + kCacheHead + at * D + d);
+        const uint8_t* vs = &codes_sm[blk - lo][d * PITCH + cache_slot(at)];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { kf[j] = to_f(x.v[j]); vf[j] = to_f(tk[BLK * D + tail_slot(D, d + j, at)]); }
-    } else if (live) {
-      const uint2 w = *reinterpret_cast<const uint2*>(kc + at * D + d);
+        for (int j = 0; j < 8; ++j) {
+          kf[j] = float(int(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xFFu) - 128) * sc.x;
+          vf[j] = float(int(vs[j * PITCH]) - 128) * sc.y;
+        }
+      } else {
+        Vec8T<T> x;
+        x.q = *reinterpret_cast<const uint4*>(tail + at * D + d);
+        const T* vs = tail_sm + ((at >> 5) * D + d) * HALF_PITCH + tail_slot(0, 0, at & 31);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        kf[j] = float(int(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xFFu) - 128) * ks;
-        vf[j] = float(int(kc[BLK * D + (d + j) * BLK + slot]) - 128) * vs;
+        for (int j = 0; j < 8; ++j) { kf[j] = to_f(x.v[j]); vf[j] = to_f(vs[j * HALF_PITCH]); }
       }
     }
-    *reinterpret_cast<float4*>(kd + d) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-    *reinterpret_cast<float4*>(kd + d + 4) = make_float4(kf[4], kf[5], kf[6], kf[7]);
-    *reinterpret_cast<float4*>(vd + d) = make_float4(vf[0], vf[1], vf[2], vf[3]);
-    *reinterpret_cast<float4*>(vd + d + 4) = make_float4(vf[4], vf[5], vf[6], vf[7]);
+    float* kd = ko + ((long long)bh * n + at_out) * D + d;
+    float* vd = vo + ((long long)bh * n + at_out) * D + d;
+    *reinterpret_cast<float4*>(kd) = make_float4(kf[0], kf[1], kf[2], kf[3]);
+    *reinterpret_cast<float4*>(kd + 4) = make_float4(kf[4], kf[5], kf[6], kf[7]);
+    *reinterpret_cast<float4*>(vd) = make_float4(vf[0], vf[1], vf[2], vf[3]);
+    *reinterpret_cast<float4*>(vd + 4) = make_float4(vf[4], vf[5], vf[6], vf[7]);
   }
 }
 
@@ -276,14 +299,12 @@ cudaError_t append_typed(const CacheView& c, const Strided& q, int Hq, const Str
                          const void* sinv, int table_rows, int Tn, cudaStream_t stream) {
   const int per_head = (Tn + kCacheBlock - 2) / kCacheBlock + 1;       // blocks that T tokens can touch
   const long long kv_ctas = (long long)c.B * c.Hkv * per_head;
-  const long long q_threads = q.p == nullptr ? 0 : (long long)c.B * Hq * Tn * (D / 16);
-  const long long q_want = (q_threads + kAppendThreads - 1) / kAppendThreads, q_cap = (long long)device_sm_count() * 16;
-  const long long q_ctas = q_want < q_cap ? q_want : q_cap;
-  if (kv_ctas + q_ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  kv_append_kernel<T, D><<<unsigned(kv_ctas + q_ctas), kAppendThreads, 0, stream>>>(
-      c, q, Hq, k, v, static_cast<T*>(q_out), static_cast<const T*>(cosv), static_cast<const T*>(sinv), table_rows, Tn, int(kv_ctas), per_head);
+  const long long pieces = q.p == nullptr ? 0 : (long long)Hq * Tn * (D / 16);
+  const long long q_ctas = (pieces + kAppendThreads - 1) / kAppendThreads;               // of a sequence
+  if (kv_ctas + q_ctas * c.B > 0x7fffffffll || pieces > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   ++g_launch_count;
-  return cudaGetLastError();
+  return launch_chained(kv_append_kernel<T, D>, dim3(unsigned(kv_ctas + q_ctas * c.B)), kAppendThreads, 0, 0, stream, c, q, Hq, k, v, static_cast<T*>(q_out),
+                        static_cast<const T*>(cosv), static_cast<const T*>(sinv), table_rows, Tn, int(kv_ctas), int(q_ctas), per_head);
 }
 
 template <typename T, int D>
@@ -291,9 +312,8 @@ cudaError_t read_typed(const CacheView& c, const int* first, int n, float* k, fl
   const int chunks = (n + 63) / 64;
   const long long ctas = (long long)c.B * c.Hkv * chunks;
   if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  kv_read_kernel<T, D><<<unsigned(ctas), 256, 0, stream>>>(c, first, n, k, v, chunks);
   ++g_launch_count;
-  return cudaGetLastError();
+  return launch_chained(kv_read_kernel<T, D>, dim3(unsigned(ctas)), 256, 0, 0, stream, c, first, n, k, v, chunks);
 }
 
 }  // namespace

@@ -18,6 +18,7 @@
 // Rounding: logits, softmax, sums and the hidden values are fp32 (the router's fp32 weight enters the tensor cores as the sum of three
 // bf16 values, 24 bits); a hidden value enters the second product as the sum of two (2^-16), so y is rounded to bf16 once.
 #include "decode.cuh"
+#include "launch.cuh"
 #include "ops.cuh"
 #include "mma_sync.cuh"
 #include "parts.cuh"
@@ -454,7 +455,8 @@ moe_route_kernel(const Params p) {
   float* logits = reinterpret_cast<float*>(smem);          // [T][E] of this CTA's columns
   float* full = logits + p.T * p.E;
   float* part = full + p.T * p.E;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_start();
+  wait_for_previous();
   router_products(p, part, rank * kWarps + warp, kRouteCluster * kWarps);
   __syncthreads();
   add_logits(p, part, logits);
@@ -491,7 +493,7 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   __shared__ uint64_t bars[kWarps][kUpStages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int routes = p.T * p.K;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_start();
   Ring ring;
   ring.stages = kUpStages;
   ring.base = smem + warp * kUpStages * kTile;
@@ -500,8 +502,8 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   ring.lane = lane;
   ring.init();
   if (threadIdx.x == 0) tma_prefetch_desc(&weights);
+  wait_for_previous();
   if constexpr (ROUTED) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     read_routing<true>(p, r);
   } else {
     __shared__ int counts[kChunks][kExperts];
@@ -648,7 +650,8 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   ring.status = p.status;
   ring.lane = lane;
   ring.init();
-  asm volatile("griddepcontrol.wait;" ::: "memory");       // what follows reads what the first kernel wrote
+  let_next_start();
+  wait_for_previous();
   read_routing<false>(p, r);
   const int live = r.entries;
 
@@ -934,38 +937,18 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
       !encode_weights(&down, a.down, a.I, a.H, a.E, kDownCols, kDownRows, 1))
     return cudaErrorInvalidValue;
 
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = a.stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 0;
   const bool routed = (long long)a.E * a.H * (a.router_bf16 ? 2 : 4) + (long long)a.T * a.H * 2 > kRouteInPlace;
   if (routed) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kRouteCluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(kRouteCluster);
-    cfg.dynamicSmemBytes = route_shared(a.T, a.E);
     ++g_launch_count;
-    if ((err = cudaLaunchKernelEx(&cfg, moe_route_kernel, p)) != cudaSuccess) return err;
-    attr[0] = cudaLaunchAttribute{};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    err = launch_chained(moe_route_kernel, dim3(kRouteCluster), kThreads, route_shared(a.T, a.E), kRouteCluster, a.stream, p);
+    if (err != cudaSuccess) return err;
   }
-  cfg.gridDim = dim3(unsigned(sms));
-  cfg.dynamicSmemBytes = up_shared(a.T, a.E, p.up_warps, routed);
   ++g_launch_count;
-  err = routed ? cudaLaunchKernelEx(&cfg, moe_up_kernel<true>, up, p) : cudaLaunchKernelEx(&cfg, moe_up_kernel<false>, up, p);
+  err = launch_chained(routed ? moe_up_kernel<true> : moe_up_kernel<false>, dim3(unsigned(sms)), kThreads, up_shared(a.T, a.E, p.up_warps, routed), 0,
+                       a.stream, up, p);
   if (err != cudaSuccess) return err;
-  attr[0] = cudaLaunchAttribute{};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 1;
-  cfg.dynamicSmemBytes = down_shared(a.T, p.down_warps);
   ++g_launch_count;
-  return cudaLaunchKernelEx(&cfg, moe_down_kernel, down, p);
+  return launch_chained(moe_down_kernel, dim3(unsigned(sms)), kThreads, down_shared(a.T, p.down_warps), 0, a.stream, down, p);
 }
 
 }  // namespace mts
