@@ -45,23 +45,46 @@ __device__ __forceinline__ void rotate8(Vec8T<T>& lo, Vec8T<T>& hi, const T* c, 
   }
 }
 
-// 127 x / a to the nearest integer: the product with 127 / a decides except within 0.001 of a half, where the quotient does.
-__device__ __forceinline__ uint32_t code_of(float x, float amax, float inv) {
-  const float y = x * inv;
-  float r = rintf(y);
-  if (!(fabsf(y - r) < 0.499f) || amax < 1e-30f) {
-    const float down = amax > 1e30f ? 0x1p-10f : 1.f;      // 127 x must not overflow; scaling by a power of two is exact
-    r = rintf(__fdiv_rn(x * down * 127.f, amax * down));
+// Codes of eight values of a block whose largest magnitude is amax, inv = 127 / amax.  Adding 1.5 * 2^23 to the product leaves the nearest
+// integer in the low bits of the sum (half to even); where the product is within 0.001 of a half, the correctly rounded
+// quotient 127 x / amax decides.  `x * down` keeps 127 x from overflowing (a power of two: exact).
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const Vec8T<T>& x, float amax, float inv) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t bits[8];
+  float off = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float v = to_f(x.v[j]), t = fmaf(v, inv, kMagic);
+    bits[j] = __float_as_uint(t);
+    off = fmaxf(off, fabsf(fmaf(v, inv, -__fsub_rn(t, kMagic))));
   }
-  return uint32_t(int(r) + 128) & 0xFFu;
+  if (off > 0.499f || amax < 1e-30f) {                     // 127 / amax may not be finite for such amax
+    const float down = amax > 1e30f ? 0x1p-10f : 1.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits[j] = uint32_t(int(rintf(__fdiv_rn(to_f(x.v[j]) * down * 127.f, amax * down))));
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __byte_perm(__byte_perm(bits[4 * i], bits[4 * i + 1], 0x0040), __byte_perm(bits[4 * i + 2], bits[4 * i + 3], 0x0040), 0x5410) ^ 0x80808080u;
+  return make_uint2(w[0], w[1]);
 }
+
+// Largest magnitude of pairs of 16-bit values, as their bits: the order of the bits is the order of the values, and a NaN is above
+// infinity.
+__device__ __forceinline__ uint32_t larger(uint32_t most, uint32_t pair) { return __vmaxu2(most, pair & 0x7FFF7FFFu); }
+__device__ __forceinline__ uint32_t larger(uint32_t most, const uint4& q) { return larger(larger(larger(larger(most, q.x), q.y), q.z), q.w); }
+template <typename T> __device__ __forceinline__ float value_of(uint32_t bits);
+template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+template <> __device__ __forceinline__ float value_of<__half>(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
 
 constexpr int kAppendThreads = 256;
 
 // One CTA per (block that the step touches, K/V head, sequence); the CTAs behind those rotate q.
 // A thread owns eight dims of the lower half of a head and their partners in the upper half, for one token.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads)
+__global__ void __launch_bounds__(kAppendThreads, D == 128 ? 2 : 4)
 kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __restrict__ q_out, const T* __restrict__ cosv,
                  const T* __restrict__ sinv, int table_rows, int Tn, int kv_ctas, int q_ctas, int blocks_per_head) {
   constexpr int VEC = D / 16;                              // threads per token
@@ -91,7 +114,8 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
   }
 
   __shared__ unsigned amax_sm[2][kAppendThreads / 32];
-  __shared__ __align__(16) uint8_t v_sm[D * BLK];
+  constexpr int V_PITCH = BLK + 4;
+  __shared__ __align__(16) uint8_t v_sm[D * V_PITCH];
   const int item = int(blockIdx.x) % blocks_per_head;
   const int bh = int(blockIdx.x) / blocks_per_head;
   const int h = bh % c.Hkv, b = bh / c.Hkv;
@@ -162,23 +186,20 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
       }
       continue;
     }
-    // largest magnitude as an integer: the order of the bits is the order of the values, and a NaN is above infinity
-    unsigned ka = 0, va = 0;
+    uint32_t ka = 0, va = 0;
 #pragma unroll
-    for (int it = 0; it < ITER; ++it)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ka = max(ka, max(__float_as_uint(fabsf(to_f(klo[it].v[j]))), __float_as_uint(fabsf(to_f(khi[it].v[j])))));
-        va = max(va, max(__float_as_uint(fabsf(to_f(vlo[it].v[j]))), __float_as_uint(fabsf(to_f(vhi[it].v[j])))));
-      }
-    ka = __reduce_max_sync(0xffffffffu, ka);
-    va = __reduce_max_sync(0xffffffffu, va);
+    for (int it = 0; it < ITER; ++it) {
+      ka = larger(larger(ka, klo[it].q), khi[it].q);
+      va = larger(larger(va, vlo[it].q), vhi[it].q);
+    }
+    ka = __reduce_max_sync(0xffffffffu, max(ka & 0xFFFFu, ka >> 16));
+    va = __reduce_max_sync(0xffffffffu, max(va & 0xFFFFu, va >> 16));
     if ((tid & 31) == 0) { amax_sm[0][tid >> 5] = ka; amax_sm[1][tid >> 5] = va; }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) { ka = max(ka, amax_sm[0][w]); va = max(va, amax_sm[1][w]); }
-    const bool k_ok = ka < 0x7f800000u, v_ok = va < 0x7f800000u;
-    const float kamax = __uint_as_float(ka), vamax = __uint_as_float(va);
+    const float kamax = value_of<T>(ka), vamax = value_of<T>(va);
+    const bool k_ok = kamax < CUDART_INF_F, v_ok = vamax < CUDART_INF_F;                  // false for a NaN
     const float kinv = k_ok && ka != 0 ? __fdiv_rn(127.f, kamax) : 0.f, vinv = v_ok && va != 0 ? __fdiv_rn(127.f, vamax) : 0.f;
     uint8_t* record = c.records + ((long long)bh * c.blocks + blk) * record_bytes(D);
     uint8_t* kc = record + kCacheHead;
@@ -193,31 +214,32 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
       const int idx = it * kAppendThreads + tid;
       const int tok = idx / VEC, vec = idx % VEC;
       if (tok >= BLK) continue;
-      uint32_t w[4] = {0, 0, 0, 0};
+      const uint2 none = make_uint2(0x80808080u, 0x80808080u);
+      *reinterpret_cast<uint2*>(kc + tok * D + vec * 8) = kinv > 0.f ? codes_of(klo[it], kamax, kinv) : none;
+      *reinterpret_cast<uint2*>(kc + tok * D + D / 2 + vec * 8) = kinv > 0.f ? codes_of(khi[it], kamax, kinv) : none;
+      // Values are stored by dim, where the tokens of a pair are neighbours: each of the two threads takes four dims of both.
+      const int slot = cache_slot(tok & ~1), odd = tok & 1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t a = kinv > 0.f ? code_of(to_f(klo[it].v[j]), kamax, kinv) : 128u;
-        const uint32_t d = kinv > 0.f ? code_of(to_f(khi[it].v[j]), kamax, kinv) : 128u;
-        w[j >> 2] |= a << (8 * (j & 3));
-        w[2 + (j >> 2)] |= d << (8 * (j & 3));
-      }
-      *reinterpret_cast<uint2*>(kc + tok * D + vec * 8) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(kc + tok * D + D / 2 + vec * 8) = make_uint2(w[2], w[3]);
-      const int slot = cache_slot(tok);
+      for (int half = 0; half < 2; ++half) {
+        const uint2 w = vinv > 0.f ? codes_of(half ? vhi[it] : vlo[it], vamax, vinv) : none;
+        const uint32_t theirs = __shfl_xor_sync(0xffffffffu, odd ? w.x : w.y, VEC);
+        const uint32_t even_token = odd ? theirs : w.x, odd_token = odd ? w.y : theirs;
+        uint8_t* dst = v_sm + (half * (D / 2) + vec * 8 + odd * 4) * V_PITCH + slot;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v_sm[(vec * 8 + j) * BLK + slot] = uint8_t(vinv > 0.f ? code_of(to_f(vlo[it].v[j]), vamax, vinv) : 128u);
-        v_sm[(D / 2 + vec * 8 + j) * BLK + slot] = uint8_t(vinv > 0.f ? code_of(to_f(vhi[it].v[j]), vamax, vinv) : 128u);
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint16_t*>(dst + j * V_PITCH) = uint16_t(((even_token >> (8 * j)) & 0xFFu) | (((odd_token >> (8 * j)) & 0xFFu) << 8));
       }
     }
     __syncthreads();
-    for (int i = tid; i < D * BLK / 16; i += kAppendThreads)
-      reinterpret_cast<uint4*>(vc)[i] = reinterpret_cast<const uint4*>(v_sm)[i];
+    for (int i = tid; i < D * BLK / 16; i += kAppendThreads) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(v_sm + i / 4 * V_PITCH + i % 4 * 16);
+      reinterpret_cast<uint4*>(vc)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
 // One CTA per 64 positions of a (sequence, K/V head), which lie in two blocks at most.  The values of a block are stored by dim, so
-// they pass through shared memory; then D / 8 consecutive threads write the dims of one token.
+// they pass through shared memory; then D / 4 consecutive threads write the dims of one token.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restrict__ ko, float* __restrict__ vo, int chunks) {
@@ -256,41 +278,38 @@ kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restr
     }
   }
   __syncthreads();
-  constexpr int VEC = D / 8;
+  constexpr int VEC = D / 4;
 #pragma unroll 2
   for (int i = threadIdx.x; i < 64 * VEC; i += 256) {
-    const int tok = i / VEC, d = i % VEC * 8, at_out = chunk * 64 + tok;
+    const int tok = i / VEC, d = i % VEC * 4, at_out = chunk * 64 + tok;
     if (at_out >= n) break;
     const long long p = p0 + tok;
-    float kf[8], vf[8];
+    float kf[4], vf[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) kf[j] = vf[j] = 0.f;
+    for (int j = 0; j < 4; ++j) kf[j] = vf[j] = 0.f;
     if (p >= 0 && p < total) {
       const int blk = int(p / BLK), at = int(p % BLK);
       if (blk < closed) {
         const uint8_t* record = record0 + (blk - lo) * record_bytes(D);
         const float2 sc = *reinterpret_cast<const float2*>(record);
-        const uint2 w = *reinterpret_cast<const uint2*>(record + kCacheHead + at * D + d);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(record + kCacheHead + at * D + d);
         const uint8_t* vs = &codes_sm[blk - lo][d * PITCH + cache_slot(at)];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          kf[j] = float(int(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xFFu) - 128) * sc.x;
+        for (int j = 0; j < 4; ++j) {
+          kf[j] = float(int((w >> (8 * j)) & 0xFFu) - 128) * sc.x;
           vf[j] = float(int(vs[j * PITCH]) - 128) * sc.y;
         }
       } else {
-        Vec8T<T> x;
-        x.q = *reinterpret_cast<const uint4*>(tail + at * D + d);
+        const uint2 w = *reinterpret_cast<const uint2*>(tail + at * D + d);
+        const T* ks = reinterpret_cast<const T*>(&w);
         const T* vs = tail_sm + ((at >> 5) * D + d) * HALF_PITCH + tail_slot(0, 0, at & 31);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { kf[j] = to_f(x.v[j]); vf[j] = to_f(vs[j * HALF_PITCH]); }
+        for (int j = 0; j < 4; ++j) { kf[j] = to_f(ks[j]); vf[j] = to_f(vs[j * HALF_PITCH]); }
       }
     }
-    float* kd = ko + ((long long)bh * n + at_out) * D + d;
-    float* vd = vo + ((long long)bh * n + at_out) * D + d;
-    *reinterpret_cast<float4*>(kd) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-    *reinterpret_cast<float4*>(kd + 4) = make_float4(kf[4], kf[5], kf[6], kf[7]);
-    *reinterpret_cast<float4*>(vd) = make_float4(vf[0], vf[1], vf[2], vf[3]);
-    *reinterpret_cast<float4*>(vd + 4) = make_float4(vf[4], vf[5], vf[6], vf[7]);
+    const long long at_d = ((long long)bh * n + at_out) * D + d;
+    *reinterpret_cast<float4*>(ko + at_d) = make_float4(kf[0], kf[1], kf[2], kf[3]);
+    *reinterpret_cast<float4*>(vo + at_d) = make_float4(vf[0], vf[1], vf[2], vf[3]);
   }
 }
 
