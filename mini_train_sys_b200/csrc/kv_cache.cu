@@ -2,8 +2,7 @@
 //
 //   a = max |x| over the 64 x D values of a finished block,  scale = a / 127,  code = rint(127 x / a)  (half to even)
 //
-// For 16-bit x the product 127 x is exact in fp32 and 127 x / a is either a half exactly or at least 2^-12 away from one, so
-// a correctly rounded quotient gives the code that exact arithmetic gives.
+// What bounds it: reading the new tokens and writing their codes, 3 bytes a value.
 #include "decode.cuh"
 #include "launch.cuh"
 #include "ops.cuh"
@@ -18,51 +17,64 @@ namespace {
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <typename T> union Vec8T { uint4 q; uint32_t w[4]; T v[8]; };
 
-template <typename T> union Vec8T { uint4 q; T v[8]; };
-
-// x c -+ y s as the rotary kernel computes it: the products of 16-bit factors are exact in fp32, their sum is rounded there and
-// then to T.
-template <typename T>
-__device__ __forceinline__ T rotate_one(T x, T c, T y, T s, bool minus) {
-  const float p = __fmul_rn(to_f(x), to_f(c)), q = __fmul_rn(to_f(y), to_f(s));
-  return from_f<T>(minus ? __fsub_rn(p, q) : __fadd_rn(p, q));
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf162(a, b); }
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_half2(a, b); }
 
+// Half-split rotation as the rotary kernel computes it: the products of 16-bit factors are exact in fp32, their sum is rounded there
+// and then to T.
 template <typename T>
 __device__ __forceinline__ void rotate8(Vec8T<T>& lo, Vec8T<T>& hi, const T* c, const T* s) {
   Vec8T<T> cv, sv;
   cv.q = *reinterpret_cast<const uint4*>(c);
   sv.q = *reinterpret_cast<const uint4*>(s);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const T a = lo.v[j], b = hi.v[j];
-    lo.v[j] = rotate_one(a, cv.v[j], b, sv.v[j], true);
-    hi.v[j] = rotate_one(b, cv.v[j], a, sv.v[j], false);
+  for (int j = 0; j < 4; ++j) {
+    const float2 a = unpack2<T>(lo.w[j]), b = unpack2<T>(hi.w[j]), cc = unpack2<T>(cv.w[j]), ss = unpack2<T>(sv.w[j]);
+    lo.w[j] = pack2<T>(fmaf(a.x, cc.x, -__fmul_rn(b.x, ss.x)), fmaf(a.y, cc.y, -__fmul_rn(b.y, ss.y)));
+    hi.w[j] = pack2<T>(fmaf(b.x, cc.x, __fmul_rn(a.x, ss.x)), fmaf(b.y, cc.y, __fmul_rn(a.y, ss.y)));
   }
 }
 
-// Codes of eight values of a block whose largest magnitude is amax, inv = 127 / amax.  Adding 1.5 * 2^23 to the product leaves the nearest
-// integer in the low bits of the sum (half to even); where the product is within 0.001 of a half, the correctly rounded
-// quotient 127 x / amax decides.  `x * down` keeps 127 x from overflowing (a power of two: exact).
+// Codes of eight values of a block whose largest magnitude is amax: 127 x / amax to the nearest integer, a half to the even one.
+// With whole mantissas, x = X 2^i and amax = A 2^j, a half is 254 X 2^(i-j) = A (2n + 1).  127 is prime, so it divides 2n + 1 (then n
+// is 63: x is half of amax, not a rare value) or A.  Where it does not divide A, everything else is at least 1 / (2 A) >= 2^-12 from a
+// half, and a product with 127 / amax, made two units in the last place too large, is right: it is off by 4e-5 at most, and takes
+// half of amax to just above 63.5, hence to 64, the even one.  Adding 1.5 * 2^23 leaves the integer in the low bits of the sum.
+// Blocks with other A (and with a subnormal or huge amax) take correctly rounded quotients, scaled by a power of two.
+struct Quantizer {
+  float amax, inv;
+  bool quick;
+};
+template <typename T> __device__ __forceinline__ bool mantissa_is_plain(uint32_t bits);
+template <> __device__ __forceinline__ bool mantissa_is_plain<__nv_bfloat16>(uint32_t bits) { return (bits & 0x7Fu) != 0x7Eu; }   // 254 = 2 * 127
+template <> __device__ __forceinline__ bool mantissa_is_plain<__half>(uint32_t bits) { return bits >= 0x400u && ((bits & 0x3FFu) | 0x400u) % 127u != 0u; }
+
 template <typename T>
-__device__ __forceinline__ uint2 codes_of(const Vec8T<T>& x, float amax, float inv) {
+__device__ __forceinline__ uint2 codes_of(const Vec8T<T>& x, const Quantizer& q) {
   constexpr float kMagic = 12582912.f;
   uint32_t bits[8];
-  float off = 0.f;
+  if (q.quick) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float v = to_f(x.v[j]), t = fmaf(v, inv, kMagic);
-    bits[j] = __float_as_uint(t);
-    off = fmaxf(off, fabsf(fmaf(v, inv, -__fsub_rn(t, kMagic))));
-  }
-  if (off > 0.499f || amax < 1e-30f) {                     // 127 / amax may not be finite for such amax
-    const float down = amax > 1e30f ? 0x1p-10f : 1.f;
+    for (int j = 0; j < 4; ++j) {
+      const float2 v = unpack2<T>(x.w[j]);
+      bits[2 * j] = __float_as_uint(fmaf(v.x, q.inv, kMagic));
+      bits[2 * j + 1] = __float_as_uint(fmaf(v.y, q.inv, kMagic));
+    }
+  } else {
+    const float scale = q.amax > 1.f ? 0x1p-60f : 0x1p60f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) bits[j] = uint32_t(int(rintf(__fdiv_rn(to_f(x.v[j]) * down * 127.f, amax * down))));
+    for (int j = 0; j < 8; ++j) {
+      const float2 v = unpack2<T>(x.w[j >> 1]);
+      bits[j] = q.amax > 0.f ? uint32_t(int(rintf(__fdiv_rn(((j & 1) ? v.y : v.x) * scale * 127.f, q.amax * scale)))) : 0u;
+    }
   }
   uint32_t w[2];
 #pragma unroll
@@ -80,6 +92,7 @@ template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(uint32_t bi
 template <> __device__ __forceinline__ float value_of<__half>(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
 
 constexpr int kAppendThreads = 256;
+constexpr int kQPieces = 4;              // of 32 bytes of q, a thread
 
 // One CTA per (block that the step touches, K/V head, sequence); the CTAs behind those rotate q.
 // A thread owns eight dims of the lower half of a head and their partners in the upper half, for one token.
@@ -95,21 +108,33 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
   wait_for_previous();
   if (int(blockIdx.x) >= kv_ctas) {                        // ---- q: a CTA takes consecutive pieces of one sequence ----
     const unsigned per_token = unsigned(Hq) * VEC, pieces = unsigned(Tn) * per_token;    // at most 2^31, checked by the launcher
-    const unsigned at = unsigned(blockIdx.x) - unsigned(kv_ctas), b = at / unsigned(q_ctas), piece = at % unsigned(q_ctas) * kAppendThreads + tid;
-    if (piece >= pieces) return;
-    const unsigned t = piece / per_token, rest = piece % per_token, h = rest / VEC, vec = rest % VEC;
-    T* dst = q_out + (((long long)b * Tn + t) * Hq + h) * D + vec * 8;
-    Vec8T<T> lo, hi;
-    lo.q = hi.q = make_uint4(0, 0, 0, 0);
-    const int p = c.start[b] + int(t);
-    if (int(t) < c.count[b] && p >= 0 && p < c.blocks * BLK) {
-      const T* src = static_cast<const T*>(q.p) + b * q.sb + h * q.sh + t * q.st + vec * 8;
-      lo.q = *reinterpret_cast<const uint4*>(src);
-      hi.q = *reinterpret_cast<const uint4*>(src + D / 2);
-      if (cosv != nullptr && p < table_rows) rotate8(lo, hi, cosv + (long long)p * D + vec * 8, sinv + (long long)p * D + vec * 8);
+    const unsigned at = unsigned(blockIdx.x) - unsigned(kv_ctas), b = at / unsigned(q_ctas), base = at % unsigned(q_ctas) * (kQPieces * kAppendThreads) + tid;
+    const int start = c.start[b], count = c.count[b];
+    Vec8T<T> lo[kQPieces], hi[kQPieces];
+    unsigned t[kQPieces], rest[kQPieces];
+#pragma unroll
+    for (int i = 0; i < kQPieces; ++i) {                   // all loads before the first store
+      const unsigned piece = base + i * kAppendThreads;
+      t[i] = piece / per_token;
+      rest[i] = piece % per_token;
+      lo[i].q = hi[i].q = make_uint4(0, 0, 0, 0);
+      const int p = start + int(t[i]);
+      if (piece < pieces && int(t[i]) < count && p >= 0 && p < c.blocks * BLK) {
+        const T* src = static_cast<const T*>(q.p) + b * q.sb + rest[i] / VEC * q.sh + t[i] * q.st + rest[i] % VEC * 8;
+        lo[i].q = *reinterpret_cast<const uint4*>(src);
+        hi[i].q = *reinterpret_cast<const uint4*>(src + D / 2);
+      }
     }
-    *reinterpret_cast<uint4*>(dst) = lo.q;
-    *reinterpret_cast<uint4*>(dst + D / 2) = hi.q;
+#pragma unroll
+    for (int i = 0; i < kQPieces; ++i) {
+      const int p = start + int(t[i]);
+      if (base + i * kAppendThreads >= pieces) break;
+      if (cosv != nullptr && int(t[i]) < count && p >= 0 && p < table_rows && p < c.blocks * BLK)
+        rotate8(lo[i], hi[i], cosv + (long long)p * D + rest[i] % VEC * 8, sinv + (long long)p * D + rest[i] % VEC * 8);
+      T* dst = q_out + (((long long)b * Tn + t[i]) * Hq + rest[i] / VEC) * D + rest[i] % VEC * 8;
+      *reinterpret_cast<uint4*>(dst) = lo[i].q;
+      *reinterpret_cast<uint4*>(dst + D / 2) = hi[i].q;
+    }
     return;
   }
 
@@ -198,30 +223,35 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) { ka = max(ka, amax_sm[0][w]); va = max(va, amax_sm[1][w]); }
-    const float kamax = value_of<T>(ka), vamax = value_of<T>(va);
-    const bool k_ok = kamax < CUDART_INF_F, v_ok = vamax < CUDART_INF_F;                  // false for a NaN
-    const float kinv = k_ok && ka != 0 ? __fdiv_rn(127.f, kamax) : 0.f, vinv = v_ok && va != 0 ? __fdiv_rn(127.f, vamax) : 0.f;
+    auto quantizer = [](uint32_t bits) {
+      Quantizer q;
+      q.amax = value_of<T>(bits);
+      q.quick = mantissa_is_plain<T>(bits) && q.amax > 1e-30f && q.amax < 1e30f;
+      q.inv = __uint_as_float(__float_as_uint(__fdiv_rn(127.f, q.amax)) + 2u);
+      if (!(q.amax < CUDART_INF_F)) q.amax = CUDART_NAN_F;                               // the whole block reads NaN
+      return q;
+    };
+    const Quantizer kq = quantizer(ka), vq = quantizer(va);
     uint8_t* record = c.records + ((long long)bh * c.blocks + blk) * record_bytes(D);
     uint8_t* kc = record + kCacheHead;
     uint8_t* vc = kc + BLK * D;
     if (tid == 0) {
       float* sc = reinterpret_cast<float*>(record);
-      sc[0] = k_ok ? __fdiv_rn(kamax, 127.f) : CUDART_NAN_F;     // a block that holds a NaN or an infinity reads NaN
-      sc[1] = v_ok ? __fdiv_rn(vamax, 127.f) : CUDART_NAN_F;
+      sc[0] = __fdiv_rn(kq.amax, 127.f);
+      sc[1] = __fdiv_rn(vq.amax, 127.f);
     }
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       const int idx = it * kAppendThreads + tid;
       const int tok = idx / VEC, vec = idx % VEC;
       if (tok >= BLK) continue;
-      const uint2 none = make_uint2(0x80808080u, 0x80808080u);
-      *reinterpret_cast<uint2*>(kc + tok * D + vec * 8) = kinv > 0.f ? codes_of(klo[it], kamax, kinv) : none;
-      *reinterpret_cast<uint2*>(kc + tok * D + D / 2 + vec * 8) = kinv > 0.f ? codes_of(khi[it], kamax, kinv) : none;
+      *reinterpret_cast<uint2*>(kc + tok * D + vec * 8) = codes_of(klo[it], kq);
+      *reinterpret_cast<uint2*>(kc + tok * D + D / 2 + vec * 8) = codes_of(khi[it], kq);
       // Values are stored by dim, where the tokens of a pair are neighbours: each of the two threads takes four dims of both.
       const int slot = cache_slot(tok & ~1), odd = tok & 1;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint2 w = vinv > 0.f ? codes_of(half ? vhi[it] : vlo[it], vamax, vinv) : none;
+        const uint2 w = codes_of(half ? vhi[it] : vlo[it], vq);
         const uint32_t theirs = __shfl_xor_sync(0xffffffffu, odd ? w.x : w.y, VEC);
         const uint32_t even_token = odd ? theirs : w.x, odd_token = odd ? w.y : theirs;
         uint8_t* dst = v_sm + (half * (D / 2) + vec * 8 + odd * 4) * V_PITCH + slot;
@@ -319,7 +349,7 @@ cudaError_t append_typed(const CacheView& c, const Strided& q, int Hq, const Str
   const int per_head = (Tn + kCacheBlock - 2) / kCacheBlock + 1;       // blocks that T tokens can touch
   const long long kv_ctas = (long long)c.B * c.Hkv * per_head;
   const long long pieces = q.p == nullptr ? 0 : (long long)Hq * Tn * (D / 16);
-  const long long q_ctas = (pieces + kAppendThreads - 1) / kAppendThreads;               // of a sequence
+  const long long q_ctas = (pieces + kQPieces * kAppendThreads - 1) / (kQPieces * kAppendThreads);      // of a sequence
   if (kv_ctas + q_ctas * c.B > 0x7fffffffll || pieces > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   ++g_launch_count;
   return launch_chained(kv_append_kernel<T, D>, dim3(unsigned(kv_ctas + q_ctas * c.B)), kAppendThreads, 0, 0, stream, c, q, Hq, k, v, static_cast<T*>(q_out),
