@@ -6,16 +6,16 @@
 // share a K/V head, times the new tokens of the step).  Every warp has a ring of blocks of its own in shared memory, which bulk
 // copies fill (one for the keys of a block with its scales, one for its values), so the warps run without barriers and each
 // keeps 8 to 16 KB of the cache in flight.  A lane's 16 adjacent bytes are its K or V fragment of several steps (the V rows are
-// stored in that order); 4 bytes become two fp16 pairs, 1152 too large, in two instructions, and the sums start from what that adds
-// (-1152 times the sum of the query, or of the probabilities, which a product with ones gives); both products run on m16n8k16 with the tokens (K) or
+// stored in that order); 4 bytes become two fp16 pairs in two instructions, 1152 too large, or in four.  Keys stay too large, and a
+// score starts from what that adds (-1152 times the sum of the query: 1e-5 in a logit, the same for every key); values do not,
+// because their sums cancel over a long context (8e-4 of an output over 131k tokens; exact values: 2e-4, the rounding to fp16).  Both products run on m16n8k16 with the tokens (K) or
 // the head's dims (V) as rows and eight query rows as columns.  The (sequence, head, row tile, block) units of
 // the whole batch are one list, cut into equal parts for the warps that fit on the machine: sequences of unlike lengths, and a
 // single long one, keep every SM busy, and a warp streams across the ends of sequences.  A second kernel joins the parts of
 // the (sequence, head, row tile) items that were cut.
 // What bounds it: reading the codes, 2 D bytes per token and K/V head.
 //
-// Rounding: codes are exact in fp16 (and 1152 more than they are still exact; in fp32 sums it costs 2^-24 of 1152 sum p, for values of
-// about 40).  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
+// Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
 // queries keep their eight bits in fp16.  Probabilities are rounded to fp16 (2^-11 of each, at a scale of 2^14 so that the
 // smallest kept one is 2^-38 of the largest); the sum of probabilities, the maximum and the output accumulators are fp32.  In
 // the unfinished block, whose values are bf16, a probability is the sum of two bf16 values.
@@ -442,8 +442,8 @@ cached_attention_kernel(const Params p) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               uint32_t a0, a1, a2, a3;
-              codes_to_half(kr[m][0][i], a0, a2);
-              codes_to_half(kr[m][1][i], a1, a3);
+              codes_to_biased(kr[m][0][i], a0, a2);
+              codes_to_biased(kr[m][1][i], a1, a3);
 #pragma unroll
               for (int n = 0; n < NQ; ++n) {
                 const float from[4] = {qbias[n][0], qbias[n][1], qbias[n][0], qbias[n][1]};
@@ -481,14 +481,11 @@ cached_attention_kernel(const Params p) {
             pf[m][n][0] = transpose8x8(pack_half2(s[m][n][0], s[m][n][1]));
             pf[m][n][1] = transpose8x8(pack_half2(s[m][n][2], s[m][n][3]));
           }
-        float vbias[NQ][4];                                  // -1152 times the sum of the rounded probabilities
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
+        for (int n = 0; n < NQ; ++n) {                       // the sum of the rounded probabilities
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int m = 0; m < 4; ++m) mma_f16(sum, kOnes, kOnes, kOnes, kOnes, pf[m][n][0], pf[m][n][1]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vbias[n][i] = -kCodeBias * sum[i & 1];
           st.l[n][0] += sum[0];
           st.l[n][1] += sum[1];
         }
@@ -500,6 +497,7 @@ cached_attention_kernel(const Params p) {
           for (int d = 0; d < 2; ++d)
 #pragma unroll
             for (int v = 0; v < 2; ++v) read_words<4>(vst + (16 * (d0 + d) + 8 * v) * BLK, vr[d][v]);
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
           float acc[2][NQ][4];
 #pragma unroll
           for (int m = 0; m < 4; ++m)
@@ -510,7 +508,7 @@ cached_attention_kernel(const Params p) {
               codes_to_half(vr[d][1][m], a1, a3);
 #pragma unroll
               for (int n = 0; n < NQ; ++n) {
-                if (m == 0) mma_f16_from(acc[d][n], vbias[n], a0, a1, a2, a3, pf[0][n][0], pf[0][n][1]);
+                if (m == 0) mma_f16_from(acc[d][n], zero, a0, a1, a2, a3, pf[0][n][0], pf[0][n][1]);
                 else mma_f16(acc[d][n], a0, a1, a2, a3, pf[m][n][0], pf[m][n][1]);
               }
             }

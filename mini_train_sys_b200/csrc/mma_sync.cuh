@@ -41,12 +41,20 @@ __device__ __forceinline__ uint32_t pack_bf162(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Four excess-128 codes to two pairs of fp16 numbers: a byte below the byte 0x64 is 1024 + the byte, so the pairs hold value + 1152.
-// The products start from -1152 times the sum of the other factor, which takes it out again.
+// Four excess-128 codes to two pairs of fp16 numbers.  A byte below the byte 0x64 is 1024 + the byte, so the pairs hold value + 1152:
+// a product of them may start from -1152 times the sum of the other factor, which takes it out again.
 constexpr float kCodeBias = 1152.f;
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ void codes_to_biased(uint32_t w, uint32_t& lo, uint32_t& hi) {
   lo = __byte_perm(w, 0x64646464u, 0x4140);
   hi = __byte_perm(w, 0x64646464u, 0x4342);
+}
+// The values themselves: the subtraction is exact.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  codes_to_biased(w, lo, hi);
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), bias), b = __hsub2(*reinterpret_cast<const __half2*>(&hi), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
 }
 
 }  // namespace mts

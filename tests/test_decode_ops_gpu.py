@@ -100,6 +100,29 @@ def test_codes_of_halves_extremes_and_non_finite_blocks(ops):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_codes_for_every_mantissa_of_the_largest_value(ops, dtype):
+    """Blocks whose largest value runs through the mantissas of the type, with every odd multiple of 1 / 254 of it that the type can
+    express (exact halves) and random values."""
+
+    mantissas = torch.arange(128, 256) if dtype == torch.bfloat16 else torch.arange(1024, 2048)
+    heads = mantissas.numel()
+    amax = (mantissas.double() / mantissas[0]).to(DEV)
+    halves = (torch.arange(127, device=DEV) * 2 + 1).double()[None] * amax[:, None] / 254
+    halves = torch.where(halves.to(dtype).double() == halves, halves, torch.zeros_like(halves))
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    k = (torch.rand(heads, 64 * 32, generator=gen, device=DEV, dtype=torch.float64) * 2 - 1) * amax[:, None]
+    k[:, 0], k[:, 1:128], k[:, 128:255] = amax, halves, -halves
+    k = k.to(dtype).view(1, heads, 64, 32)
+    cache = QuantizedKVCache(layers=1, batch=1, kv_heads=heads, head_dim=32, capacity=64, dtype=dtype, device=DEV)
+    cache.begin(padded=64)
+    ops.kv_append(cache, 0, k, k)
+    want = torch.round(k[0].double() * 127 / k[0].double().abs().amax((1, 2), keepdim=True)).int()
+    assert torch.equal(cache.codes[0, 0, :, 0, 0].reshape(heads, 64, 32).int() - 128, want)
+    vr = ops.kv_read(cache, 0, torch.zeros(1, dtype=torch.int32, device=DEV), 64)[1][0]
+    assert ((vr.double() - want * (amax / 127)[:, None, None]).abs() <= 2 ** -22 * want.abs() * amax[:, None, None]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim,hkv,group", [(32, 3, 1), (64, 2, 1), (64, 1, 12), (128, 2, 4), (64, 2, 40)])
 @pytest.mark.parametrize("new", [1, 2, 17, 65])
 def test_cached_attention(ops, dtype, dim, hkv, group, new):
