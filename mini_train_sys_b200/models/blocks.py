@@ -100,6 +100,25 @@ class CausalSelfAttention(nn.Module):
         ctx = ctx.transpose(1, 2).contiguous().view(b, s, h)
         return add_dropped(ops, self.resid_dropout, project(ops, self.out, ctx), residual)
 
+    def forward_cached(self, x: torch.Tensor, ops: OpsBackend, rope_cos: torch.Tensor, rope_sin: torch.Tensor, cache, layer: int,
+                       residual: torch.Tensor) -> torch.Tensor:
+        """One step of cached decoding: ``x`` [B, T, H] are the new tokens of the open step of ``cache``.
+
+        A prompt (nothing cached yet) attends to itself with the exact keys and values and fills the cache; later steps append and
+        attend over the cache.  The tables are the full ones: positions come from the cache's lengths."""
+
+        b, s, h = x.shape
+        fused = project(ops, self.qkv, x).view(b, s, 3, self.cfg.n_heads, self.cfg.head_dim)
+        q, k, v = (fused[:, :, j].transpose(1, 2) for j in range(3))
+        if cache.held == 0:
+            q, k = ops.rope(q, k, rope_cos[:s], rope_sin[:s])
+            ops.kv_append(cache, layer, k, v)
+            ctx = ops.attention(q, k, v, is_causal=True, dropout_p=0.0)
+        else:
+            ctx = ops.cached_attention(ops.kv_append(cache, layer, k, v, q=q, cos=rope_cos, sin=rope_sin), cache, layer)
+        ctx = ctx.transpose(1, 2).contiguous().view(b, s, h)
+        return residual + project(ops, self.out, ctx)
+
 
 class DenseFeedForward(nn.Module):
     def __init__(self, cfg: ModelConfig) -> None:
@@ -116,6 +135,12 @@ class DenseFeedForward(nn.Module):
     def forward(self, x: torch.Tensor, ops: OpsBackend, residual: torch.Tensor | None = None) -> FeedForwardOutput:
         act = ops.swiglu(project(ops, self.gate, x), project(ops, self.up, x))
         return FeedForwardOutput(add_dropped(ops, self.dropout, project(ops, self.down, act), residual))
+
+    def forward_tokens(self, x: torch.Tensor, ops: OpsBackend, residual: torch.Tensor) -> torch.Tensor:
+        return self(x, ops, residual=residual).hidden_states
+
+
+FEW_TOKENS = 64     # up to which the experts' weights are streamed once for all tokens instead of sorting rows for grouped GEMMs
 
 
 class MoEFeedForward(nn.Module):
@@ -149,6 +174,16 @@ class MoEFeedForward(nn.Module):
             router_metrics=route.metrics,
         )
 
+    def forward_tokens(self, x: torch.Tensor, ops: OpsBackend, residual: torch.Tensor) -> torch.Tensor:
+        """The layer in a decoding step: a few tokens go through the backend's one-call form (no balance statistics)."""
+
+        tokens = x.reshape(-1, x.shape[-1])
+        if tokens.shape[0] > FEW_TOKENS or self.expert_dispatch is not None or not hasattr(ops, "moe_tokens"):
+            return self(x, ops, residual=residual).hidden_states
+        y = ops.moe_tokens(tokens, self.router.weight, self.gate_up_proj, self.down_proj, self.cfg.experts_per_token,
+                           normalize=self.cfg.router_normalize_topk)
+        return residual + y.view(x.shape)
+
 
 def build_feed_forward(cfg: ModelConfig) -> nn.Module:
     return MoEFeedForward(cfg) if cfg.is_moe else DenseFeedForward(cfg)
@@ -173,6 +208,10 @@ class TransformerBlock(nn.Module):
         x = self.attn(h, ops, rope_cos, rope_sin, residual=res)
         h, res = self.ffn_norm.with_residual(x, ops)
         return self.ffn(h, ops, residual=res)      # hidden_states already include the residual
+
+    def forward_cached(self, x: torch.Tensor, ops: OpsBackend, rope_cos: torch.Tensor, rope_sin: torch.Tensor, cache, layer: int) -> torch.Tensor:
+        x = self.attn.forward_cached(self.attn_norm(x, ops), ops, rope_cos, rope_sin, cache, layer, residual=x)
+        return self.ffn.forward_tokens(self.ffn_norm(x, ops), ops, residual=x)
 
 
 SwiGLUMLP = DenseFeedForward

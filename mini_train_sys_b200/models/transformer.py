@@ -117,6 +117,47 @@ class MiniTransformer(nn.Module):
         logits = project(self.ops, self.lm_head, hidden)
         return self.ops.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1)), logits
 
+    @torch.no_grad()
+    def decode(self, input_ids: torch.Tensor, cache, counts: torch.Tensor | None = None) -> torch.Tensor:
+        """One step of cached decoding: append ``input_ids`` [B, T] to ``cache`` (``QuantizedKVCache``) and return the logits [B, V]
+        behind the last new token of every sequence.
+
+        ``counts`` [B] holds the number of new tokens of each sequence where the batch is padded on the right; a sequence without
+        one gets the logits behind its padding, which mean nothing.  Positions continue from the cached lengths."""
+
+        if self.training:
+            raise RuntimeError("decode() needs eval mode")
+        if cache.layers != len(self.blocks) or cache.kv_heads != self.cfg.n_heads or cache.head_dim != self.cfg.head_dim:
+            raise ValueError("the cache was made for another model")
+        if cache.dtype != self.activation_dtype:
+            raise ValueError(f"the cache holds {cache.dtype}, the model's activations are {self.activation_dtype}")
+        if input_ids.shape[0] != cache.batch:
+            raise ValueError(f"{input_ids.shape[0]} sequences for a cache of {cache.batch}")
+        steps = input_ids.shape[1]
+        if cache.held + steps > self.rotary.max_seq_len:
+            raise ValueError(f"{cache.held} cached + {steps} new tokens exceed the model's seq_len of {self.rotary.max_seq_len}")
+        cache.begin(counts, padded=steps)
+        own_embedding = getattr(self.ops, "embedding", None)
+        h = None
+        if own_embedding is not None and self.activation_dtype == torch.bfloat16:
+            h = own_embedding(input_ids, self.embed.weight)
+        h = (self.embed(input_ids) if h is None else h).to(self.activation_dtype)
+        for layer, block in enumerate(self.blocks):
+            h = block.forward_cached(h, self.ops, self.rotary.cos, self.rotary.sin, cache, layer)
+        if steps > 1:
+            last = (cache.counts.long() - 1).clamp_min(0)
+            h = h.gather(1, last[:, None, None].expand(-1, 1, h.shape[2]))
+        cache.commit()
+        return project(self.ops, self.lm_head, self.norm(h, self.ops))[:, 0]
+
+    def new_cache(self, batch: int, capacity: int | None = None):
+        """An empty 8-bit key / value cache for ``batch`` sequences of up to ``capacity`` tokens (default: the model's seq_len)."""
+
+        from mini_train_sys_b200.ops.kv_cache import QuantizedKVCache
+
+        return QuantizedKVCache(layers=len(self.blocks), batch=batch, kv_heads=self.cfg.n_heads, head_dim=self.cfg.head_dim,
+                                capacity=capacity or self.cfg.seq_len, dtype=self.activation_dtype, device=self.embed.weight.device)
+
     def forward(self, input_ids: torch.Tensor, targets: torch.Tensor | None = None, use_fused_loss: bool = False
                 ) -> tuple[torch.Tensor | None, torch.Tensor]:
         hidden = self.hidden_states(input_ids)

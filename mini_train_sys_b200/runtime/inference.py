@@ -60,24 +60,92 @@ def evaluate_loss(model: MiniTransformer, loader, device: torch.device, *, max_b
     return {"loss": mean, "perplexity": math.exp(min(mean, 50.0)), "tokens": tokens, "batches": batches}
 
 
+KV_CACHES = ("none", "int8")
+
+
+class DecodeSession:
+    """Cached decoding of one batch: ``prompt`` once, then ``step`` by step.
+
+    On a GPU with the native operators a step is captured into a CUDA graph after the first one and replayed: a step is some
+    hundred short kernels, whose launches take longer than their work."""
+
+    def __init__(self, model: MiniTransformer, batch: int, capacity: int | None = None, *, graph: bool | None = None) -> None:
+        self.model = model
+        self.cache = model.new_cache(batch, capacity)
+        on_gpu = self.cache.device.type == "cuda" and getattr(model.ops, "name", "") == "native" and model.activation_dtype == torch.bfloat16
+        if graph and not on_gpu:
+            raise ValueError("a captured step needs a GPU, the native operators and bf16 activations")
+        self.graph_wanted = on_gpu if graph is None else bool(graph)
+        self._graph: torch.cuda.CUDAGraph | None = None
+        self._steps = 0
+
+    def prompt(self, input_ids: torch.Tensor, counts: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits [B, V] behind the prompts [B, T]; ``counts`` [B] are their lengths where they are padded on the right."""
+
+        return self.model.decode(input_ids, self.cache, counts)
+
+    def step(self, token_ids: torch.Tensor) -> torch.Tensor:
+        """Logits [B, V] behind one more token [B, 1] of every sequence.  They are overwritten by the next step."""
+
+        if token_ids.shape != (self.cache.batch, 1):
+            raise ValueError(f"a step takes one token per sequence, got {tuple(token_ids.shape)}")
+        self._steps += 1
+        if not self.graph_wanted or self._steps == 1:          # the first step lays out what the kernels keep
+            return self.model.decode(token_ids, self.cache)
+        if self.cache.held + 1 > self.model.rotary.max_seq_len:
+            raise ValueError(f"{self.cache.held} cached + 1 new tokens exceed the model's seq_len of {self.model.rotary.max_seq_len}")
+        if self._graph is None:
+            self._ids = token_ids.clone()
+            held = self.cache.held
+            torch.cuda.synchronize(self.cache.device)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.device(self.cache.device), torch.cuda.graph(graph):
+                self._logits = self.model.decode(self._ids, self.cache)
+            self.cache.held = held                             # capturing has run nothing
+            self._graph = graph
+        self.cache.replayed(1)
+        self._ids.copy_(token_ids)
+        self._graph.replay()
+        return self._logits
+
+
+def _next_token(logits: torch.Tensor, temperature: float, top_k: int | None, greedy: bool, generator) -> torch.Tensor:
+    step = logits.float()
+    if greedy or temperature <= 0:
+        return step.argmax(-1, keepdim=True)
+    step = step / temperature
+    if top_k is not None and top_k > 0:
+        kth = step.topk(min(top_k, step.shape[-1]), -1).values[:, -1:]
+        step = step.masked_fill(step < kth, float("-inf"))
+    return torch.multinomial(torch.softmax(step, -1), 1, generator=generator)
+
+
 @torch.no_grad()
 def generate(model: MiniTransformer, prompt_ids: torch.Tensor, *, max_new_tokens: int, temperature: float = 1.0,
-             top_k: int | None = None, greedy: bool = False, generator: torch.Generator | None = None) -> torch.Tensor:
-    """Autoregressive decoding without a KV cache: the prefix (cropped to ``seq_len``) is re-encoded every step."""
+             top_k: int | None = None, greedy: bool = False, generator: torch.Generator | None = None, kv_cache: str = "none") -> torch.Tensor:
+    """Autoregressive decoding.  Without a cache the prefix (cropped to ``seq_len``) is re-encoded every step; with
+    ``kv_cache="int8"`` every token is encoded once and finished blocks of 64 keys and values are held in 8 bits, and prompt and
+    new tokens together must fit in ``seq_len``."""
 
+    if kv_cache not in KV_CACHES:
+        raise ValueError(f"kv_cache must be one of {KV_CACHES}, got {kv_cache!r}")
     ids = prompt_ids.clone()
     limit = model.cfg.seq_len
-    for _ in range(max_new_tokens):
-        window = ids[:, -limit:]
-        _, logits = model(window)
-        step = logits[:, -1, :].float()
-        if greedy or temperature <= 0:
-            nxt = step.argmax(-1, keepdim=True)
-        else:
-            step = step / temperature
-            if top_k is not None and top_k > 0:
-                kth = step.topk(min(top_k, step.shape[-1]), -1).values[:, -1:]
-                step = step.masked_fill(step < kth, float("-inf"))
-            nxt = torch.multinomial(torch.softmax(step, -1), 1, generator=generator)
+    if kv_cache == "none":
+        for _ in range(max_new_tokens):
+            _, logits = model(ids[:, -limit:])
+            ids = torch.cat((ids, _next_token(logits[:, -1, :], temperature, top_k, greedy, generator)), dim=1)
+        return ids
+    if max_new_tokens <= 0:
+        return ids
+    reach = ids.shape[1] + max_new_tokens - 1                  # the last token is not fed back
+    if reach > limit:
+        raise ValueError(f"{ids.shape[1]} prompt + {max_new_tokens} new tokens exceed the model's seq_len of {limit}; cached decoding does not crop")
+    session = DecodeSession(model, ids.shape[0], reach)
+    logits = session.prompt(ids)
+    for i in range(max_new_tokens):
+        nxt = _next_token(logits, temperature, top_k, greedy, generator)
         ids = torch.cat((ids, nxt), dim=1)
+        if i + 1 < max_new_tokens:
+            logits = session.step(nxt)
     return ids

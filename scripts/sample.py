@@ -1,7 +1,8 @@
-"""Generate tokens from a consolidated checkpoint (greedy or temperature / top-k sampling, no KV cache).
+"""Generate tokens from a consolidated checkpoint (greedy or temperature / top-k sampling, with or without a key / value cache).
 
     python scripts/sample.py --checkpoint <dir> --prompt-ids 1,2,3 --max-new-tokens 32 --top-k 40
     python scripts/sample.py --checkpoint <dir> --tokenizer <tokenizer dir> --prompt "Once upon a time"
+    python scripts/sample.py --checkpoint <dir> --prompt-ids 1,2,3 --ops native --kv-cache int8
 
 (The reference ships this entry point as an unimplemented scaffold: scripts/sample.py:2-3.)
 """
@@ -21,7 +22,7 @@ import torch  # noqa: E402
 
 from mini_train_sys_b200.runtime.config import load_yaml_dict  # noqa: E402
 from mini_train_sys_b200.runtime.device import resolve_device  # noqa: E402
-from mini_train_sys_b200.runtime.inference import generate, load_model_for_inference  # noqa: E402
+from mini_train_sys_b200.runtime.inference import KV_CACHES, generate, load_model_for_inference  # noqa: E402
 
 
 def main(argv=None) -> int:
@@ -37,12 +38,16 @@ def main(argv=None) -> int:
     ap.add_argument("--greedy", action="store_true")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--ops", default="torch")
+    ap.add_argument("--kv-cache", choices=KV_CACHES, default="none",
+                    help="int8: encode every token once and keep its keys and values in 8 bits; none: re-encode the prefix every step")
     ap.add_argument("--device", choices=["auto", "cpu", "cuda"], default="auto")
     args = ap.parse_args(argv)
 
     device = resolve_device(args.device)
     payload = load_yaml_dict(args.model_config).get("model") if args.model_config else None
-    model = load_model_for_inference(args.checkpoint, model_payload=payload, ops=args.ops, device=device)
+    # the cached decoding kernels work on bf16 activations
+    dtype = torch.bfloat16 if args.kv_cache != "none" and device.type == "cuda" and args.ops != "torch" else torch.float32
+    model = load_model_for_inference(args.checkpoint, model_payload=payload, ops=args.ops, device=device, dtype=dtype)
     tokenizer = None
     if args.tokenizer:
         from mini_train_sys_b200.data.tokenizer import load_tokenizer
@@ -60,7 +65,7 @@ def main(argv=None) -> int:
         raise SystemExit("prompt token id outside the model vocabulary")
     gen = torch.Generator(device=device.type if device.type == "cuda" else "cpu").manual_seed(args.seed)
     out = generate(model, torch.tensor([ids], device=device), max_new_tokens=args.max_new_tokens, temperature=args.temperature,
-                   top_k=args.top_k, greedy=args.greedy, generator=gen)[0].tolist()
+                   top_k=args.top_k, greedy=args.greedy, generator=gen, kv_cache=args.kv_cache)[0].tolist()
     record = {"event": "sample", "prompt_tokens": len(ids), "tokens": out}
     if tokenizer is not None:
         record["text"] = tokenizer.decode(out)

@@ -1,0 +1,142 @@
+"""A model's cached decoding against its plain forward pass, and the run of its parts together."""
+
+import pytest
+import torch
+
+from mini_train_sys_b200.models import MiniTransformer, ModelConfig, get_ops_backend
+from mini_train_sys_b200.runtime.inference import DecodeSession, generate
+
+
+def make_model(ffn, *, ops="torch", device="cpu", dtype=torch.float32, seq_len=64, hidden=128, heads=4, **kw):
+    torch.manual_seed(3)
+    cfg = ModelConfig(vocab_size=97, seq_len=seq_len, n_layers=2, n_heads=heads, hidden_size=hidden, intermediate_size=128, ffn_type=ffn,
+                      num_experts=4, experts_per_token=2, dropout=0.1, **kw)
+    return MiniTransformer(cfg, get_ops_backend(ops), activation_dtype=dtype).to(device).eval()
+
+
+@pytest.mark.parametrize("ffn", ["dense", "moe"])
+def test_fewer_tokens_than_a_block_decode_exactly(ffn):
+    """Up to 63 tokens nothing is in 8 bits: fp32 logits differ by the order of their sums only."""
+
+    model = make_model(ffn, tie_word_embeddings=ffn == "moe")
+    ids = torch.randint(0, 97, (3, 60))
+    with torch.no_grad():
+        full = model(ids)[1]
+    session = DecodeSession(model, 3, 63)
+    got = [session.prompt(ids[:, :20])]
+    got += [session.step(ids[:, i:i + 1]).clone() for i in range(20, 40)]
+    got.append(model.decode(ids[:, 40:], session.cache))                        # a second prompt on top of a filled cache
+    for position, logits in zip([19, *range(20, 40), 59], got):
+        torch.testing.assert_close(logits, full[:, position], rtol=1e-4, atol=1e-4)
+    assert session.cache.lengths.tolist() == [60, 60, 60]
+
+
+def test_padded_prompts_equal_single_ones():
+    model = make_model("moe")
+    ids = torch.randint(0, 97, (2, 30))
+    batch = DecodeSession(model, 2, 63)
+    logits = batch.prompt(ids, torch.tensor([30, 11]))
+    singles = []
+    for row, n in ((0, 30), (1, 11)):
+        alone = DecodeSession(model, 1, 63)
+        singles.append((alone, alone.prompt(ids[row:row + 1, :n])))
+    torch.testing.assert_close(logits, torch.cat([s[1] for s in singles]), rtol=1e-4, atol=1e-4)
+    token = torch.tensor([[5], [6]])
+    for _ in range(3):
+        got = batch.step(token)
+        torch.testing.assert_close(got, torch.cat([s.step(token[i:i + 1]) for i, (s, _) in enumerate(singles)]), rtol=1e-4, atol=1e-4)
+
+
+def test_generate_with_and_without_a_cache():
+    model = make_model("moe")
+    prompt = torch.randint(0, 97, (2, 9))
+    plain = generate(model, prompt, max_new_tokens=40, greedy=True)
+    assert torch.equal(generate(model, prompt, max_new_tokens=40, greedy=True, kv_cache="int8"), plain)
+    assert torch.equal(generate(model, prompt, max_new_tokens=0, kv_cache="int8"), prompt)
+    draws = [generate(model, prompt, max_new_tokens=8, top_k=5, generator=torch.Generator().manual_seed(1), kv_cache=k) for k in ("none", "int8")]
+    assert torch.equal(*draws)
+    with pytest.raises(ValueError, match="seq_len"):
+        generate(model, prompt, max_new_tokens=57, kv_cache="int8")
+    with pytest.raises(ValueError, match="kv_cache"):
+        generate(model, prompt, max_new_tokens=1, kv_cache="fp4")
+
+
+def test_refusals():
+    model = make_model("dense")
+    cache = model.new_cache(2)
+    ids = torch.randint(0, 97, (2, 4))
+    with pytest.raises(RuntimeError, match="eval"):
+        model.train().decode(ids, cache)
+    model.eval()
+    with pytest.raises(ValueError, match="another model"):
+        make_model("dense", heads=2).decode(ids, cache)
+    with pytest.raises(ValueError, match="cache of 2"):
+        model.decode(ids[:1], cache)
+    with pytest.raises(ValueError, match="seq_len"):
+        model.decode(torch.zeros(2, 65, dtype=torch.long), cache)
+    with pytest.raises(ValueError, match="one token per sequence"):
+        DecodeSession(model, 2).step(ids)
+    with pytest.raises(ValueError, match="captured step"):
+        DecodeSession(model, 2, graph=True)
+    other = model.new_cache(2)
+    other.dtype = torch.bfloat16
+    with pytest.raises(ValueError, match="activations"):
+        model.decode(ids, other)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ffn", ["dense", "moe"])
+def test_native_decoding_on_a_gpu(ffn):
+    """Prompt, steps and their captured form on the native kernels.  Fewer tokens than a block: nothing is in 8 bits, and a logit
+    differs from the plain pass's by bf16 roundings: some 2 x 8 of 2^-8 each along the residual path, 4 * 2^-8 together, doubled
+    for the head's weights."""
+
+    model = make_model(ffn, ops="native", device="cuda", dtype=torch.bfloat16, hidden=256, seq_len=256)
+    ids = torch.randint(0, 97, (3, 200), device="cuda")
+    with torch.no_grad():
+        full = model(ids[:, :60])[1].float()
+    sessions = {g: DecodeSession(model, 3, graph=g) for g in (False, True)}
+    for session in sessions.values():
+        first = session.prompt(ids[:, :20]).float()
+        assert (first - full[:, 19]).norm() <= 8 * 2 ** -8 * full[:, 19].norm()
+    for i in range(20, 200):
+        eager, replayed = (s.step(ids[:, i:i + 1]) for s in sessions.values())
+        assert torch.equal(eager, replayed) and torch.isfinite(eager).all(), i
+        if i < 60:
+            assert (eager.float() - full[:, i]).norm() <= 8 * 2 ** -8 * full[:, i].norm(), i
+    used = model.ops.dispatch_summary()
+    assert used["cached_attention:native"] and used["kv_append:native"] and not used.get("cached_attention:fallback")
+    assert (used.get("moe_tokens:native", 0) > 0) == (ffn == "moe")
+    assert sessions[True].cache.held == 200 and torch.equal(sessions[True].cache.records, sessions[False].cache.records)
+
+
+@pytest.mark.gpu
+def test_generate_on_a_gpu():
+    model = make_model("moe", ops="native", device="cuda", dtype=torch.bfloat16, hidden=256, seq_len=256)
+    prompt = torch.randint(0, 97, (2, 100), device="cuda")
+    out = generate(model, prompt, max_new_tokens=100, greedy=True, kv_cache="int8")
+    assert out.shape == (2, 200) and torch.equal(out[:, :100], prompt)
+    assert torch.equal(out, generate(model, prompt, max_new_tokens=100, greedy=True, kv_cache="int8"))
+
+
+def test_sample_command_with_a_cache(tmp_path, capsys, repo_root):
+    import importlib.util
+    import json
+
+    import yaml
+
+    spec = importlib.util.spec_from_file_location("sample_command", repo_root / "scripts" / "sample.py")
+    sample = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(sample)
+    model = make_model("moe")
+    torch.save(model.state_dict(), tmp_path / "model.pt")
+    payload = {"model": {"vocab_size": 97, "seq_len": 64, "n_layers": 2, "n_heads": 4, "hidden_size": 128, "intermediate_size": 128,
+                         "ffn_type": "moe", "num_experts": 4, "experts_per_token": 2}}
+    (tmp_path / "model.yaml").write_text(yaml.safe_dump(payload))
+    args = ["--checkpoint", str(tmp_path / "model.pt"), "--model-config", str(tmp_path / "model.yaml"), "--device", "cpu", "--prompt-ids", "1,2,3",
+            "--max-new-tokens", "6", "--greedy"]
+    tokens = []
+    for kind in ("none", "int8"):
+        assert sample.main([*args, "--kv-cache", kind]) == 0
+        tokens.append(json.loads(capsys.readouterr().out.strip().splitlines()[-1])["tokens"])
+    assert tokens[0] == tokens[1] and len(tokens[0]) == 9
