@@ -45,7 +45,7 @@ constexpr int kTile = 8192;              // bytes of a copy: 16 rows x 256 colum
 constexpr int kUpCols = 256, kUpRows = 8, kDownCols = 128, kDownRows = 32;
 constexpr int kColumns = 32;             // tokens of an entry: four products of eight
 constexpr int kEntries = kExperts + kRoutes / kColumns;
-constexpr int kSumPitch = kDownRows + 1;
+constexpr int kSumPitch = kDownRows + 4;  // floats; keeps four rows of a token on 16 bytes
 // Stages of a warp's ring in the first kernel, and in the second, whose sums need room too.
 constexpr int kUpStages = 3;
 __host__ __device__ constexpr int down_stages(int T) { return T <= 16 ? 3 : 2; }
@@ -68,6 +68,9 @@ struct Params {
   long long ldx;
   const void* router;
   int router_bf16;
+  const __nv_bfloat16* gate_up;
+  const __nv_bfloat16* down;
+  int prefetch_up, prefetch_down;        // bring weights to L2 ahead of their use
   __nv_bfloat16* y;
   __nv_bfloat16* hidden;       // [2][T * K][I]: high and low part
   int* routing;                // published: number of entries, the entries, order and token of every route, weights (1 + kEntries + 2 T K words)
@@ -75,12 +78,23 @@ struct Params {
   float* part;                 // [2 * CTAs][T][32]
   int* status;
   int T, E, K, H, I, normalize;
+  int tile_ctas;               // CTAs of a row tile in the second kernel; 0 where all CTAs share the list of units
   int up_warps, down_warps;    // warps of a CTA that stream: no more than can have work, so that small problems leave shared memory free
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// Asks for `bytes` at p to come to L2; p and bytes are multiples of 16.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  if (bytes > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+// The share of part i of n of a matrix of `bytes`.
+__device__ __forceinline__ void prefetch_share(const void* p, long long bytes, int i, int n) {
+  const long long share = (bytes / n / 16 + 1) * 16, begin = share * i;
+  if (begin < bytes) prefetch_l2(static_cast<const uint8_t*>(p) + begin, uint32_t(min(share, bytes - begin)));
 }
 
 // The ring of one warp.  Lane 0 starts copies; a stage is free once every lane has taken its fragments.
@@ -502,6 +516,9 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   ring.lane = lane;
   ring.init();
   if (threadIdx.x == 0) tma_prefetch_desc(&weights);
+  // While the routing kernel runs: bring what nearly all experts will be asked for to L2.
+  if (ROUTED && p.prefetch_up && threadIdx.x < p.E)
+    prefetch_share(p.gate_up + (long long)threadIdx.x * 2 * p.I * p.H, 4LL * p.I * p.H, blockIdx.x, gridDim.x);
   wait_for_previous();
   if constexpr (ROUTED) {
     read_routing<true>(p, r);
@@ -546,6 +563,8 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   if constexpr (!ROUTED) {
     if (blockIdx.x == 0) publish(p, r);
   }
+  if (p.prefetch_down && threadIdx.x < r.entries)          // what the second kernel will read
+    prefetch_share(p.down + (long long)r.entry_expert[threadIdx.x] * p.H * p.I, 2LL * p.H * p.I, blockIdx.x, gridDim.x);
 
   // The columns of up to 16 tokens of a unit are loaded before its tile is waited for, those of more in place.
   struct Columns {
@@ -640,8 +659,8 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int routes = p.T * p.K, sum_size = p.T * kSumPitch;
   float* sums = reinterpret_cast<float*>(smem + p.down_warps * down_stages(p.T) * kTile); // [warps][T][pitch]
-#pragma unroll 1
-  for (int i = threadIdx.x; i < p.down_warps * sum_size; i += kThreads) sums[i] = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x * 4; i < p.down_warps * sum_size; i += kThreads * 4) *reinterpret_cast<float4*>(sums + i) = make_float4(0.f, 0.f, 0.f, 0.f);
   if (threadIdx.x == 0) tma_prefetch_desc(&weights);
   Ring ring;
   ring.stages = down_stages(p.T);
@@ -656,10 +675,21 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   const int live = r.entries;
 
   const int steps = (p.I + kDownCols - 1) / kDownCols, tiles = (p.H + kDownRows - 1) / kDownRows;
-  const int per_tile = live * steps, N = tiles * per_tile, ctas = min(int(gridDim.x), N);
-  if (int(blockIdx.x) >= ctas) return;
-  const Parts parts(N, ctas);
-  const int c0 = parts.begin(blockIdx.x), c1 = parts.begin(blockIdx.x + 1);
+  const int per_tile = live * steps, N = tiles * per_tile;
+  // Small problems: a row tile is the work of as many CTAs as there are for each, so that every CTA has one piece to hand over.
+  const int group = min(p.tile_ctas, per_tile), ctas = group > 0 ? group : min(int(gridDim.x), N);
+  const Parts parts(group > 0 ? per_tile : N, ctas);
+  int c0, c1;
+  if (group > 0) {
+    const int tile = int(blockIdx.x) / p.tile_ctas, at = int(blockIdx.x) % p.tile_ctas;
+    if (tile >= tiles || at >= group) return;
+    c0 = tile * per_tile + parts.begin(at);
+    c1 = tile * per_tile + parts.begin(at + 1);
+  } else {
+    if (int(blockIdx.x) >= ctas) return;
+    c0 = parts.begin(blockIdx.x);
+    c1 = parts.begin(blockIdx.x + 1);
+  }
   // The units of this warp: its share of what the CTA has of each row tile, one after the other.
   struct Stream {
     int tile, u, end, expert, step;
@@ -798,15 +828,19 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     for (int i = threadIdx.x * 4; i < p.T * kDownRows; i += kThreads * 4) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
       float* at = sums + i / kDownRows * kSumPitch + i % kDownRows;
-#pragma unroll 4
-      for (int w = 0; w < p.down_warps; ++w, at += sum_size)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { v[k] += at[k]; at[k] = 0.f; }
+      for (int w = 0; w < kWarps; ++w, at += sum_size) {
+        if (w >= p.down_warps) break;
+        const float4 q = *reinterpret_cast<const float4*>(at);
+        *reinterpret_cast<float4*>(at) = make_float4(0.f, 0.f, 0.f, 0.f);
+        v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+      }
       if (whole) store(i, v);
       else *reinterpret_cast<float4*>(own + i) = make_float4(v[0], v[1], v[2], v[3]);
     }
     if (!whole) {
-      const int f = parts.owner(tile * per_tile), l = parts.owner((tile + 1) * per_tile - 1);
+      const int f = group > 0 ? tile * p.tile_ctas : parts.owner(tile * per_tile);
+      const int l = group > 0 ? f + group - 1 : parts.owner((tile + 1) * per_tile - 1);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -822,10 +856,14 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
         for (int i = threadIdx.x * 4; i < p.T * kDownRows; i += kThreads * 4) {
           const float4 q = __ldcg(reinterpret_cast<const float4*>(from + i));
           float v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll 8
-          for (int k = 0; k < l - f; ++k) {
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(rest + 2 * (long long)k * p.T * kDownRows + i));
-            v[0] += o.x; v[1] += o.y; v[2] += o.z; v[3] += o.w;
+#pragma unroll 1
+          for (int k0 = 0; k0 < l - f; k0 += 8) {
+            float4 o[8];                 // eight parts in flight
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              o[k] = k0 + k < l - f ? __ldcg(reinterpret_cast<const float4*>(rest + 2 * (long long)(k0 + k) * p.T * kDownRows + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) { v[0] += o[k].x; v[1] += o[k].y; v[2] += o[k].z; v[3] += o[k].w; }
           }
           store(i, v);
         }
@@ -858,6 +896,9 @@ bool encode_weights(CUtensorMap* map, const void* base, long long cols, long lon
 
 // Bytes of x and the router's weight up to which every CTA of the first kernel routes by itself.
 constexpr long long kRouteInPlace = 48 * 1024;
+constexpr long long kPrefetchBytes = 48ll << 20;
+// Units of a CTA up to which the second kernel gives a row tile to CTAs of its own.
+constexpr long long kSmallUnits = 32;
 
 size_t part_bytes(int T, int E) { return size_t(kWarps) * ((E + 15) / 16 * 16) * ((T + 7) / 8 * 8) * 4; }
 size_t route_shared(int T, int E) { return part_bytes(T, E) + size_t(2) * T * E * 4; }
@@ -924,6 +965,12 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   Params p;
   p.x = static_cast<const __nv_bfloat16*>(a.x); p.ldx = a.ldx;
   p.router = a.router; p.router_bf16 = a.router_bf16;
+  p.gate_up = static_cast<const __nv_bfloat16*>(a.gate_up);
+  p.down = static_cast<const __nv_bfloat16*>(a.down);
+  // Half of L2 at most, and gate and up only where the routing can be guessed: four routes an expert and more.
+  const long long matrix = 2LL * a.H * a.I;
+  p.prefetch_up = 2 * matrix * a.E <= kPrefetchBytes && (long long)a.T * a.K >= 4LL * a.E;
+  p.prefetch_down = matrix * entries <= kPrefetchBytes;
   p.y = static_cast<__nv_bfloat16*>(a.y);
   p.routing = reinterpret_cast<int*>(ws);
   p.hidden = reinterpret_cast<__nv_bfloat16*>(ws + w.hidden);
@@ -931,7 +978,10 @@ cudaError_t launch_moe_tokens(const MoeTokensArgs& a) {
   p.arrived = reinterpret_cast<unsigned*>(ws + w.arrived);
   p.status = a.status;
   p.T = a.T; p.E = a.E; p.K = a.K; p.H = a.H; p.I = a.I; p.normalize = a.normalize;
-  p.up_warps = warps_for(items); p.down_warps = warps_for(units);
+  const int row_tiles = (a.H + kDownRows - 1) / kDownRows;
+  p.tile_ctas = row_tiles <= sms / 2 && units <= kSmallUnits * sms ? sms / row_tiles : 0;
+  p.up_warps = warps_for(items);
+  p.down_warps = p.tile_ctas > 0 ? warps_for((units + row_tiles * p.tile_ctas - 1) / (row_tiles * p.tile_ctas) * sms) : warps_for(units);
   CUtensorMap up, down;
   if (!encode_weights(&up, a.gate_up, a.H, a.I, 2LL * a.E, kUpCols, kUpRows, 2) ||
       !encode_weights(&down, a.down, a.I, a.H, a.E, kDownCols, kDownRows, 1))
