@@ -615,14 +615,20 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
         mma_bf16(acc[0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b0.v[s].x, b0.v[s].y);
         mma_bf16(acc_odd, a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b0.v[s].z, b0.v[s].w);
       }
-#pragma unroll
-      for (int j = 1; j < kColumns / 8; ++j) {
-        if (j * 8 >= n) break;
-        if (j > 1) load(b1, rows[j], step);
+      auto multiply = [&](int j, const Columns& b) {
 #pragma unroll
         for (int s = 0; s < kUpCols / 32; ++s) {
-          mma_bf16(acc[j], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b1.v[s].x, b1.v[s].y);
-          mma_bf16(acc[j], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b1.v[s].z, b1.v[s].w);
+          mma_bf16(acc[j], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.v[s].x, b.v[s].y);
+          mma_bf16(acc[j], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.v[s].z, b.v[s].w);
+        }
+      };
+      if (n > 8) {                       // each set of columns is loaded while the one before is multiplied
+        if (n > 16) load(b0, rows[2], step);
+        multiply(1, b1);
+        if (n > 16) {
+          if (n > 24) load(b1, rows[3], step);
+          multiply(2, b0);
+          if (n > 24) multiply(3, b1);
         }
       }
     }
@@ -679,16 +685,18 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   // Small problems: a row tile is the work of as many CTAs as there are for each, so that every CTA has one piece to hand over.
   const int group = min(p.tile_ctas, per_tile), ctas = group > 0 ? group : min(int(gridDim.x), N);
   const Parts parts(group > 0 ? per_tile : N, ctas);
-  int c0, c1;
+  int c0, c1, first_tile;
   if (group > 0) {
-    const int tile = int(blockIdx.x) / p.tile_ctas, at = int(blockIdx.x) % p.tile_ctas;
-    if (tile >= tiles || at >= group) return;
-    c0 = tile * per_tile + parts.begin(at);
-    c1 = tile * per_tile + parts.begin(at + 1);
+    first_tile = int(blockIdx.x / unsigned(p.tile_ctas));
+    const int at = int(blockIdx.x) - first_tile * p.tile_ctas;
+    if (first_tile >= tiles || at >= group) return;
+    c0 = first_tile * per_tile + parts.begin(at);
+    c1 = first_tile * per_tile + parts.begin(at + 1);
   } else {
     if (int(blockIdx.x) >= ctas) return;
     c0 = parts.begin(blockIdx.x);
     c1 = parts.begin(blockIdx.x + 1);
+    first_tile = int(unsigned(c0) / unsigned(per_tile));
   }
   // The units of this warp: its share of what the CTA has of each row tile, one after the other.
   struct Stream {
@@ -701,14 +709,15 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
       s.u = s0 + shares.begin(min(warp, p.down_warps));
       s.end = s0 + shares.begin(min(warp + 1, p.down_warps));
       if (s.u == s.end) continue;
-      s.expert = (s.u - s.tile * per_tile) / steps;
-      s.step = (s.u - s.tile * per_tile) % steps;
+      s.expert = int(unsigned(s.u - s.tile * per_tile) / unsigned(steps));
+      s.step = s.u - s.tile * per_tile - s.expert * steps;
       return;
     }
     s.u = s.end = 0;
   };
-  Stream ahead{c0 / per_tile, 0, 0, 0, 0};
+  Stream ahead{first_tile, 0, 0, 0, 0};
   enter(ahead);
+  Stream now = ahead;                    // where the products are
   auto next_copy = [&]() {
     if (ahead.u == ahead.end) return;
     ring.copy(&weights, ahead.step * kDownCols, ahead.tile * kDownRows, r.entry_expert[ahead.expert]);
@@ -744,12 +753,13 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
   };
   float* mine = sums + warp * sum_size;
 #pragma unroll 1
-  for (int tile = c0 / per_tile; tile * per_tile < c1; ++tile) {
+  for (int tile = first_tile; tile * per_tile < c1; ++tile) {
     const int s0 = max(c0, tile * per_tile), s1 = min(c1, (tile + 1) * per_tile);
-    const Parts shares(s1 - s0, p.down_warps);
-    const int u = s0 + shares.begin(min(warp, p.down_warps));
-    int units = s0 + shares.begin(min(warp + 1, p.down_warps)) - u;
-    int at_entry = (u - tile * per_tile) / steps, step = (u - tile * per_tile) % steps;
+    int units = now.tile == tile ? now.end - now.u : 0, at_entry = now.expert, step = now.step;
+    if (now.tile == tile) {
+      ++now.tile;
+      enter(now);
+    }
 #pragma unroll 1
     for (; units > 0; ++at_entry) {      // one entry of this row tile
       const int n0 = r.entry_begin[at_entry], n = r.entry_tokens[at_entry];
@@ -790,11 +800,14 @@ moe_down_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
               }
         };
         multiply(0, b0);
-#pragma unroll
-        for (int j = 1; j < kColumns / 8; ++j) {
-          if (j * 8 >= n) break;
-          if (j > 1) load(b1, rows[j], step);
-          multiply(j, b1);
+        if (n > 8) {
+          if (n > 16) load(b0, rows[2], step);
+          multiply(1, b1);
+          if (n > 16) {
+            if (n > 24) load(b1, rows[3], step);
+            multiply(2, b0);
+            if (n > 24) multiply(3, b1);
+          }
         }
       }
       step = 0;
