@@ -6,9 +6,7 @@
 // share a K/V head, times the new tokens of the step).  Every warp has a ring of blocks of its own in shared memory, which bulk
 // copies fill (one for the keys of a block with its scales, one for its values), so the warps run without barriers and each
 // keeps 8 to 16 KB of the cache in flight.  A lane's 16 adjacent bytes are its K or V fragment of several steps (the V rows are
-// stored in that order); 4 bytes become two fp16 pairs in two instructions, 1152 too large, or in four.  Keys stay too large, and a
-// score starts from what that adds (-1152 times the sum of the query: 1e-5 in a logit, the same for every key); values do not,
-// because their sums cancel over a long context (8e-4 of an output over 131k tokens; exact values: 2e-4, the rounding to fp16).  Both products run on m16n8k16 with the tokens (K) or
+// stored in that order); 4 bytes become two fp16 pairs in four instructions; both products run on m16n8k16 with the tokens (K) or
 // the head's dims (V) as rows and eight query rows as columns.  The (sequence, head, row tile, block) units of
 // the whole batch are one list, cut into equal parts for the warps that fit on the machine: sequences of unlike lengths, and a
 // single long one, keep every SM busy, and a warp streams across the ends of sequences.  A second kernel joins the parts of
@@ -378,7 +376,6 @@ cached_attention_kernel(const Params p) {
 
     uint32_t qf[NQ][KW][2];              // fp16 query fragments, scaled: column g of every tile, dims 4 KW c ... of the head
     float qscale[NQ][2];                 // log2(e) / sqrt(D) times the power of two taken out, for the columns 2c, 2c + 1
-    float qbias[NQ][2];                  // -1152 times the sum of the scaled query
     int limit[NQ][2];                    // last position that a column sees
     int start = 0, fresh = 0;
     int stage = 0;
@@ -417,11 +414,6 @@ cached_attention_kernel(const Params p) {
               qf[n][i][j] = Act<T>::kHalf ? w[2 * i + j] : pack_half2(Act<T>::lo(w[2 * i + j]) * down, Act<T>::hi(w[2 * i + j]) * down);
 #pragma unroll
           for (int j = 0; j < 2; ++j) qscale[n][j] = p.sm_log2 * __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < KW; ++i) mma_f16(sum, kOnes, kOnes, kOnes, kOnes, qf[n][i][0], qf[n][i][1]);
-          qbias[n][0] = -kCodeBias * sum[0];
-          qbias[n][1] = -kCodeBias * sum[1];
         }
       }
       if (cur.at < cur.closed) {
@@ -442,12 +434,11 @@ cached_attention_kernel(const Params p) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               uint32_t a0, a1, a2, a3;
-              codes_to_biased(kr[m][0][i], a0, a2);
-              codes_to_biased(kr[m][1][i], a1, a3);
+              codes_to_half(kr[m][0][i], a0, a2);
+              codes_to_half(kr[m][1][i], a1, a3);
 #pragma unroll
               for (int n = 0; n < NQ; ++n) {
-                const float from[4] = {qbias[n][0], qbias[n][1], qbias[n][0], qbias[n][1]};
-                if (i == 0) mma_f16_from(s[m0 + m][n], from, a0, a1, a2, a3, qf[n][0][0], qf[n][0][1]);
+                if (i == 0) mma_f16_first(s[m0 + m][n], a0, a1, a2, a3, qf[n][0][0], qf[n][0][1]);
                 else mma_f16(s[m0 + m][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
               }
             }
@@ -497,7 +488,6 @@ cached_attention_kernel(const Params p) {
           for (int d = 0; d < 2; ++d)
 #pragma unroll
             for (int v = 0; v < 2; ++v) read_words<4>(vst + (16 * (d0 + d) + 8 * v) * BLK, vr[d][v]);
-          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
           float acc[2][NQ][4];
 #pragma unroll
           for (int m = 0; m < 4; ++m)
@@ -508,7 +498,7 @@ cached_attention_kernel(const Params p) {
               codes_to_half(vr[d][1][m], a1, a3);
 #pragma unroll
               for (int n = 0; n < NQ; ++n) {
-                if (m == 0) mma_f16_from(acc[d][n], zero, a0, a1, a2, a3, pf[0][n][0], pf[0][n][1]);
+                if (m == 0) mma_f16_first(acc[d][n], a0, a1, a2, a3, pf[0][n][0], pf[0][n][1]);
                 else mma_f16(acc[d][n], a0, a1, a2, a3, pf[m][n][0], pf[m][n][1]);
               }
             }

@@ -362,35 +362,57 @@ __device__ __forceinline__ void router_products(const Params& p, float* part, in
   }
 }
 
-// The logits [t][e] of up to four tokens: a warp an expert, all loads of 1024 columns in flight, every sum in the same order.
+// The logits [t][e] of up to four tokens: a warp an expert, the loads of 1024 columns in flight, every sum in the same order.
 constexpr int kFewTokens = 4;
 __device__ __forceinline__ void router_few(const Params& p, float* logits) {
   const int lane = threadIdx.x & 31;
+  constexpr int AHEAD = 4;
 #pragma unroll 1
   for (int e = threadIdx.x >> 5; e < p.E; e += kWarps) {
     float acc[kFewTokens] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int d = lane * 8; d < p.H; d += 256) {
-      float w[8];
-      if (p.router_bf16) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.router) + (long long)e * p.H + d));
-        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll 1
+    for (int d0 = lane * 8; d0 < p.H; d0 += 256 * AHEAD) {
+      float4 w[AHEAD][2];
+      uint4 x[AHEAD][kFewTokens];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { w[2 * i] = __uint_as_float(v[i] << 16); w[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u); }
-      } else {
-        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + (long long)e * p.H + d);
-        const float4 a = __ldg(src), b = __ldg(src + 1);
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+      for (int i = 0; i < AHEAD; ++i) {
+        const int d = d0 + 256 * i;
+        w[i][0] = w[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d < p.H) {
+          const long long at = (long long)e * p.H + d;
+          if (p.router_bf16) {
+            w[i][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const __nv_bfloat16*>(p.router) + at));          // eight bf16 values
+          } else {
+            w[i][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at));
+            w[i][1] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at) + 1);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kFewTokens; ++t) {
+          x[i][t] = make_uint4(0, 0, 0, 0);
+          if (d < p.H && t < p.T) x[i][t] = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.ldx + d));
+        }
       }
 #pragma unroll
-      for (int t = 0; t < kFewTokens; ++t) {
-        if (t >= p.T) break;
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.ldx + d));
-        const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+      for (int i = 0; i < AHEAD; ++i) {
+        float v[8] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w, w[i][1].x, w[i][1].y, w[i][1].z, w[i][1].w};
+        if (p.router_bf16) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[t] = fmaf(__uint_as_float(v[i] << 16), w[2 * i], acc[t]);
-          acc[t] = fmaf(__uint_as_float(v[i] & 0xFFFF0000u), w[2 * i + 1], acc[t]);
+          for (int j = 3; j >= 0; --j) {
+            const uint32_t pair = __float_as_uint(v[j]);
+            v[2 * j + 1] = __uint_as_float(pair & 0xFFFF0000u);
+            v[2 * j] = __uint_as_float(pair << 16);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kFewTokens; ++t) {
+          if (t >= p.T) break;
+          const uint32_t q[4] = {x[i][t].x, x[i][t].y, x[i][t].z, x[i][t].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[t] = fmaf(__uint_as_float(q[j] << 16), v[2 * j], acc[t]);
+            acc[t] = fmaf(__uint_as_float(q[j] & 0xFFFF0000u), v[2 * j + 1], acc[t]);
+          }
         }
       }
     }

@@ -26,7 +26,10 @@ _SLOT = [((t & 7) >> 1) * 16 + (t >> 4) * 4 + ((t >> 3) & 1) * 2 + (t & 1) for t
 
 
 class QuantizedKVCache:
-    """Cache of all layers of a model; the operators take it with a layer index."""
+    """Cache of all layers of a model; the operators take it with a layer index.
+
+    The buffers are made once and written in place (captured graphs and the native layers hold their addresses); a copy of the
+    object (``copy.deepcopy``) has its own."""
 
     def __init__(self, *, layers: int, batch: int, kv_heads: int, head_dim: int, capacity: int, dtype: torch.dtype = torch.bfloat16,
                  device: torch.device | str = "cuda") -> None:
@@ -51,6 +54,9 @@ class QuantizedKVCache:
         self.padded: int | None = None  # padded number of new tokens of the open step
 
         self.native: dict[int, object] = {}     # layers as the native backend holds them
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "native": {}}      # a copy (of a beam, of a shared prompt) has buffers of its own
 
     @property
     def codes(self) -> torch.Tensor:

@@ -37,7 +37,8 @@ def fill(ops, cache, layer, k, v, lengths):
 def assert_attention(o, q, keys, values, starts, counts):
     """Bound per output: its own rounding (half a step), and 2^-11 (fp16 probabilities: half a step each) of sum p |v|, with a
     quarter more for the fp32 sums and exponentials behind them.  Probabilities are held times 2^14, where the smallest fp16 value
-    is 2^-24: below 2^-39 of the largest one a probability is lost, which is at most 2^-39 of the largest value for each key."""
+    is 2^-24: below 2^-39 of the largest one a probability is lost, which is at most 2^-39 of the largest value for each key.
+    Outputs below the type's smallest normal value are rounded to half of its smallest step."""
 
     half = torch.finfo(o.dtype).eps / 2
     for b, (s, n) in enumerate(zip(starts, counts)):
@@ -47,6 +48,7 @@ def assert_attention(o, q, keys, values, starts, counts):
         want, mass = dr.attend(q[b, :, :n], dr.held(keys[b, :, :s + n]), dr.held(values[b, :, :s + n]), s)
         err = (o[b, :, :n].double() - want).abs()
         bound = half * want.abs() + 1.25 * 2 ** -11 * mass + 2 ** -39 * (s + n) * values[b, :, :s + n].abs().max().double()
+        bound += torch.finfo(o.dtype).tiny * half
         assert torch.isfinite(o[b, :, :n]).all() and (err <= bound).all(), (b, float((err - bound).max()))
 
 
@@ -188,6 +190,31 @@ def test_a_non_finite_token_stays_in_its_sequence_and_its_block(ops):
     assert outs[1][1, :, 70:].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_queries_and_repeated_steps_and_copies(ops, dtype):
+    """Logits of some hundreds; a step that is appended twice; a copy that goes on by itself."""
+
+    import copy
+
+    k, v = rows(2, 2, 700, 64, 14, dtype), rows(2, 2, 700, 64, 15, dtype, spread=False)
+    q = (rows(2, 6, 20, 64, 16, torch.float32, spread=False) * 8).to(dtype)
+    q[:, 2:4] = (q[:, 2:4].float() * 4).to(dtype).abs()           # no sign cancels in the sums
+    cache = QuantizedKVCache(layers=1, batch=2, kv_heads=2, head_dim=64, capacity=704, dtype=dtype, device=DEV)
+    fill(ops, cache, 0, k, v, [640, 597])
+    fresh = [torch.stack([t[b, :, s:s + 20] for b, s in enumerate((640, 597))]) for t in (k, v)]
+    other = copy.deepcopy(cache)
+    for c, repeats in ((cache, 2), (other, 1)):
+        for _ in range(repeats):
+            c.begin(padded=20)
+            ops.kv_append(c, 0, *fresh)
+        assert_attention(ops.cached_attention(q, c, 0), q, k, v, [640, 597], [20, 20])
+        c.commit()
+    assert torch.equal(cache.records, other.records) and cache.records.data_ptr() != other.records.data_ptr()
+    cache.begin(padded=20)
+    ops.kv_append(cache, 0, *fresh)
+    assert other.lengths.tolist() == [660, 617] and not torch.equal(cache.tail, other.tail)
+
+
 def test_two_streams_and_replays(ops):
     """Two caches on two streams at once, and one captured step replayed while its lengths move on, equal the plain calls."""
 
@@ -269,6 +296,16 @@ def test_moe_tokens(ops, tokens, experts, top_k, hidden, inter):
         assert_moe(y, dr.moe(x, r, gu, dn, top_k, normalize))
         assert torch.equal(y, ops.moe_tokens(x, r, gu, dn, top_k, normalize=normalize))
     assert ops.dispatch["moe_tokens:native"] and not ops.dispatch["moe_tokens:fallback"]
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 4, 5])
+@pytest.mark.parametrize("router_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("experts,hidden", [(8, 768), (24, 2056)])
+def test_moe_tokens_of_both_routings(ops, tokens, router_dtype, experts, hidden):
+    """Few tokens and many, small routers and large ones are routed by different code."""
+
+    x, r, gu, dn = moe_inputs(tokens, experts, hidden, 64, 7, router_dtype)
+    assert_moe(ops.moe_tokens(x, r, gu, dn, 3, normalize=True), dr.moe(x, r, gu, dn, 3, True))
 
 
 def test_moe_tokens_crowded_ties_strides_and_weights(ops):
