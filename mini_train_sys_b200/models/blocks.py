@@ -178,7 +178,8 @@ class MoEFeedForward(nn.Module):
         """The layer in a decoding step: a few tokens go through the backend's one-call form (no balance statistics)."""
 
         tokens = x.reshape(-1, x.shape[-1])
-        if tokens.shape[0] > FEW_TOKENS or self.expert_dispatch is not None or not hasattr(ops, "moe_tokens"):
+        limited = self.router.enforce_capacity and self.cfg.expert_capacity_factor is not None
+        if tokens.shape[0] > FEW_TOKENS or limited or self.expert_dispatch is not None or not hasattr(ops, "moe_tokens"):
             return self(x, ops, residual=residual).hidden_states
         y = ops.moe_tokens(tokens, self.router.weight, self.gate_up_proj, self.down_proj, self.cfg.experts_per_token,
                            normalize=self.cfg.router_normalize_topk)

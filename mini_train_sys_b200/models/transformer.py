@@ -117,6 +117,18 @@ class MiniTransformer(nn.Module):
         logits = project(self.ops, self.lm_head, hidden)
         return self.ops.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1)), logits
 
+    def check_decodable(self) -> None:
+        """Refuse what cached decoding would pass over: it calls the parts of a block one by one, so neither a module's hooks (analysis,
+        staged parameters of a sharding engine) nor a wrapper's forward would run."""
+
+        if not hasattr(self.ops, "cached_attention"):
+            raise ValueError(f"the {self.ops.name!r} operators have no cached decoding")
+        for block in self.blocks:
+            if not isinstance(block, TransformerBlock):
+                raise RuntimeError(f"cached decoding needs a plain model, not blocks wrapped in {type(block).__name__}")
+            if any(m._forward_hooks or m._forward_pre_hooks for m in block.modules()):
+                raise RuntimeError("cached decoding does not run the hooks that are registered on the model's blocks")
+
     @torch.no_grad()
     def decode(self, input_ids: torch.Tensor, cache, counts: torch.Tensor | None = None) -> torch.Tensor:
         """One step of cached decoding: append ``input_ids`` [B, T] to ``cache`` (``QuantizedKVCache``) and return the logits [B, V]
@@ -127,6 +139,7 @@ class MiniTransformer(nn.Module):
 
         if self.training:
             raise RuntimeError("decode() needs eval mode")
+        self.check_decodable()
         if cache.layers != len(self.blocks) or cache.kv_heads != self.cfg.n_heads or cache.head_dim != self.cfg.head_dim:
             raise ValueError("the cache was made for another model")
         if cache.dtype != self.activation_dtype:

@@ -84,6 +84,13 @@ def bf16_weight(weight: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def kept_bf16(weight: torch.Tensor) -> torch.Tensor | None:
+    """The copy that ``bf16_weight`` holds of ``weight``, if any."""
+
+    hit = _weight_cache.get(weight.data_ptr())
+    return hit[3] if hit is not None and hit[0]() is not None else None
+
+
 def _gemm(a, b, out, M, N, K, *, a_mn=False, b_mn=False, mode=GEMM_DENSE, epilogue=EPI_STORE, accumulate=False,
           atomic_out=False, aux=None, tile_group=None, num_row_tiles=None, group_rows=None, num_groups=1,
           b_group_stride_rows=0, out_group_stride=0, ldo=None, sm_limit=0, pair=None, k_splits=1, gather_a=None, gather_b=None,

@@ -63,21 +63,29 @@ def evaluate_loss(model: MiniTransformer, loader, device: torch.device, *, max_b
 KV_CACHES = ("none", "int8")
 
 
+# operators whose plain forms ask the device for numbers, which a captured step cannot
+_CAPTURED_OPS = ("kv_append", "cached_attention", "moe_tokens", "fused_moe")
+
+
 class DecodeSession:
     """Cached decoding of one batch: ``prompt`` once, then ``step`` by step.
 
     On a GPU with the native operators a step is captured into a CUDA graph after the first one and replayed: a step is some
-    hundred short kernels, whose launches take longer than their work."""
+    hundred short kernels, whose launches take longer than their work.  Where the kernels do not cover the model (a head dimension
+    other than 32, 64 and 128, ...) steps stay eager, or are refused with ``graph=True``.  Weights that change in place or move are
+    noticed, and the step is captured again; a model whose parameters are replaced by others needs a new session."""
 
     def __init__(self, model: MiniTransformer, batch: int, capacity: int | None = None, *, graph: bool | None = None) -> None:
         self.model = model
+        model.check_decodable()
         self.cache = model.new_cache(batch, capacity)
         on_gpu = self.cache.device.type == "cuda" and getattr(model.ops, "name", "") == "native" and model.activation_dtype == torch.bfloat16
         if graph and not on_gpu:
             raise ValueError("a captured step needs a GPU, the native operators and bf16 activations")
         self.graph_wanted = on_gpu if graph is None else bool(graph)
+        self._insisted = bool(graph)
         self._graph: torch.cuda.CUDAGraph | None = None
-        self._steps = 0
+        self._prepared = False
 
     def prompt(self, input_ids: torch.Tensor, counts: torch.Tensor | None = None) -> torch.Tensor:
         """Logits [B, V] behind the prompts [B, T]; ``counts`` [B] are their lengths where they are padded on the right."""
@@ -89,24 +97,62 @@ class DecodeSession:
 
         if token_ids.shape != (self.cache.batch, 1):
             raise ValueError(f"a step takes one token per sequence, got {tuple(token_ids.shape)}")
-        self._steps += 1
-        if not self.graph_wanted or self._steps == 1:          # the first step lays out what the kernels keep
+        if not self.graph_wanted:
             return self.model.decode(token_ids, self.cache)
+        if self._graph is not None and self._weights() != self._captured:
+            self._graph, self._prepared = None, False
+        if not self._prepared:
+            return self._eager_step(token_ids)
         if self.cache.held + 1 > self.model.rotary.max_seq_len:
             raise ValueError(f"{self.cache.held} cached + 1 new tokens exceed the model's seq_len of {self.model.rotary.max_seq_len}")
         if self._graph is None:
-            self._ids = token_ids.clone()
-            held = self.cache.held
-            torch.cuda.synchronize(self.cache.device)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.device(self.cache.device), torch.cuda.graph(graph):
-                self._logits = self.model.decode(self._ids, self.cache)
-            self.cache.held = held                             # capturing has run nothing
-            self._graph = graph
+            self._capture(token_ids)
+        if self.model.training:
+            raise RuntimeError("decode() needs eval mode")
+        if any(m._forward_hooks or m._forward_pre_hooks for m in self._modules):
+            self.model.check_decodable()
         self.cache.replayed(1)
         self._ids.copy_(token_ids)
         self._graph.replay()
         return self._logits
+
+    def _eager_step(self, token_ids: torch.Tensor) -> torch.Tensor:
+        """The step before a capture: it lays out what the kernels keep, and shows whether they cover the model."""
+
+        def plain_calls() -> int:
+            return sum(self.model.ops.dispatch[f"{op}:fallback"] for op in _CAPTURED_OPS)
+
+        before = plain_calls()
+        logits = self.model.decode(token_ids, self.cache)
+        if plain_calls() != before:
+            if self._insisted:
+                raise ValueError("the native kernels do not cover this model: its steps cannot be captured")
+            self.graph_wanted = False
+        self._prepared = True
+        return logits
+
+    def _capture(self, token_ids: torch.Tensor) -> None:
+        from mini_train_sys_b200.ops.native_backend import kept_bf16
+
+        self._ids = token_ids.clone()
+        self._modules = list(self.model.blocks.modules())
+        self._tensors = [*self.model.parameters(), *self.model.buffers()]
+        held = self.cache.held
+        torch.cuda.synchronize(self.cache.device)
+        graph = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.device(self.cache.device), torch.cuda.graph(graph):
+                self._logits = self.model.decode(self._ids, self.cache)
+        finally:
+            self.cache.held, self.cache.padded = held, None        # capturing has run nothing
+        self._copies = [kept_bf16(t) for t in self._tensors]           # the graph reads them: not to be freed while it lives
+        self._captured = self._weights()
+        self._graph = graph
+
+    def _weights(self) -> list[tuple[int, int]]:
+        """Addresses and versions of the weights: a graph reads them where they were, and bf16 copies of fp32 ones as they were."""
+
+        return [(t.data_ptr(), 0 if t.is_inference() else t._version) for t in self._tensors]
 
 
 def _next_token(logits: torch.Tensor, temperature: float, top_k: int | None, greedy: bool, generator) -> torch.Tensor:

@@ -84,6 +84,46 @@ def test_refusals():
         model.decode(ids, other)
 
 
+def test_an_enforced_capacity_holds_in_decoding():
+    """Routes beyond an expert's capacity are dropped as in the plain pass over the same tokens."""
+
+    model = make_model("moe", expert_capacity_factor=0.5, expert_min_capacity=1)
+    ids = torch.randint(0, 97, (3, 20))
+    free = model.decode(ids, model.new_cache(3))
+    for block in model.blocks:
+        block.ffn.router.enforce_capacity = True
+    with torch.no_grad():
+        full = model(ids)[1][:, -1]
+    assert not torch.allclose(free, full, rtol=1e-3, atol=1e-3)
+    torch.testing.assert_close(model.decode(ids, model.new_cache(3)), full, rtol=1e-4, atol=1e-4)
+
+
+def test_what_decoding_would_pass_over_is_refused():
+    ids = torch.randint(0, 97, (2, 4))
+    with pytest.raises(ValueError, match="no cached decoding"):
+        DecodeSession(make_model("moe", ops="reference"), 2)
+    model = make_model("moe")
+    session = DecodeSession(model, 2)
+    for part in (model.blocks[1], model.blocks[0].ffn.router):
+        handle = part.register_forward_hook(lambda *_: None)
+        with pytest.raises(RuntimeError, match="hooks"):
+            session.prompt(ids)
+        handle.remove()
+    session.prompt(ids)
+
+    class Wrapper(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def __getattr__(self, name):
+            return super().__getattr__(name) if name == "inner" else getattr(self.inner, name)
+
+    model.blocks[0] = Wrapper(model.blocks[0])
+    with pytest.raises(RuntimeError, match="Wrapper"):
+        session.step(ids[:, :1])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("ffn", ["dense", "moe"])
 def test_native_decoding_on_a_gpu(ffn):
@@ -108,6 +148,42 @@ def test_native_decoding_on_a_gpu(ffn):
     assert used["cached_attention:native"] and used["kv_append:native"] and not used.get("cached_attention:fallback")
     assert (used.get("moe_tokens:native", 0) > 0) == (ffn == "moe")
     assert sessions[True].cache.held == 200 and torch.equal(sessions[True].cache.records, sessions[False].cache.records)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [2, 65])
+def test_captured_steps_follow_the_weights(batch):
+    """A batch whose tokens take the one-call form of the experts and one whose tokens are sorted; weights changed between steps."""
+
+    model = make_model("moe", ops="native", device="cuda", dtype=torch.bfloat16, hidden=256, seq_len=256)
+    ids = torch.randint(0, 97, (batch, 30), device="cuda")
+    eager, replayed = (DecodeSession(model, batch, graph=g) for g in (False, True))
+    for session in (eager, replayed):
+        session.prompt(ids[:, :20])
+    seen = []
+    for i in range(20, 30):
+        if i in (23, 27):
+            with torch.no_grad():
+                for p in model.blocks.parameters():
+                    p.mul_(1.25)
+        seen.append(replayed._graph)
+        assert torch.equal(eager.step(ids[:, i:i + 1]), replayed.step(ids[:, i:i + 1])), i
+    assert replayed._graph is not None and len({id(g) for g in seen if g is not None}) >= 2
+    handle = model.blocks[0].attn.register_forward_hook(lambda *_: None)
+    with pytest.raises(RuntimeError, match="hooks"):
+        replayed.step(ids[:, :1])
+    handle.remove()
+
+
+@pytest.mark.gpu
+def test_a_model_that_the_kernels_do_not_cover_decodes_eagerly():
+    model = make_model("moe", ops="native", device="cuda", dtype=torch.bfloat16, hidden=192, seq_len=256)      # heads of 48
+    prompt = torch.randint(0, 97, (2, 10), device="cuda")
+    assert generate(model, prompt, max_new_tokens=6, greedy=True, kv_cache="int8").shape == (2, 16)
+    session = DecodeSession(model, 2, graph=True)
+    session.prompt(prompt)
+    with pytest.raises(ValueError, match="do not cover"):
+        session.step(prompt[:, :1])
 
 
 @pytest.mark.gpu
