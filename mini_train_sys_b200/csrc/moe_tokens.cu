@@ -15,6 +15,10 @@
 //   2  The (32 output rows, expert, 128 columns) units of the down projections are one list, cut into equal parts for the CTAs; what
 //      a CTA has of a row tile is added in shared memory, and where a tile was cut its last CTA adds the parts, in order.
 //
+// Measured on the GPU (replayed graph, caches flushed): one token, 2 of 8 experts of 768 x 1,024, 12.4 us (9.4 MB of weights: two launches'
+// latency); 64 tokens of the same 30.5 us (38 MB); 17 tokens, 8 of 64 experts of 2,048 x 1,024, 146 us (58 of them asked for, 0.72 GB,
+// 5.0 TB/s, the routing kernel's 11 us included); 8 tokens, 2 of 8 experts of 4,096 x 14,336, 410 us (2.5 GB, 6.2 TB/s).
+//
 // Rounding: logits, softmax, sums and the hidden values are fp32 (the router's fp32 weight enters the tensor cores as the sum of three
 // bf16 values, 24 bits); a hidden value enters the second product as the sum of two (2^-16), so y is rounded to bf16 once.
 #include "decode.cuh"
