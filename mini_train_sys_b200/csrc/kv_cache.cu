@@ -3,7 +3,7 @@
 //   a = max |x| over the 64 x D values of a finished block,  scale = a / 127,  code = rint(127 x / a)  (half to even)
 //
 // What bounds them: appending reads the new tokens once and writes their codes, 3 bytes a value (and q, 4 bytes a value); reading
-// back reads a byte a value and writes two.  So they are bound by memory for a prompt and by their launch for one token.
+// back reads a byte a value and writes four.  So they are bound by memory for a prompt and by their launch for one token.
 // Measured on the GPU (replayed graph, caches flushed), an append and a read-back of 12 heads of 64: one sequence of 448 tokens,
 // one new, 6.4 us; 64 ragged sequences of up to 512 tokens, one new, 18.4 us (50 MB moved, 2.7 TB/s); 16 ragged prompts of up to
 // 2,048 tokens 80.7 us (338 MB, 4.2 TB/s), of which the append, whose conversions keep the issue slots busy, takes half.

@@ -9,6 +9,9 @@ minitrain/model/ops.py:18-90).  Three implementations exist:
 
 The reference names ``triton`` and ``cuda`` are accepted as aliases of ``native`` so
 that reference run YAMLs keep loading.
+
+Beside the protocol, ``torch`` and ``native`` have the operators of cached decoding: ``kv_append``, ``cached_attention``,
+``kv_read`` and ``moe_tokens`` (documented in ``ops/torch_backend.py``; no gradient).
 """
 
 from __future__ import annotations
