@@ -5,8 +5,8 @@
 // What bounds them: appending reads the new tokens once and writes their codes, 3 bytes a value (and q, 4 bytes a value); reading
 // back reads a byte a value and writes four.  So they are bound by memory for a prompt and by their launch for one token.
 // Measured on the GPU (replayed graph, caches flushed), an append and a read-back of 12 heads of 64: one sequence of 448 tokens,
-// one new, 6.4 us; 64 ragged sequences of up to 512 tokens, one new, 18.4 us (50 MB moved, 2.7 TB/s); 16 ragged prompts of up to
-// 2,048 tokens 80.7 us (338 MB, 4.2 TB/s), of which the append, whose conversions keep the issue slots busy, takes half.
+// one new, 5.2 us; 64 ragged sequences of up to 512 tokens, one new, 18.2 us (51 MB, 2.8 TB/s); 16 ragged prompts of up to
+// 2,048 tokens 78.2 us (338 MB, 4.3 TB/s), of which the append, whose conversions keep the issue slots busy, takes half.
 #include "decode.cuh"
 #include "launch.cuh"
 #include "ops.cuh"
@@ -272,78 +272,83 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
   }
 }
 
-// One CTA per 64 positions of a (sequence, K/V head), which lie in two blocks at most.  The values of a block are stored by dim, so
-// they pass through shared memory; then D / 4 consecutive threads write the dims of one token.
+// One CTA of D threads per 64 positions of a (sequence, K/V head), which lie in two blocks at most.  A thread has four dims of the 16
+// tokens whose values are adjacent in a row of V: it reads 16 bytes of four rows of V and four dims of each token's keys, so the
+// values need not pass through shared memory to be written by token, all loads are in flight at once, and two lanes with
+// neighbouring tokens use a whole sector of V between them.
+template <int D>
+struct ReadThread {
+  static constexpr int VEC = D / 4, L = VEC < 16 ? VEC : 16;
+  int a, dim;                            // the tokens 2 a + {0, 1, 8, 9} of every 16; first dim
+  __device__ __forceinline__ ReadThread(int tid) : a(tid / L % 4), dim((tid % L + tid / (4 * L) * L) * 4) {}
+  __device__ __forceinline__ int token(int x) const { return 2 * a + ((x >> 1) & 1) * 8 + (x & 1); }
+};
+
+// code - 128 from byte x of w: 2^23 + code is the float with code in its low bits
+__device__ __forceinline__ float decode(uint32_t w, int x) { return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + x)) - 8388736.f; }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(D)
 kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restrict__ ko, float* __restrict__ vo, int chunks) {
   constexpr int BLK = kCacheBlock;
-  constexpr int PITCH = BLK + 4;                           // bytes of a row of codes
-  constexpr int HALF_PITCH = BLK / 2 + 2;                  // values of a row of half the unfinished block
-  __shared__ __align__(16) uint8_t codes_sm[2][D * PITCH];
-  __shared__ __align__(16) T tail_sm[2 * D * HALF_PITCH];
   let_next_start();
   wait_for_previous();
+  const ReadThread<D> me(threadIdx.x);
   const int chunk = int(blockIdx.x) % chunks;
   const int bh = int(blockIdx.x) / chunks;
   const int b = bh / c.Hkv;
   const int total = min(min(max(c.start[b], 0), c.blocks * BLK) + max(c.count[b], 0), c.blocks * BLK), closed = total / BLK;
-  const long long p0 = (long long)first[b] + chunk * 64;
-  const int lo = int(max(p0, 0ll) / BLK);                  // the two blocks
-  const uint8_t* record0 = c.records + ((long long)bh * c.blocks + lo) * record_bytes(D);
-  const T* tail = static_cast<const T*>(c.tail) + ((long long)bh * 2 + (closed & 1)) * 2 * BLK * D;
-  const bool reaches = p0 + 64 > 0 && p0 < total;          // else only zeros are written
+  const long long from = first[b], p0 = from + chunk * 64;
+  const long long out0 = (long long)bh * n - from;         // row of position 0
+#pragma unroll 1
+  for (long long blk = p0 >> 6; blk <= (p0 + 63) >> 6; ++blk) {
+    const long long base = blk * BLK;
+    const int lo = int(max(p0 - base, 0ll)), hi = int(min(min(p0 + 64, from + n) - base, (long long)BLK));      // of the block's tokens
+    const int live = blk < 0 ? 0 : int(min(max(total - base, 0ll), (long long)BLK));
+    auto write = [&](int t, float4 k, float4 v) {
+      if (t < lo || t >= hi) return;
+      if (t >= live) k = v = make_float4(0.f, 0.f, 0.f, 0.f);
+      const long long at = (out0 + base + t) * D + me.dim;
+      *reinterpret_cast<float4*>(ko + at) = k;
+      *reinterpret_cast<float4*>(vo + at) = v;
+    };
+    if (live == BLK) {
+      const uint8_t* record = c.records + ((long long)bh * c.blocks + blk) * record_bytes(D);
+      uint4 v[4];
+      uint32_t k[BLK / 4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (!reaches || lo + j > closed || (lo + j) * (long long)BLK >= total) continue;
-    if (lo + j < closed) {
-      const uint8_t* vc = record0 + j * record_bytes(D) + kCacheHead + BLK * D;
-      for (int i = threadIdx.x; i < D * BLK / 16; i += 256) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vc + i * 16);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(&codes_sm[j][i / 4 * PITCH + i % 4 * 16]);
-        dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(record + kCacheHead + BLK * D + (me.dim + j) * BLK + me.a * 16);
+#pragma unroll
+      for (int i = 0; i < BLK / 4; ++i) k[i] = *reinterpret_cast<const uint32_t*>(record + kCacheHead + (i / 4 * 16 + me.token(i)) * D + me.dim);
+      const float2 sc = *reinterpret_cast<const float2*>(record);
+#pragma unroll
+      for (int i = 0; i < BLK / 4; ++i) {
+        const int x = i & 3;
+        auto word = [&](const uint4& w) { return i < 4 ? w.x : i < 8 ? w.y : i < 12 ? w.z : w.w; };
+        write(i / 4 * 16 + me.token(i), make_float4(decode(k[i], 0) * sc.x, decode(k[i], 1) * sc.x, decode(k[i], 2) * sc.x, decode(k[i], 3) * sc.x),
+              make_float4(decode(word(v[0]), x) * sc.y, decode(word(v[1]), x) * sc.y, decode(word(v[2]), x) * sc.y, decode(word(v[3]), x) * sc.y));
+      }
+    } else if (live > 0) {
+      const T* tail = static_cast<const T*>(c.tail) + ((long long)bh * 2 + (closed & 1)) * 2 * BLK * D;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        Vec8T<T> v[4];
+        uint2 k[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j].q = *reinterpret_cast<const uint4*>(tail + BLK * D + (half * D + me.dim + j) * (BLK / 2) + me.a * 8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = *reinterpret_cast<const uint2*>(tail + (half * 32 + i / 4 * 16 + me.token(i)) * D + me.dim);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 k01 = unpack2<T>(k[i].x), k23 = unpack2<T>(k[i].y);
+          write(half * 32 + i / 4 * 16 + me.token(i), make_float4(k01.x, k01.y, k23.x, k23.y),
+                make_float4(to_f(v[0].v[i]), to_f(v[1].v[i]), to_f(v[2].v[i]), to_f(v[3].v[i])));
+        }
       }
     } else {
-      for (int i = threadIdx.x; i < D * BLK / 8; i += 256) {
-        const uint4 w = *reinterpret_cast<const uint4*>(tail + BLK * D + i * 8);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(&tail_sm[i / 4 * HALF_PITCH + i % 4 * 8]);
-        dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
-      }
+#pragma unroll 4
+      for (int i = 0; i < BLK / 4; ++i) write(i / 4 * 16 + me.token(i), make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f));
     }
-  }
-  __syncthreads();
-  constexpr int VEC = D / 4;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < 64 * VEC; i += 256) {
-    const int tok = i / VEC, d = i % VEC * 4, at_out = chunk * 64 + tok;
-    if (at_out >= n) break;
-    const long long p = p0 + tok;
-    float kf[4], vf[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) kf[j] = vf[j] = 0.f;
-    if (p >= 0 && p < total) {
-      const int blk = int(p / BLK), at = int(p % BLK);
-      if (blk < closed) {
-        const uint8_t* record = record0 + (blk - lo) * record_bytes(D);
-        const float2 sc = *reinterpret_cast<const float2*>(record);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(record + kCacheHead + at * D + d);
-        const uint8_t* vs = &codes_sm[blk - lo][d * PITCH + cache_slot(at)];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          kf[j] = float(int((w >> (8 * j)) & 0xFFu) - 128) * sc.x;
-          vf[j] = float(int(vs[j * PITCH]) - 128) * sc.y;
-        }
-      } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(tail + at * D + d);
-        const T* ks = reinterpret_cast<const T*>(&w);
-        const T* vs = tail_sm + ((at >> 5) * D + d) * HALF_PITCH + tail_slot(0, 0, at & 31);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { kf[j] = to_f(ks[j]); vf[j] = to_f(vs[j * HALF_PITCH]); }
-      }
-    }
-    const long long at_d = ((long long)bh * n + at_out) * D + d;
-    *reinterpret_cast<float4*>(ko + at_d) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-    *reinterpret_cast<float4*>(vo + at_d) = make_float4(vf[0], vf[1], vf[2], vf[3]);
   }
 }
 
@@ -366,7 +371,7 @@ cudaError_t read_typed(const CacheView& c, const int* first, int n, float* k, fl
   const long long ctas = (long long)c.B * c.Hkv * chunks;
   if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   ++g_launch_count;
-  return launch_chained(kv_read_kernel<T, D>, dim3(unsigned(ctas)), 256, 0, 0, stream, c, first, n, k, v, chunks);
+  return launch_chained(kv_read_kernel<T, D>, dim3(unsigned(ctas)), D, 0, 0, stream, c, first, n, k, v, chunks);
 }
 
 }  // namespace
