@@ -4,18 +4,17 @@
 //
 // One pass over the cache with a running maximum and sum.  Keys and values are read once per tile of query rows (the heads that
 // share a K/V head, times the new tokens of the step).  Every warp has a ring of blocks of its own in shared memory, which bulk
-// copies fill (one for the keys of a block with its scales, one for its values), so the warps run without barriers and each
-// keeps 8 to 16 KB of the cache in flight.  A lane's 16 adjacent bytes are its K or V fragment of several steps (the V rows are
+// copies fill (one for the keys of a block with its scales, one for its values; two each at D = 128), so the warps run without barriers
+// and each keeps 8 to 16 KB of the cache in flight.  A lane's 16 adjacent bytes are its K or V fragment of several steps (the V rows are
 // stored in that order); 4 bytes become two fp16 pairs in four instructions; both products run on m16n8k16 with the tokens (K) or
 // the head's dims (V) as rows and eight query rows as columns.  The (sequence, head, row tile, block) units of
 // the whole batch are one list, cut into equal parts for the warps that fit on the machine: sequences of unlike lengths, and a
 // single long one, keep every SM busy, and a warp streams across the ends of sequences.  A second kernel joins the parts of
 // the (sequence, head, row tile) items that were cut.
 // What bounds it: reading the codes, 2 D bytes per token and K/V head.  Measured on the GPU (replayed graph, caches flushed), one new
-// token: 64 ragged sequences of up to 2,048 tokens, 12 heads of 64, 25.1 us (101 MB, 4.0 TB/s); one of 131,071 tokens, 16 heads
-// on 4 of 64, 21.4 us (67 MB, 3.1 TB/s); eight ragged ones of up to 32,768, 32 heads on 8 of 128, 62 us (269 MB, 4.3 TB/s).  The first two have
-// some 7 us of launch, counting and joining besides the stream; in the third a warp waits for its copies and converts codes in turn,
-// and twelve warps an SM (what 64 KB of codes in flight and the accumulators of 128 dims leave) overlap the two only in part.
+// token: 64 ragged sequences of up to 2,048 tokens, 12 heads of 64, 24.7 us (101 MB, 4.1 TB/s); one of 131,071 tokens, 16 heads
+// on 4 of 64, 20.9 us (67 MB, 3.2 TB/s); eight ragged ones of up to 32,768, 32 heads on 8 of 128, 54.3 us (269 MB, 4.9 TB/s).  The first
+// two have some 7 us of launch, counting and joining besides the stream.
 //
 // Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
 // queries keep their eight bits in fp16.  Probabilities are rounded to fp16 (2^-11 of each, at a scale of 2^14 so that the
@@ -100,8 +99,11 @@ __device__ __forceinline__ void count_units(const Params& p, int* prefix, int* s
   }
 }
 
-// A stage of a warp's ring: the head of a record (its scales), keys, values, and the query rows of an item that begins.  The codes are
-// 16 KB a warp at any head dimension.
+// A stage of a warp's ring: the head of a record (its scales), keys, values, and the query rows of an item that begins.  Keys and values
+// come in pieces of 4 KB (2 KB at D = 32), each with a barrier of its own, so that a piece is asked for again as soon as it is read:
+// at D = 128, where they are two pieces each, three are on their way while one is worked on (54.3 against 62.0 us with one piece
+// each for eight ragged sequences of up to 32,768, 32 heads on 8).  Pieces of 2 KB at D = 64 cost more instructions than they hide.
+__host__ __device__ constexpr int pieces(int D) { return D < 128 ? 1 : 2; }
 __host__ __device__ constexpr int ring_stages(int D) { return D < 64 ? 2 : 1; }
 __host__ __device__ constexpr int stage_bytes(int D, int NQ) { return record_bytes(D) + 8 * NQ * D * 2; }
 __host__ __device__ constexpr int shared_bytes(int D, int NQ) {
@@ -266,7 +268,8 @@ cached_attention_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];          // rings (afterwards the exchange of the outputs), prefix
   __shared__ float ml_sm[kWarps][ROWS][2];
   __shared__ int scratch[kWarps];
-  __shared__ uint64_t bars[kWarps][STAGES][2];             // keys, values of a stage
+  constexpr int SPLIT = pieces(D), PIECE = BLK * D / SPLIT;
+  __shared__ uint64_t bars[kWarps][STAGES][2 * SPLIT];     // the pieces of a stage: keys, then values
   int* prefix = reinterpret_cast<int*>(smem + shared_bytes(D, NQ));
   float* o_sm = reinterpret_cast<float*>(smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -320,28 +323,34 @@ cached_attention_kernel(const Params p) {
     // that do not exist are copied with the rest and not used.
     if (lane == 0) {
 #pragma unroll
-      for (int t = 0; t < STAGES; ++t) { mbar_init(&bars[warp][t][0], 1); mbar_init(&bars[warp][t][1], 1); }
+      for (int t = 0; t < STAGES; ++t)
+#pragma unroll
+        for (int i = 0; i < 2 * SPLIT; ++i) mbar_init(&bars[warp][t][i], 1);
       mbar_fence_init();
     }
     __syncwarp();
     Cursor ahead = cur;
     int u_ahead = u0;
-    auto tail_of = [&](const Cursor& k) {
-      return static_cast<const uint8_t*>(p.tail) + (((long long)k.b * p.Hkv + k.h) * 2 + (k.closed & 1)) * (4 * BLK * D) + (k.at - k.closed) * (BLK * D);
+    const uint8_t* src;                  // of the unit ahead: its keys; its values are values_at bytes behind them
+    bool finished;
+    auto locate = [&]() {
+      const long long bh = (long long)ahead.b * p.Hkv + ahead.h;
+      finished = ahead.at < ahead.closed;
+      src = finished ? p.records + (bh * p.blocks + ahead.at) * record_bytes(D) + kCacheHead
+                     : static_cast<const uint8_t*>(p.tail) + (bh * 2 + (ahead.closed & 1)) * (4 * BLK * D) + (ahead.at - ahead.closed) * (BLK * D);
     };
-    auto copy_k = [&](int stage) {
-      __syncwarp();                      // every lane has read what the copies overwrite
+    locate();
+    // piece i of the unit ahead; behind the last one the cursor moves on
+    auto copy = [&](int stage, int i) {
+      __syncwarp();                      // every lane has read what the copy overwrites
       if (u_ahead < u1) {
         uint8_t* dst = ring + stage * STAGE;
-        uint64_t* bar = &bars[warp][stage][0];
-        const bool begins = u_ahead == u0 || ahead.at == 0, finished = ahead.at < ahead.closed;
+        uint64_t* bar = &bars[warp][stage][i];
+        const bool begins = i == 0 && (u_ahead == u0 || ahead.at == 0);
+        const int head = i == 0 && finished ? kCacheHead : 0;
         if (lane == 0) {
-          mbar_expect_tx(bar, BLK * D + (finished ? kCacheHead : 0) + (begins ? ROWS * D * 2 : 0));
-          if (finished) {
-            bulk_copy(dst, p.records + (((long long)ahead.b * p.Hkv + ahead.h) * p.blocks + ahead.at) * record_bytes(D), kCacheHead + BLK * D, bar);
-          } else {
-            bulk_copy(dst + KEYS, tail_of(ahead), BLK * D, bar);
-          }
+          mbar_expect_tx(bar, PIECE + head + (begins ? ROWS * D * 2 : 0));
+          bulk_copy(dst + KEYS + i * PIECE - head, src + (i >= SPLIT && !finished ? BLK * D : 0) + i * PIECE - head, PIECE + head, bar);
         }
         if (begins) {
           __syncwarp();                  // the bytes are expected before any arrive
@@ -351,21 +360,13 @@ cached_attention_kernel(const Params p) {
             bulk_copy(dst + QUERIES + lane * (D * 2), static_cast<const T*>(p.q) + ahead.b * p.sb + head * p.sh + t * p.st, D * 2, bar);
           }
         }
-      }
-    };
-    auto copy_v = [&](int stage) {       // then the cursor moves on
-      __syncwarp();
-      if (u_ahead < u1) {
-        if (lane == 0) {
-          uint64_t* bar = &bars[warp][stage][1];
-          mbar_expect_tx(bar, BLK * D);
-          const uint8_t* src = ahead.at < ahead.closed
-                                   ? p.records + (((long long)ahead.b * p.Hkv + ahead.h) * p.blocks + ahead.at) * record_bytes(D) + kCacheHead + BLK * D
-                                   : tail_of(ahead) + 2 * BLK * D;
-          bulk_copy(ring + stage * STAGE + VALUES, src, BLK * D, bar);
+        if (i == 2 * SPLIT - 1) {
+          ++u_ahead;
+          if (u_ahead < u1) {
+            ahead.next(p);
+            locate();
+          }
         }
-        ++u_ahead;
-        if (u_ahead < u1) ahead.next(p);
       }
     };
     bool lost = false;                   // a copy did not come in time: the rest is not waited for, the host sees the status
@@ -376,7 +377,9 @@ cached_attention_kernel(const Params p) {
       }
     };
 #pragma unroll
-    for (int t = 0; t < STAGES; ++t) { copy_k(t); copy_v(t); }
+    for (int t = 0; t < STAGES; ++t)
+#pragma unroll
+      for (int i = 0; i < 2 * SPLIT; ++i) copy(t, i);
 
     uint32_t qf[NQ][KW][2];              // fp16 query fragments, scaled: column g of every tile, dims 4 KW c ... of the head
     float qscale[NQ][2];                 // log2(e) / sqrt(D) times the power of two taken out, for the columns 2c, 2c + 1
@@ -428,6 +431,7 @@ cached_attention_kernel(const Params p) {
         float s[4][NQ][4];
 #pragma unroll
         for (int m0 = 0; m0 < 4; m0 += 2) {                  // two token tiles at a time: two chains of products
+          if (SPLIT == 2 && m0 == 2) arrive(stage, 1, parity);
           uint32_t kr[2][2][KW];
 #pragma unroll
           for (int m = 0; m < 2; ++m)
@@ -446,8 +450,8 @@ cached_attention_kernel(const Params p) {
                 else mma_f16(s[m0 + m][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
               }
             }
+          if (SPLIT == 2 || m0 == 2) copy(stage, m0 / 2 * (SPLIT - 1));
         }
-        copy_k(stage);
         float f[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -484,9 +488,10 @@ cached_attention_kernel(const Params p) {
           st.l[n][0] += sum[0];
           st.l[n][1] += sum[1];
         }
-        arrive(stage, 1, parity);
+        arrive(stage, SPLIT, parity);
 #pragma unroll
         for (int d0 = 0; d0 < DT; d0 += 2) {
+          if (SPLIT == 2 && d0 == DT / 2) arrive(stage, 3, parity);
           uint32_t vr[2][2][4];
 #pragma unroll
           for (int d = 0; d < 2; ++d)
@@ -513,11 +518,13 @@ cached_attention_kernel(const Params p) {
 #pragma unroll
               for (int i = 0; i < 4; ++i)  // a block that a row does not see at all must not reach it through its scale
                 if (!masked || base <= limit[n][i & 1]) st.o[n][d0 + d][i] = fmaf(acc[d][n][i], sc.y, st.o[n][d0 + d][i]);
+          if (SPLIT == 2 && d0 + 2 == DT / 2) copy(stage, 2);
         }
-        copy_v(stage);
+        copy(stage, 2 * SPLIT - 1);
       } else {                             // ---- half of the unfinished block, in the activation type ----
         const int base = cur.closed * BLK + (cur.at - cur.closed) * 32;
         const int valid = start + fresh - base;              // tokens that exist
+        if (SPLIT == 2) arrive(stage, 1, parity);
         float s[2][NQ][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -545,12 +552,14 @@ cached_attention_kernel(const Params p) {
             }
           }
         }
-        copy_k(stage);
+#pragma unroll
+        for (int i = 0; i < SPLIT; ++i) copy(stage, i);
         float one[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) one[n][0] = one[n][1] = 1.f;
         update_max<D, NQ, 2>(st, s, one);
-        arrive(stage, 1, parity);
+#pragma unroll
+        for (int i = SPLIT; i < 2 * SPLIT; ++i) arrive(stage, i, parity);
         uint32_t ph[2][NQ][2], pl[2][NQ][2], keep[2][2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -599,7 +608,8 @@ cached_attention_kernel(const Params p) {
             }
           }
         }
-        copy_v(stage);
+#pragma unroll
+        for (int i = SPLIT; i < 2 * SPLIT; ++i) copy(stage, i);
       }
       if (++stage == STAGES) { stage = 0; parity ^= 1; }
 
