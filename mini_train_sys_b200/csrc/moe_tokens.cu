@@ -16,8 +16,8 @@
 //      a CTA has of a row tile is added in shared memory, and where a tile was cut its last CTA adds the parts, in order.
 //
 // Measured on the GPU (replayed graph, caches flushed): one token, 2 of 8 experts of 768 x 1,024, 12.4 us (9.4 MB of weights: two launches'
-// latency); 64 tokens of the same 30.5 us (38 MB); 17 tokens, 8 of 64 experts of 2,048 x 1,024, 146 us (58 of them asked for, 0.72 GB,
-// 5.0 TB/s, the routing kernel's 11 us included); 8 tokens, 2 of 8 experts of 4,096 x 14,336, 410 us (2.5 GB, 6.2 TB/s).
+// latency); 64 tokens of the same 30.5 us (38 MB); 17 tokens, 8 of 64 experts of 2,048 x 1,024, 134 us (58 of them asked for, 0.72 GB,
+// 5.4 TB/s, the routing kernel's 11 us included); 8 tokens, 2 of 8 experts of 4,096 x 14,336, 383 us (2.5 GB, 6.6 TB/s).
 //
 // Rounding: logits, softmax, sums and the hidden values are fp32 (the router's fp32 weight enters the tensor cores as the sum of three
 // bf16 values, 24 bits); a hidden value enters the second product as the sum of two (2^-16), so y is rounded to bf16 once.
@@ -569,11 +569,17 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
 
   const int tiles = (p.I + kUpRows - 1) / kUpRows, steps = (p.H + kUpCols - 1) / kUpCols;
   const int N = r.entries * tiles;
-  const Parts parts(N, gridDim.x);
-  const int c0 = parts.begin(blockIdx.x), c1 = parts.begin(blockIdx.x + 1);
-  const Parts shares(c1 - c0, p.up_warps);
-  const int i0 = c0 + shares.begin(min(warp, p.up_warps)), i1 = c0 + shares.begin(min(warp + 1, p.up_warps));
-  int left = (i1 - i0) * steps, ahead_step = 0, ahead_expert = i0 / tiles, ahead_tile = i0 % tiles;
+  // Items in turn over all warps of the machine, the CTAs first: every SM reads from all over the weights.  With one stretch of them
+  // for each CTA the slowest SM took a quarter longer than the mean (58 experts of 2,048 x 1,024: 146 against 134 us for the layer;
+  // 8 of 4,096 x 14,336: 420 against 383).
+  const int stride = int(gridDim.x) * p.up_warps, i0 = warp < p.up_warps ? warp * int(gridDim.x) + int(blockIdx.x) : N;
+  const int count = i0 < N ? (N - 1 - i0) / stride + 1 : 0, by_expert = stride / tiles, by_tile = stride % tiles;
+  auto advance = [&](int& expert, int& tile) {
+    expert += by_expert;
+    tile += by_tile;
+    if (tile >= tiles) { tile -= tiles; ++expert; }
+  };
+  int left = count * steps, ahead_step = 0, ahead_expert = i0 / tiles, ahead_tile = i0 % tiles;
   int expert = ahead_expert, tile_at = ahead_tile;
   auto next_copy = [&]() {
     if (left == 0) return;
@@ -581,7 +587,7 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     ring.copy(&weights, ahead_step * kUpCols, ahead_tile * kUpRows, 2 * r.entry_expert[ahead_expert]);
     if (++ahead_step == steps) {
       ahead_step = 0;
-      if (++ahead_tile == tiles) { ahead_tile = 0; ++ahead_expert; }
+      advance(ahead_expert, ahead_tile);
     }
   };
 #pragma unroll 1
@@ -610,9 +616,9 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     }
   };
 #pragma unroll 1
-  for (int items = i1 - i0; items > 0; --items) {
+  for (int items = count; items > 0; --items) {
     const int row = tile_at * kUpRows + g, n0 = r.entry_begin[expert], n = r.entry_tokens[expert];
-    if (++tile_at == tiles) { tile_at = 0; ++expert; }
+    advance(expert, tile_at);
     const __nv_bfloat16* rows[kColumns / 8];
 #pragma unroll
     for (int j = 0; j < kColumns / 8; ++j) rows[j] = p.x + (long long)r.token[n0 + min(j * 8 + g, n - 1)] * p.ldx + c * 8;
