@@ -112,8 +112,9 @@ class DecodeSession:
         if any(m._forward_hooks or m._forward_pre_hooks for m in self._modules):
             self.model.check_decodable()
         self.cache.replayed(1)
-        self._ids.copy_(token_ids)
-        self._graph.replay()
+        with torch.cuda.device(self.cache.device):             # on that device's current stream, behind the copy
+            self._ids.copy_(token_ids)
+            self._graph.replay()
         return self._logits
 
     def _eager_step(self, token_ids: torch.Tensor) -> torch.Tensor:
