@@ -725,6 +725,33 @@ cached_attention_kernel(const Params p) {
 
 // (This kernel does not let the next one start early: CTAs of another attention that fill the SMs would hold the room of those
 // that have yet to join, 24.8 against 31.7 us for 64 ragged sequences.)
+// The parts of an item [begin, end): its candidates are the warps of the first and of the last CTA, and one part of every CTA
+// between (those lie within the item).
+struct ItemParts {
+  const Parts parts;
+  int begin, end, i0, i1, between, candidates;
+  __device__ __forceinline__ ItemParts(const Parts& all, int first, int units) : parts(all), begin(first), end(first + units) {
+    i0 = parts.owner(begin);
+    i1 = parts.owner(end - 1);
+    between = max(i1 - i0 - 1, 0);
+    candidates = kWarps + (i1 > i0 ? between + kWarps : 0);
+  }
+  // where candidate k is, -1 where it has nothing of the item; `whole`: it has all of it, and its owner has written the output
+  __device__ __forceinline__ int at(int k, bool& whole) const {
+    const int i = k < kWarps ? i0 : k < kWarps + between ? i0 + 1 + k - kWarps : i1;
+    const int w = k < kWarps ? k : k < kWarps + between ? 0 : k - kWarps - between;
+    const int c0 = parts.begin(i), c1 = parts.begin(i + 1);
+    if (c0 >= begin && c1 <= end) {                        // within the item: its warps are one part
+      whole |= c0 == begin && c1 == end;
+      return w == 0 && c0 < c1 ? 2 * i * kWarps : -1;
+    }
+    const int x0 = c0 + part_begin<kWarps>(c1 - c0, w), x1 = c0 + part_begin<kWarps>(c1 - c0, w + 1);
+    if (x0 >= end || x1 <= begin || x0 >= x1) return -1;
+    whole |= x0 <= begin && x1 >= end;
+    return 2 * (i * kWarps + w) + (x0 <= begin ? 1 : 0);
+  }
+};
+
 // Joins the parts of one row, a CTA a row, and zeroes the rows of padding; rows of items that were not cut are there already.
 // The weight of every part first, then the eight warps add the outputs of every eighth part, and the eight sums in order.
 constexpr int kJoinThreads = 256;
@@ -753,30 +780,15 @@ join_parts_kernel(const Params p, int rows_per_tile) {
   }
   count_units<kJoinThreads>(p, prefix, scratch);
   const Parts parts(prefix[p.B], p.ctas);
-  const int begin = prefix[b] + (h * p.row_tiles + row / rows_per_tile) * units_of(span), end = begin + units_of(span);
-  const int i0 = parts.owner(begin), i1 = parts.owner(end - 1);
-  // candidates: the warps of the first and of the last CTA, and one part of every CTA between (those lie within the item)
-  const int between = max(i1 - i0 - 1, 0), candidates = kWarps + (i1 > i0 ? between + kWarps : 0);
+  const ItemParts item(parts, prefix[b] + (h * p.row_tiles + row / rows_per_tile) * units_of(span), units_of(span));
+  const int candidates = item.candidates;
   wait_for_previous();                   // everything above read only what the kernel before this one does not write
   bool whole = false;
   float m = -CUDART_INF_F;
   const float* src = p.part + (long long)(row % rows_per_tile) * (D + 2);
   const long long pitch = (long long)rows_per_tile * (D + 2);
   for (int k = threadIdx.x; k < candidates; k += kJoinThreads) {
-    const int i = k < kWarps ? i0 : k < kWarps + between ? i0 + 1 + k - kWarps : i1;
-    const int w = k < kWarps ? k : k < kWarps + between ? 0 : k - kWarps - between;
-    const int c0 = parts.begin(i), c1 = parts.begin(i + 1);
-    int at = -1;
-    if (c0 >= begin && c1 <= end) {                        // within the item: its warps are one part
-      if (w == 0 && c0 < c1) at = 2 * i * kWarps;
-      whole |= c0 == begin && c1 == end;
-    } else {
-      const int x0 = c0 + part_begin<kWarps>(c1 - c0, w), x1 = c0 + part_begin<kWarps>(c1 - c0, w + 1);
-      if (x0 < end && x1 > begin && x0 < x1) {
-        at = 2 * (i * kWarps + w) + (x0 <= begin ? 1 : 0);
-        whole |= x0 <= begin && x1 >= end;
-      }
-    }
+    const int at = item.at(k, whole);
     slot[k] = at;
     if (at >= 0) m = fmaxf(m, src[at * pitch + D]);
   }
@@ -820,6 +832,75 @@ join_parts_kernel(const Params p, int rows_per_tile) {
     for (int w = 0; w < kJoinThreads / 32; ++w) { sum += o_sm[w][d]; total += red[w]; }
     out[d] = Act<T>::from(sum / total);
   }
+}
+
+// The same, a warp a row: the candidates are gone through 32 at a time with a running maximum and sum.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+join_rows_kernel(const Params p, int rows_per_tile, int total_rows) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* prefix = reinterpret_cast<int*>(smem);              // [B + 1]
+  __shared__ int scratch[kJoinThreads / 32];
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31, rows = p.group * p.T;
+  count_units<kJoinThreads>(p, prefix, scratch);
+  const int at_row = int(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  wait_for_previous();                   // everything above read only what the kernel before this one does not write
+  if (at_row >= total_rows) return;
+  const int row = at_row % rows, bh = at_row / rows, h = bh % p.Hkv, b = bh / p.Hkv;
+  const int t = row / p.group, head = h * p.group + row % p.group;
+  T* out = static_cast<T*>(p.o) + (((long long)b * p.T + t) * p.Hq + head) * D;
+  const int2 span = span_of(p, b);
+  if (t >= span.y) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) out[j * 32 + lane] = Act<T>::from(0.f);
+    return;
+  }
+  const ItemParts item(Parts(prefix[p.B], p.ctas), prefix[b] + (h * p.row_tiles + row / rows_per_tile) * units_of(span), units_of(span));
+  const float* src = p.part + (long long)(row % rows_per_tile) * (D + 2);
+  const long long pitch = (long long)rows_per_tile * (D + 2);
+  float m = -CUDART_INF_F, l = 0.f, o[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) o[j] = 0.f;
+  for (int k0 = 0; k0 < item.candidates; k0 += 32) {
+    bool whole = false;
+    const int at = k0 + lane < item.candidates ? item.at(k0 + lane, whole) : -1;
+    if (__any_sync(0xffffffffu, whole)) return;
+    const float part_m = at >= 0 ? src[at * pitch + D] : -CUDART_INF_F, part_l = at >= 0 ? src[at * pitch + D + 1] : 0.f;
+    float most = fmaxf(part_m, m);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    const float base = most == -CUDART_INF_F ? 0.f : most, before = exp2f(m - base);
+    const float weight = at >= 0 ? exp2f(part_m - base) : 0.f;
+    m = most;
+    l *= before;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[j] *= before;
+    float sum = part_l * weight;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    l += sum;
+    unsigned left = __ballot_sync(0xffffffffu, at >= 0);   // the parts, in order, eight loads at a time
+    while (left != 0) {
+      float v[8][PER], a[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = left != 0 ? __ffs(int(left)) - 1 : 0;
+        a[i] = __shfl_sync(0xffffffffu, weight, from);
+        const int slot = __shfl_sync(0xffffffffu, at, from);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[i][j] = left != 0 ? src[slot * pitch + j * 32 + lane] : 0.f;
+        if (left == 0) a[i] = 0.f;
+        left &= left - 1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) o[j] = fmaf(v[i][j], a[i], o[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) out[j * 32 + lane] = Act<T>::from(o[j] / l);
 }
 
 struct Plan {
@@ -886,6 +967,11 @@ cudaError_t launch_typed(const Params& p, int cluster, cudaStream_t stream) {
   err = launch_chained(cached_attention_kernel<T, D, NQ, false>, dim3(unsigned(p.ctas)), kWarps * 32, size_t(bytes) + (p.B + 1) * 4, 0, stream, p);
   if (err != cudaSuccess) return err;
   ++g_launch_count;
+  // A CTA a row is the shorter chain (64 sequences, 768 rows: 24.8 us, with a warp a row 27.6) as long as all are resident at once; 4,480
+  // rows (14 sequences, 10 new tokens, 32 heads on 8 of 32) take 33.1 us in all with a CTA a row and 24.3 with a warp a row.
+  if (rows > (2048 / kJoinThreads) * (long long)device_sm_count())
+    return launch_chained(join_rows_kernel<T, D>, dim3(unsigned((rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32))), kJoinThreads, size_t(p.B + 1) * 4, 0, stream,
+                          p, 8 * NQ, int(rows));
   return launch_chained(join_parts_kernel<T, D>, dim3(unsigned(rows)), kJoinThreads, size_t(p.B + 1 + 2 * (p.ctas + 2 * kWarps)) * 4, 0, stream, p, 8 * NQ);
 }
 

@@ -160,6 +160,21 @@ def test_cached_attention_over_lengths_and_capacities(ops, capacity, length):
     assert_attention(ops.cached_attention(q, cache, 0), q, k, v, [length], [1])
 
 
+@pytest.mark.parametrize("counted", [[0] * 63 + [1], [1] + [0] * 62 + [1], [1] * 64])
+def test_cached_attention_of_many_rows(ops, counted):
+    """More rows than are joined at once, of sequences that are cut into many parts or into few."""
+
+    lengths = [9000 if n else 0 for n in counted] if sum(counted) < 64 else [17 * b for b in range(64)]
+    k, v = rows(64, 2, max(lengths) + 1, 32, 11), rows(64, 2, max(lengths) + 1, 32, 12, spread=False)
+    q = rows(64, 24, 1, 32, 13, spread=False)
+    cache = QuantizedKVCache(layers=1, batch=64, kv_heads=2, head_dim=32, capacity=9001, device=DEV)
+    fill(ops, cache, 0, k, v, lengths)
+    cache.begin(torch.tensor(counted, dtype=torch.int32, device=DEV))
+    fresh = [torch.stack([x[b, :, n:n + 1] for b, n in enumerate(lengths)]) for x in (k, v)]
+    ops.kv_append(cache, 0, *fresh)
+    assert_attention(ops.cached_attention(q, cache, 0), q, k, v, lengths, counted)
+
+
 def test_scores_far_apart_and_query_scales(ops):
     """One key takes all of the mass; queries that are tiny, huge or zero."""
 
