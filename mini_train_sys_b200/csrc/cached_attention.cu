@@ -14,7 +14,7 @@
 // What bounds it: reading the codes, 2 D bytes per token and K/V head.  Measured on the GPU (replayed graph, caches flushed), one new
 // token: 64 ragged sequences of up to 2,048 tokens, 12 heads of 64, 24.7 us (101 MB, 4.1 TB/s); one of 131,071 tokens, 16 heads
 // on 4 of 64, 20.9 us (67 MB, 3.2 TB/s); eight ragged ones of up to 32,768, 32 heads on 8 of 128, 54.3 us (269 MB, 4.9 TB/s).  The first
-// two have some 7 us of launch, counting and joining besides the stream.
+// two are short streams behind a launch and the counting of units, and before the join.
 //
 // Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
 // queries keep their eight bits in fp16.  Probabilities are rounded to fp16 (2^-11 of each, at a scale of 2^14 so that the
