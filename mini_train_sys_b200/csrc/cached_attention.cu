@@ -274,8 +274,9 @@ cached_attention_kernel(const Params p) {
   float* o_sm = reinterpret_cast<float*>(smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  let_next_start();
+  if (CLUSTER) let_next_start();
   wait_for_previous();
+  if (!CLUSTER) let_next_start();        // the joining kernel reads the lengths before it waits: whatever wrote them has ended by now
   Cursor cur;
   int c0, c1;                            // units of this CTA
   if constexpr (CLUSTER) {
@@ -782,7 +783,7 @@ join_parts_kernel(const Params p, int rows_per_tile) {
   const Parts parts(prefix[p.B], p.ctas);
   const ItemParts item(parts, prefix[b] + (h * p.row_tiles + row / rows_per_tile) * units_of(span), units_of(span));
   const int candidates = item.candidates;
-  wait_for_previous();                   // everything above read only what the kernel before this one does not write
+  wait_for_previous();                   // everything above read the lengths only, which were there when the kernel before this one began
   bool whole = false;
   float m = -CUDART_INF_F;
   const float* src = p.part + (long long)(row % rows_per_tile) * (D + 2);
@@ -845,7 +846,7 @@ join_rows_kernel(const Params p, int rows_per_tile, int total_rows) {
   const int lane = threadIdx.x & 31, rows = p.group * p.T;
   count_units<kJoinThreads>(p, prefix, scratch);
   const int at_row = int(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
-  wait_for_previous();                   // everything above read only what the kernel before this one does not write
+  wait_for_previous();                   // everything above read the lengths only, which were there when the kernel before this one began
   if (at_row >= total_rows) return;
   const int row = at_row % rows, bh = at_row / rows, h = bh % p.Hkv, b = bh / p.Hkv;
   const int t = row / p.group, head = h * p.group + row % p.group;

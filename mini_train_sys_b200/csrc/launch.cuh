@@ -1,6 +1,7 @@
 // Launches of the decoding kernels.  A decoding step is a chain of short kernels on one stream, so each is launched while the one
 // before it still runs (programmatic stream serialization): it lets the next one start at once and waits for the one before
-// before it touches memory.  Every thread waits, so that a kernel's end means the end of all before it.
+// before it touches memory (weights may be prefetched to L2 earlier; the kernel that joins attention reads lengths earlier, and is
+// let start only when they are there).  Every thread waits, so that a kernel's end means the end of all before it.
 #pragma once
 
 #include <cuda_runtime.h>
