@@ -71,6 +71,12 @@ class RMSNorm(nn.Module):
         return ops.rmsnorm(x, self.weight, self.eps), x
 
 
+def being_recorded(x: torch.Tensor) -> bool:
+    """Whether work on ``x`` goes into a CUDA graph: what Python decides now then holds for every replay."""
+
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class CausalSelfAttention(nn.Module):
     def __init__(self, cfg: ModelConfig) -> None:
         super().__init__()
@@ -105,12 +111,13 @@ class CausalSelfAttention(nn.Module):
         """One step of cached decoding: ``x`` [B, T, H] are the new tokens of the open step of ``cache``.
 
         A prompt (nothing cached yet) attends to itself with the exact keys and values and fills the cache; later steps append and
-        attend over the cache.  The tables are the full ones: positions come from the cache's lengths."""
+        attend over the cache, which is right at any length: so does a step that is recorded, since its replays find the cache at
+        other lengths.  The tables are the full ones: positions come from the cache's lengths."""
 
         b, s, h = x.shape
         fused = project(ops, self.qkv, x).view(b, s, 3, self.cfg.n_heads, self.cfg.head_dim)
         q, k, v = (fused[:, :, j].transpose(1, 2) for j in range(3))
-        if cache.held == 0:
+        if cache.held == 0 and not being_recorded(x):
             q, k = ops.rope(q, k, rope_cos[:s], rope_sin[:s])
             ops.kv_append(cache, layer, k, v)
             ctx = ops.attention(q, k, v, is_causal=True, dropout_p=0.0)

@@ -70,8 +70,8 @@ _CAPTURED_OPS = ("kv_append", "cached_attention", "moe_tokens", "fused_moe")
 class DecodeSession:
     """Cached decoding of one batch: ``prompt`` once, then ``step`` by step.
 
-    On a GPU with the native operators a step is captured into a CUDA graph after the first one and replayed: a step is some
-    hundred short kernels, whose launches take longer than their work.  Where the kernels do not cover the model (a head dimension
+    On a GPU with the native operators a step is captured into a CUDA graph after the first one over a filled cache and replayed: a
+    step is some hundred short kernels, whose launches take longer than their work.  ``cache.reset()`` starts anew.  Where the kernels do not cover the model (a head dimension
     other than 32, 64 and 128, ...) steps stay eager, or are refused with ``graph=True``.  Weights that change in place or move are
     noticed, and the step is captured again; a model whose parameters are replaced by others needs a new session."""
 
@@ -97,7 +97,7 @@ class DecodeSession:
 
         if token_ids.shape != (self.cache.batch, 1):
             raise ValueError(f"a step takes one token per sequence, got {tuple(token_ids.shape)}")
-        if not self.graph_wanted:
+        if not self.graph_wanted or self.cache.held == 0:          # nothing is cached: the form of a prompt, which no later step takes
             return self.model.decode(token_ids, self.cache)
         if self._graph is not None and self._weights() != self._captured:
             self._graph, self._prepared = None, False
