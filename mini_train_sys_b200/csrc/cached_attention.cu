@@ -63,8 +63,8 @@ struct Params {
 // Tokens of sequence b: before the step, and of it.
 __device__ __forceinline__ int2 span_of(const Params& p, int b) {
   const int capacity = p.blocks * BLK;
-  const int start = min(max(__ldg(p.start + b), 0), capacity);
-  return make_int2(start, min(min(max(__ldg(p.count + b), 0), p.T), capacity - start));
+  const int start = min(max(p.start[b], 0), capacity);
+  return make_int2(start, min(min(max(p.count[b], 0), p.T), capacity - start));
 }
 // Units of a (head, row tile) of it: the finished blocks, and the unfinished one in halves of 32 tokens, which are as many bytes.
 __device__ __forceinline__ int units_of(int2 span) {

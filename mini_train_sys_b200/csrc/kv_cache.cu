@@ -102,8 +102,8 @@ constexpr int kQPieces = 4;              // of 32 bytes of q, a thread
 // A thread owns eight dims of the lower half of a head and their partners in the upper half, for one token.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads, D == 128 ? 2 : 4)
-kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __restrict__ q_out, const T* __restrict__ cosv,
-                 const T* __restrict__ sinv, int table_rows, int Tn, int kv_ctas, int q_ctas, int blocks_per_head) {
+kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __restrict__ q_out, const T* cosv, const T* sinv,
+                 int table_rows, int Tn, int kv_ctas, int q_ctas, int blocks_per_head) {
   constexpr int VEC = D / 16;                              // threads per token
   constexpr int ITER = (kCacheBlock * VEC + kAppendThreads - 1) / kAppendThreads;
   constexpr int BLK = kCacheBlock;
@@ -289,7 +289,7 @@ __device__ __forceinline__ float decode(uint32_t w, int x) { return __uint_as_fl
 
 template <typename T, int D>
 __global__ void __launch_bounds__(D)
-kv_read_kernel(CacheView c, const int* __restrict__ first, int n, float* __restrict__ ko, float* __restrict__ vo, int chunks) {
+kv_read_kernel(CacheView c, const int* first, int n, float* __restrict__ ko, float* __restrict__ vo, int chunks) {
   constexpr int BLK = kCacheBlock;
   let_next_start();
   wait_for_previous();

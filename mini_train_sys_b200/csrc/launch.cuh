@@ -2,6 +2,8 @@
 // before it still runs (programmatic stream serialization): it lets the next one start at once and waits for the one before
 // before it touches memory (weights may be prefetched to L2 earlier; the kernel that joins attention reads lengths earlier, and is
 // let start only when they are there).  Every thread waits, so that a kernel's end means the end of all before it.
+// What a kernel before it may have written is read with ordinary loads: the read-only path (__ldg, or a __restrict__ pointer to const)
+// is for memory that nothing writes while the kernel lives, which begins before that wait, and its loads may be moved across the wait.
 #pragma once
 
 #include <cuda_runtime.h>

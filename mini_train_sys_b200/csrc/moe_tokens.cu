@@ -306,16 +306,16 @@ __device__ __forceinline__ void router_products(const Params& p, float* part, in
       const long long at = (long long)min(m + g + 8 * u, p.E - 1) * p.H + k;
       w[u][0] = w[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (in && p.router_bf16) {
-        w[u][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const __nv_bfloat16*>(p.router) + at));      // eight bf16 values
+        w[u][0] = *reinterpret_cast<const float4*>(static_cast<const __nv_bfloat16*>(p.router) + at);      // eight bf16 values
       } else if (in) {
-        w[u][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at));
-        w[u][1] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at) + 1);
+        w[u][0] = *reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at);
+        w[u][1] = reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at)[1];
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (j * 8 >= p.T) break;
-      b[j] = in ? __ldg(reinterpret_cast<const uint4*>(p.x + min(j * 8 + g, p.T - 1) * p.ldx + k)) : make_uint4(0, 0, 0, 0);
+      b[j] = in ? *reinterpret_cast<const uint4*>(p.x + min(j * 8 + g, p.T - 1) * p.ldx + k) : make_uint4(0, 0, 0, 0);
     }
   };
   int m = 0, q = worker;
@@ -385,16 +385,16 @@ __device__ __forceinline__ void router_few(const Params& p, float* logits) {
         if (d < p.H) {
           const long long at = (long long)e * p.H + d;
           if (p.router_bf16) {
-            w[i][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const __nv_bfloat16*>(p.router) + at));          // eight bf16 values
+            w[i][0] = *reinterpret_cast<const float4*>(static_cast<const __nv_bfloat16*>(p.router) + at);          // eight bf16 values
           } else {
-            w[i][0] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at));
-            w[i][1] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at) + 1);
+            w[i][0] = *reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at);
+            w[i][1] = reinterpret_cast<const float4*>(static_cast<const float*>(p.router) + at)[1];
           }
         }
 #pragma unroll
         for (int t = 0; t < kFewTokens; ++t) {
           x[i][t] = make_uint4(0, 0, 0, 0);
-          if (d < p.H && t < p.T) x[i][t] = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.ldx + d));
+          if (d < p.H && t < p.T) x[i][t] = *reinterpret_cast<const uint4*>(p.x + t * p.ldx + d);
         }
       }
 #pragma unroll
@@ -606,12 +606,12 @@ moe_up_kernel(const __grid_constant__ CUtensorMap weights, const Params p) {
     const __nv_bfloat16* src = row + step * kUpCols;
     if ((step + 1) * kUpCols <= p.H) {
 #pragma unroll
-      for (int s = 0; s < kUpCols / 32; ++s) b.v[s] = __ldg(reinterpret_cast<const uint4*>(src + 32 * s));
+      for (int s = 0; s < kUpCols / 32; ++s) b.v[s] = *reinterpret_cast<const uint4*>(src + 32 * s);
     } else {
 #pragma unroll
       for (int s = 0; s < kUpCols / 32; ++s) {
         b.v[s] = make_uint4(0, 0, 0, 0);
-        if (step * kUpCols + 32 * s + c * 8 < p.H) b.v[s] = __ldg(reinterpret_cast<const uint4*>(src + 32 * s));
+        if (step * kUpCols + 32 * s + c * 8 < p.H) b.v[s] = *reinterpret_cast<const uint4*>(src + 32 * s);
       }
     }
   };

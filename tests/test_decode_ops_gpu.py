@@ -365,6 +365,48 @@ def test_moe_tokens_on_two_streams_and_replayed(ops):
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("tokens,experts,hidden,inter", [(1, 8, 256, 128), (4, 8, 768, 1024), (12, 8, 768, 1024), (64, 64, 768, 256)])
+def test_operators_that_read_what_the_one_before_wrote(ops, tokens, experts, hidden, inter):
+    """Append, attention and two layers of experts in a row, each kernel started while the one before it runs: the same values as
+    with the device waited for between the calls, eagerly and replayed."""
+
+    heads = hidden // 64
+    x, r, gu, dn = moe_inputs(tokens, experts, hidden, inter, 17)
+    k, v = rows(tokens, heads, 150, 64, 18), rows(tokens, heads, 150, 64, 19, spread=False)
+    cos, sin = (t.to(DEV, torch.bfloat16) for t in rope_tables(64, 192, 10000.0))
+    cache = QuantizedKVCache(layers=1, batch=tokens, kv_heads=heads, head_dim=64, capacity=192, device=DEV)
+    fill(ops, cache, 0, k, v, [149 - 2 * (b % 60) for b in range(tokens)])
+    cache.begin()
+    fresh = [t[:, :, 149:] for t in (k, v)]
+
+    def chain(between):
+        out = []
+        q = x.view(tokens, 1, heads, 64).transpose(1, 2)
+        for _ in range(3):
+            out.append(ops.kv_append(cache, 0, *fresh, q=q, cos=cos, sin=sin))
+            between()
+            out.append(ops.cached_attention(out[-1], cache, 0))
+            between()
+            out.append(ops.moe_tokens(out[-1].transpose(1, 2).reshape(tokens, hidden), r, gu, dn, 2, normalize=True))
+            between()
+            out.append(ops.moe_tokens(out[-1], r, gu, dn, 2, normalize=False))
+            between()
+            q = out[-1].view(tokens, 1, heads, 64).transpose(1, 2)
+        return out
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(10):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(lambda: None)
+    for _ in range(10):
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_what_the_kernels_do_not_cover_takes_the_plain_path(ops):
     before = dict(ops.dispatch)
     cache = QuantizedKVCache(layers=1, batch=1, kv_heads=2, head_dim=48, capacity=128, device=DEV)
