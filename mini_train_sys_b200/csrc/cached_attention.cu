@@ -370,7 +370,7 @@ cached_attention_kernel(const Params p) {
         }
       }
     };
-    bool lost = false;                   // a copy did not come in time: the rest is not waited for, the host sees the status
+    bool lost = false;                   // a copy did not come in time: the rest is not waited for, and DecodeSession looks at the status
     auto arrive = [&](int stage, int which, uint32_t parity) {
       if (!lost && !wait_copy(&bars[warp][stage][which], parity)) {
         lost = true;

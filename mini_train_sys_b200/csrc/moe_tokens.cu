@@ -109,7 +109,7 @@ struct Ring {
   int stages, lane;
   int put = 0, get = 0;        // stage of the next copy, of the next tile
   uint32_t parity = 0;
-  bool lost = false;           // a copy did not come in time: the rest is not waited for, the host sees the status
+  bool lost = false;           // a copy did not come in time: the rest is not waited for, and DecodeSession looks at the status
 
   __device__ __forceinline__ void init() {
     if (lane == 0) {

@@ -42,13 +42,16 @@ def ext():
     return _ext
 
 
+def raise_status(word: int) -> None:
+    if word != 0:
+        raise RuntimeError(f"a native kernel reported status {word} (1 = wait timeout)")
+
+
 def check_kernel_status(device: torch.device | int | None = None) -> None:
     """Raise if any kernel on ``device`` reported a bounded-wait timeout (synchronises)."""
 
     index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
-    word = int(ext().status_tensor(index)[0].item())
-    if word != 0:
-        raise RuntimeError(f"a native kernel reported status {word} (1 = wait timeout)")
+    raise_status(int(ext().status_tensor(index)[0].item()))
 
 
 # ---------------------------------------------------------------------------------------------

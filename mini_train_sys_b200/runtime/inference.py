@@ -73,7 +73,11 @@ class DecodeSession:
     On a GPU with the native operators a step is captured into a CUDA graph after the first one over a filled cache and replayed: a
     step is some hundred short kernels, whose launches take longer than their work.  ``cache.reset()`` starts anew.  Where the kernels do not cover the model (a head dimension
     other than 32, 64 and 128, ...) steps stay eager, or are refused with ``graph=True``.  Weights that change in place or move are
-    noticed, and the step is captured again; a model whose parameters are replaced by others needs a new session."""
+    noticed, and the step is captured again; a model whose parameters are replaced by others needs a new session.
+
+    A native kernel that gives up on a wait computes on without what it waited for and raises its device's status word.  The word is
+    copied to the host behind every call, without waiting, and the next call raises RuntimeError if it was set; ``check()`` waits and
+    looks at once (``generate`` does so at its end)."""
 
     def __init__(self, model: MiniTransformer, batch: int, capacity: int | None = None, *, graph: bool | None = None) -> None:
         self.model = model
@@ -86,15 +90,56 @@ class DecodeSession:
         self._insisted = bool(graph)
         self._graph: torch.cuda.CUDAGraph | None = None
         self._prepared = False
+        self._status = self._status_word()
+        self._seen = None if self._status is None else torch.zeros_like(self._status, device="cpu", pin_memory=self._status.is_cuda)
+
+    def _status_word(self) -> torch.Tensor | None:
+        """Where the kernels of this session report, None where it runs none."""
+
+        if self.cache.device.type != "cuda" or getattr(self.model.ops, "name", "") != "native":
+            return None
+        from mini_train_sys_b200.ops.native_backend import ext
+
+        return ext().status_tensor(self.cache.device.index)
+
+    def _note_status(self) -> None:
+        if self._status is None or (self._status.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return
+        if self._status.is_cuda:
+            with torch.cuda.device(self._status.device):
+                self._seen.copy_(self._status, non_blocking=True)
+        else:
+            self._seen.copy_(self._status)
+
+    def _raise_noted(self) -> None:
+        if self._seen is not None and int(self._seen[0]) != 0:
+            self.check()
+
+    def check(self) -> None:
+        """Raise if a kernel of this session gave up on a wait (synchronises)."""
+
+        if self._status is not None:
+            from mini_train_sys_b200.ops.native_backend import raise_status
+
+            raise_status(int(self._status[0].item()))
 
     def prompt(self, input_ids: torch.Tensor, counts: torch.Tensor | None = None) -> torch.Tensor:
         """Logits [B, V] behind the prompts [B, T]; ``counts`` [B] are their lengths where they are padded on the right."""
 
-        return self.model.decode(input_ids, self.cache, counts)
+        self._raise_noted()
+        logits = self.model.decode(input_ids, self.cache, counts)
+        self._note_status()
+        return logits
 
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
         """Logits [B, V] behind one more token [B, 1] of every sequence.  They are overwritten by the next step."""
 
+        self._raise_noted()
+        logits = self._step(token_ids)
+        self._note_status()
+        return logits
+
+    def _step(self, token_ids: torch.Tensor) -> torch.Tensor:
         if token_ids.shape != (self.cache.batch, 1):
             raise ValueError(f"a step takes one token per sequence, got {tuple(token_ids.shape)}")
         if not self.graph_wanted or self.cache.held == 0:          # nothing is cached: the form of a prompt, which no later step takes
@@ -195,4 +240,5 @@ def generate(model: MiniTransformer, prompt_ids: torch.Tensor, *, max_new_tokens
         ids = torch.cat((ids, nxt), dim=1)
         if i + 1 < max_new_tokens:
             logits = session.step(nxt)
+    session.check()
     return ids

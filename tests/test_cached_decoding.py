@@ -173,6 +173,33 @@ def test_a_session_captures_no_step_of_an_empty_cache(monkeypatch):
     assert held == [1, 1]
 
 
+def test_a_reported_wait_is_raised(monkeypatch):
+    """With a status word set from the host: a session raises at the call behind the one that saw it, and at once when asked; so does
+    ``generate``, which asks at its end."""
+
+    model = make_model("moe")
+    ids = torch.randint(0, 97, (2, 5))
+    word = torch.zeros(4, dtype=torch.int32)
+    monkeypatch.setattr(DecodeSession, "_status_word", lambda self: word)
+    session = DecodeSession(model, 2)
+    session.prompt(ids)
+    session.step(ids[:, :1])
+    session.check()
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="status 1"):
+        session.check()
+    session.step(ids[:, :1])
+    for call in (lambda: session.step(ids[:, :1]), lambda: session.prompt(ids)):
+        with pytest.raises(RuntimeError, match="status 1"):
+            call()
+    for steps in (1, 2, 5):
+        with pytest.raises(RuntimeError, match="status 1"):
+            generate(model, ids, max_new_tokens=steps, kv_cache="int8")
+    word.zero_()
+    session.step(ids[:, :1])
+    assert generate(model, ids, max_new_tokens=2, kv_cache="int8").shape == (2, 7)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("ffn", ["dense", "moe"])
 def test_native_decoding_on_a_gpu(ffn):
@@ -271,6 +298,34 @@ def test_a_graph_recorded_on_an_empty_cache_is_right_at_every_length():
         # over keys that may differ by the rounding of that step: bf16 along the residual path, as against the plain pass
         assert (logits.float() - want).norm() <= 8 * 2 ** -8 * want.norm(), i
     assert cache.lengths.tolist() == [80, 80]
+
+
+@pytest.mark.gpu
+def test_a_reported_wait_is_raised_on_a_gpu():
+    from mini_train_sys_b200.ops.native_backend import ext
+
+    model = make_model("moe", ops="native", device="cuda", dtype=torch.bfloat16, hidden=256, seq_len=256)
+    ids = torch.randint(0, 97, (2, 10), device="cuda")
+    word = ext().status_tensor(0)
+    session = DecodeSession(model, 2, graph=True)
+    session.prompt(ids)
+    for _ in range(3):
+        session.step(ids[:, :1])
+    session.check()
+    word[0] = 1
+    try:
+        session.step(ids[:, :1])
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="status 1"):
+            session.step(ids[:, :1])
+        with pytest.raises(RuntimeError, match="status 1"):
+            session.check()
+        with pytest.raises(RuntimeError, match="status 1"):
+            generate(model, ids, max_new_tokens=4, kv_cache="int8")
+    finally:
+        word.zero_()
+    session.step(ids[:, :1])
+    assert generate(model, ids, max_new_tokens=4, kv_cache="int8").shape == (2, 14)
 
 
 @pytest.mark.gpu
