@@ -341,6 +341,9 @@ cached_attention_kernel(const Params p) {
                      : static_cast<const uint8_t*>(p.tail) + (bh * 2 + (ahead.closed & 1)) * (4 * BLK * D) + (ahead.at - ahead.closed) * (BLK * D);
     };
     locate();
+    // A copy did not come in time: the rest is neither asked for, since a barrier counts bytes to 2^20 only, nor waited for, and DecodeSession
+    // looks at the status.
+    bool lost = false;
     // piece i of the unit ahead; behind the last one the cursor moves on
     auto copy = [&](int stage, int i) {
       __syncwarp();                      // every lane has read what the copy overwrites
@@ -349,13 +352,13 @@ cached_attention_kernel(const Params p) {
         uint64_t* bar = &bars[warp][stage][i];
         const bool begins = i == 0 && (u_ahead == u0 || ahead.at == 0);
         const int head = i == 0 && finished ? kCacheHead : 0;
-        if (lane == 0) {
+        if (lane == 0 && !lost) {
           mbar_expect_tx(bar, PIECE + head + (begins ? ROWS * D * 2 : 0));
           bulk_copy(dst + KEYS + i * PIECE - head, src + (i >= SPLIT && !finished ? BLK * D : 0) + i * PIECE - head, PIECE + head, bar);
         }
         if (begins) {
           __syncwarp();                  // the bytes are expected before any arrive
-          if (lane < ROWS) {
+          if (lane < ROWS && !lost) {
             const int r = ahead.tile * ROWS + lane;
             const int t = r < rows ? r / p.group : 0, head = ahead.h * p.group + (r < rows ? r % p.group : 0);
             bulk_copy(dst + QUERIES + lane * (D * 2), static_cast<const T*>(p.q) + ahead.b * p.sb + head * p.sh + t * p.st, D * 2, bar);
@@ -370,7 +373,6 @@ cached_attention_kernel(const Params p) {
         }
       }
     };
-    bool lost = false;                   // a copy did not come in time: the rest is not waited for, and DecodeSession looks at the status
     auto arrive = [&](int stage, int which, uint32_t parity) {
       if (!lost && !wait_copy(&bars[warp][stage][which], parity)) {
         lost = true;

@@ -109,7 +109,9 @@ struct Ring {
   int stages, lane;
   int put = 0, get = 0;        // stage of the next copy, of the next tile
   uint32_t parity = 0;
-  bool lost = false;           // a copy did not come in time: the rest is not waited for, and DecodeSession looks at the status
+  // A copy did not come in time: the rest is neither asked for, since a barrier counts bytes to 2^20 only, nor waited for, and DecodeSession
+  // looks at the status.
+  bool lost = false;
 
   __device__ __forceinline__ void init() {
     if (lane == 0) {
@@ -119,7 +121,7 @@ struct Ring {
     __syncwarp();
   }
   __device__ __forceinline__ void copy(const CUtensorMap* map, int x, int y, int z) {
-    if (lane == 0) {
+    if (lane == 0 && !lost) {
       mbar_expect_tx(&bars[put], kTile);
       tma_load_3d(base + put * kTile, map, &bars[put], x, y, z);
     }
