@@ -39,7 +39,8 @@ struct Strided {         // [B, heads, T, D] view with a unit inner stride
   long long sb, sh, st;
 };
 
-// Appends token t < count[b] at position start[b] + t; keys and queries are rotated when `cosv` is given (tables [P, D]).
+// Appends token t < count[b] at position start[b] + t; keys and queries are rotated when `cosv` is given (tables [P, D], P > 0; a
+// position behind their end, which only a replayed graph can reach, takes the last row).
 // q_out: [B, Hq, T, D] over [B, T, Hq, D] storage; rows t >= count[b] are zeroed.  q.p may be null.
 cudaError_t launch_kv_append(const CacheView& c, const Strided& q, int Hq, const Strided& k, const Strided& v, void* q_out, const void* cosv,
                              const void* sinv, int table_rows, int T, cudaStream_t stream);

@@ -133,8 +133,10 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
     for (int i = 0; i < kQPieces; ++i) {
       const int p = start + int(t[i]);
       if (base + i * kAppendThreads >= pieces) break;
-      if (cosv != nullptr && int(t[i]) < count && p >= 0 && p < table_rows && p < c.blocks * BLK)
-        rotate8(lo[i], hi[i], cosv + (long long)p * D + rest[i] % VEC * 8, sinv + (long long)p * D + rest[i] % VEC * 8);
+      if (cosv != nullptr && int(t[i]) < count && p >= 0 && p < c.blocks * BLK) {
+        const long long at = (long long)min(p, table_rows - 1) * D + rest[i] % VEC * 8;
+        rotate8(lo[i], hi[i], cosv + at, sinv + at);
+      }
       T* dst = q_out + (((long long)b * Tn + t[i]) * Hq + rest[i] / VEC) * D + rest[i] % VEC * 8;
       *reinterpret_cast<uint4*>(dst) = lo[i].q;
       *reinterpret_cast<uint4*>(dst + D / 2) = hi[i].q;
@@ -186,8 +188,10 @@ kv_append_kernel(CacheView c, Strided q, int Hq, Strided k, Strided v, T* __rest
         khi[it].q = *reinterpret_cast<const uint4*>(ks + D / 2);
         vlo[it].q = *reinterpret_cast<const uint4*>(vs);
         vhi[it].q = *reinterpret_cast<const uint4*>(vs + D / 2);
-        if (cosv != nullptr && p < table_rows)
-          rotate8(klo[it], khi[it], cosv + (long long)p * D + vec * 8, sinv + (long long)p * D + vec * 8);
+        if (cosv != nullptr) {
+          const long long at = (long long)min(p, table_rows - 1) * D + vec * 8;
+          rotate8(klo[it], khi[it], cosv + at, sinv + at);
+        }
       } else if (closes && p < start) {
         klo[it].q = *reinterpret_cast<const uint4*>(tk + tok * D + vec * 8);
         khi[it].q = *reinterpret_cast<const uint4*>(tk + tok * D + D / 2 + vec * 8);

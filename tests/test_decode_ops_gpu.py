@@ -282,6 +282,47 @@ def test_two_streams_and_replays(ops):
     assert torch.equal(replayed.codes, plain.codes) and torch.equal(replayed.lengths, plain.lengths)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_replays_behind_the_rotary_tables_take_their_last_row(ops, dtype, dim):
+    """A graph that is replayed beyond the tables it was recorded with: the codes, the open block and the queries of the plain form."""
+
+    from mini_train_sys_b200.models.ops import get_ops_backend
+
+    table, steps = 70, 75
+    k, v, q = rows(2, 2, 3 * steps, dim, 21, dtype), rows(2, 2, 3 * steps, dim, 22, dtype), rows(2, 4, 3 * steps, dim, 23, dtype)
+    cos, sin = (t.to(DEV, dtype) for t in rope_tables(dim, table, 10000.0))
+    full = [torch.cat((t, t[-1:].expand(256 - table, -1))).cpu() for t in (cos, sin)]
+    cache = QuantizedKVCache(layers=1, batch=2, kv_heads=2, head_dim=dim, capacity=256, dtype=dtype, device=DEV)
+    plain = QuantizedKVCache(layers=1, batch=2, kv_heads=2, head_dim=dim, capacity=256, dtype=dtype, device="cpu")
+    static = [t[:, :, :3].clone() for t in (k, v, q)]
+
+    def step(backend, into, kt, vt, qt, c, s):
+        into.begin(padded=3)
+        out = backend.kv_append(into, 0, kt, vt, q=qt, cos=c, sin=s)
+        into.commit()
+        return out
+
+    step(ops, QuantizedKVCache(layers=1, batch=2, kv_heads=2, head_dim=dim, capacity=64, dtype=dtype, device=DEV), *static, cos, sin)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(ops, cache, *static, cos, sin)
+    cache.held = 0                                    # the capture has run nothing
+    for i in range(steps):
+        piece = [t[:, :, 3 * i:3 * i + 3] for t in (k, v, q)]
+        for dst, src in zip(static, piece):
+            dst.copy_(src)
+        cache.replayed(3)
+        graph.replay()
+        want = step(get_ops_backend("torch"), plain, *(t.cpu() for t in piece), *full)
+        # products of 16-bit factors are exact in fp32, so both forms round the same sum
+        assert torch.equal(out.cpu(), want), i
+    first = torch.zeros(2, dtype=torch.int32)
+    got, want = ops.kv_read(cache, 0, first.to(DEV), 3 * steps), get_ops_backend("torch").kv_read(plain, 0, first, 3 * steps)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------------------------------------
 # mixture of experts for a few tokens
 # ---------------------------------------------------------------------------------------------
