@@ -159,6 +159,13 @@ template <> struct Act<__half> {
   }
 };
 
+// The values of a pair that are infinite or NaN, as a mask: the exponent is all ones, and one more carries into the sign's place.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t kExponent = Act<T>::kHalf ? 0x7C007C00u : 0x7F807F80u, kOne = Act<T>::kHalf ? 0x04000400u : 0x00800080u;
+  return (((w & kExponent) + kOne) >> 15 & 0x00010001u) * 0xFFFFu;
+}
+
 // Running statistics and output of 8 * NQ query rows in one warp.  A lane holds the columns 2c and 2c + 1 of every tile of
 // eight rows (the statistics are the same in the eight lanes that share c) and the dims g and g + 8 of every 16.
 template <int D, int NQ>
@@ -595,6 +602,48 @@ cached_attention_kernel(const Params p) {
           }
           st.l[n][0] += sum[0];
           st.l[n][1] += sum[1];
+        }
+        // A token that some rows do not see has the probability 0 there, which times an infinity or a NaN is a NaN.  Where the half may
+        // hold such a token, values that are not finite are added to the rows that see them, and are zero in the product.
+        if (fresh > 1 && base + 32 > start + 1) {
+          uint8_t* mine = ring + stage * STAGE + VALUES + g * 64 + c * 16;
+          uint32_t found = 0;
+#pragma unroll 1
+          for (int d = 0; d < D; d += 8) {
+            uint32_t w[4];
+            read_words<4>(mine + d * 64, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) found |= not_finite<T>(w[i] & keep[i >> 1][i & 1]);
+          }
+          if (__any_sync(0xffffffffu, found != 0)) {
+#pragma unroll 1
+            for (int token = 0; token < min(valid, 32); ++token) {
+              const uint8_t* row = here + VALUES + g * 64 + tail_slot(0, 0, token) * 2;
+#pragma unroll
+              for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                  const uint32_t bits = *reinterpret_cast<const uint16_t*>(row + (16 * d + 8 * v) * 64);
+                  const float value = Act<T>::lo(bits & not_finite<T>(bits));
+#pragma unroll
+                  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                      if (base + token <= limit[n][j]) st.o[n][d][j + 2 * v] += value;
+                }
+            }
+            __syncwarp();
+#pragma unroll 1
+            for (int d = 0; d < D; d += 8) {
+              uint32_t w[4];
+              read_words<4>(mine + d * 64, w);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] &= ~not_finite<T>(w[i]);
+              *reinterpret_cast<uint4*>(mine + d * 64) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            fence_proxy_async_smem();      // before the next copy into this stage
+            __syncwarp();
+          }
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {

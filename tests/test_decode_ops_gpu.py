@@ -206,6 +206,48 @@ def test_a_non_finite_token_stays_in_its_sequence_and_its_block(ops):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group,batch,capacity", [(32, 1, 1, 256), (64, 3, 2, 256), (64, 24, 3, 8192), (128, 1, 2, 256), (128, 8, 40, 4096)])
+@pytest.mark.parametrize("start", [0, 70, 100])
+def test_a_later_token_that_is_not_finite_reaches_no_earlier_row_of_an_open_block(ops, dtype, dim, group, batch, capacity, start):
+    """Values and keys of a step whose block stays open: rows before a NaN or an infinity are those of a clean step, rows behind it hold
+    it.  Both ways of sharing the work, and both halves of the block."""
+
+    new = 20
+    k, v = rows(batch, 2, start + new, dim, 31, dtype), rows(batch, 2, start + new, dim, 32, dtype, spread=False)
+    q = rows(batch, 2 * group, new, dim, 33, dtype, spread=False)
+    inf = float("inf")
+    for name, where, token, value in (("v", 1, 5, inf), ("v", 1, 17, -inf), ("v", 0, 1, float("nan")), ("k", 1, 8, float("nan")), ("k", 0, 19, inf)):
+        outs = []
+        for broken in (False, True):
+            fresh = {n: t[:, :, start:].clone() for n, t in (("k", k), ("v", v))}
+            if broken:
+                fresh[name][0, where, token, 3] = value
+            cache = QuantizedKVCache(layers=1, batch=batch, kv_heads=2, head_dim=dim, capacity=capacity, dtype=dtype, device=DEV)
+            if start:
+                fill(ops, cache, 0, k, v, [start] * batch)
+            cache.begin(padded=new)
+            ops.kv_append(cache, 0, fresh["k"], fresh["v"])
+            outs.append(ops.cached_attention(q, cache, 0))
+        clean, got = outs
+        hit = slice(where * group, (where + 1) * group)
+        others = [h for h in range(2 * group) if not where * group <= h < (where + 1) * group]
+        assert torch.isfinite(clean).all() and torch.equal(got[1:], clean[1:]) and torch.equal(got[0, others], clean[0, others])
+        # sums in another order: the bound of the other tests, on values of this size
+        early = (got[0, hit, :token].double() - clean[0, hit, :token].double()).abs()
+        assert (early <= torch.finfo(dtype).eps * clean[0, hit, :token].double().abs() + 2.5 * 2 ** -11 * v.abs().max().double()).all()
+        late = got[0, hit, token:]
+        if name == "k":
+            # a score of +inf is the row's maximum and makes a NaN of it, one of -inf is a probability of 0
+            alone = value != value or q[0, hit, token:, 3].float() > 0
+            assert (late.isnan().all(-1) == alone).all() and torch.isfinite(late[~late.isnan().all(-1)]).all()
+        else:
+            others = [d for d in range(dim) if d != 3]
+            want = clean[0, hit, token:, others].double()
+            assert (late[..., others].double() - want).abs().max() <= torch.finfo(dtype).eps * want.abs().max() + 2.5 * 2 ** -11 * v.abs().max().double()
+            assert late[..., 3].isnan().all() if value != value else (late[..., 3] == value).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_large_queries_and_repeated_steps_and_copies(ops, dtype):
     """Logits of some hundreds; a step that is appended twice; a copy that goes on by itself."""
 
