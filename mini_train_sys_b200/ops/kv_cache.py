@@ -280,6 +280,13 @@ def attention_plain(q: torch.Tensor, cache: QuantizedKVCache, layer: int) -> tor
     t = torch.arange(new, device=q.device)
     seen = torch.arange(n, device=q.device) <= (start[:, None] + t)[..., None]
     scores = scores.masked_fill(~seen[:, None, None], float("-inf"))
-    out = torch.einsum("bhgts,bhsd->bhgtd", torch.softmax(scores, -1), values).reshape(b, hq, new, d)
+    finite = torch.isfinite(values)
+    out = torch.einsum("bhgts,bhsd->bhgtd", torch.softmax(scores, -1), torch.where(finite, values, torch.zeros_like(values)))
+    if not bool(finite.all()):
+        # a masked probability of 0 times an infinity or a NaN would be a NaN: what is not finite is added to the rows that see it
+        rest = torch.where(finite, torch.zeros_like(values), values)
+        for at in (~finite).any(-1).any(1).any(0).nonzero().flatten().tolist():
+            out += torch.where(seen[:, None, None, :, at, None], rest[:, :, None, None, at], torch.zeros_like(out))
+    out = out.reshape(b, hq, new, d)
     live = (t < count[:, None])[:, None, :, None]
     return torch.where(live, out, torch.zeros_like(out)).to(q.dtype)

@@ -70,6 +70,42 @@ def test_ragged_steps_padding_and_empty_rows(ops):
     assert cache.lengths.tolist() == counts and cache.held == 70
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("start", [0, 50, 100])
+def test_a_later_token_that_is_not_finite_reaches_no_earlier_row(ops, dtype, start):
+    """Rows before a NaN or an infinity are those of a clean step, up to the block that a finished one shares a scale in."""
+
+    new = 20
+    k, v = rows(2, 2, start + new, 32, 1, dtype), rows(2, 2, start + new, 32, 2, dtype)
+    q = rows(2, 4, new, 32, 3, dtype)
+    inf = float("inf")
+    for name, token, value in (("v", 16, inf), ("v", 16, float("nan")), ("v", 17, -inf), ("k", 18, float("nan"))):
+        outs = []
+        for broken in (False, True):
+            fresh = {n: t[:, :, start:].clone() for n, t in (("k", k), ("v", v))}
+            if broken:
+                fresh[name][0, 1, token, 3] = value
+            cache = make_cache(batch=2, dtype=dtype)
+            if start:
+                cache.begin(padded=start)
+                ops.kv_append(cache, 0, k[:, :, :start], v[:, :, :start])
+                cache.commit()
+            cache.begin(padded=new)
+            ops.kv_append(cache, 0, fresh["k"], fresh["v"])
+            outs.append(ops.cached_attention(q, cache, 0))
+        clean, got = outs
+        assert torch.isfinite(clean).all() and torch.equal(got[1], clean[1]) and torch.equal(got[0, :2], clean[0, :2])
+        closed = (start + new) // 64 * 64 - start                 # rows of the step in finished blocks
+        first = token if token >= closed else 0                   # rows from here on may see it
+        torch.testing.assert_close(got[0, 2:, :first], clean[0, 2:, :first], rtol=torch.finfo(dtype).eps, atol=1e-6)
+        late = got[0, 2:, token:]
+        if name == "v" and token >= closed:
+            assert late[..., 3].isnan().all() if value != value else (late[..., 3] == value).all()
+            torch.testing.assert_close(late[..., 4:], clean[0, 2:, token:, 4:], rtol=torch.finfo(dtype).eps, atol=1e-6)
+        else:
+            assert late.isnan().any(-1).all()
+
+
 def test_codes_are_those_of_exact_arithmetic():
     # halves: 127 x / a = n + 1/2 for x = a / 2 (63.5 -> 64, half to even), and no value between two halves is moved
     x = torch.zeros(1, 64, 32)
