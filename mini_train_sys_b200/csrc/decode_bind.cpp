@@ -133,17 +133,24 @@ struct KvLayer {
   static mts::Strided rows_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 };
 
+// What the kernels cover of a layer with experts of width I, its weights aside.
+bool moe_tokens_fits(const Tensor& x, const Tensor& router, int64_t I, int64_t top_k) {
+  if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() != 2 || router.dim() != 2) return false;
+  const int64_t T = x.size(0), H = x.size(1), E = router.size(0);
+  if (T > mts::kMoeTokensMax || H <= 0 || H % 8 != 0 || H > (1 << 20) || x.stride(1) != 1 || !aligned16(x) || (T > 1 && x.stride(0) % 8 != 0)) return false;
+  if (E < 1 || E > 64 || top_k < 1 || top_k > 8 || top_k > E || I <= 0 || I % 8 != 0 || I > (1 << 20)) return false;
+  return router.size(1) == H && (router.scalar_type() == at::kFloat || router.scalar_type() == at::kBFloat16) && router.device() == x.device() &&
+         router.is_contiguous() && aligned16(router);
+}
+
 // None for inputs that the kernels do not cover.
 py::object moe_tokens(const Tensor& x, const Tensor& router, const Tensor& gate_up, const Tensor& down, int64_t top_k, bool normalize,
                       const Tensor& status) {
-  if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() != 2 || router.dim() != 2 || gate_up.dim() != 3 || down.dim() != 3) return py::none();
+  if (gate_up.dim() != 3 || down.dim() != 3 || !moe_tokens_fits(x, router, down.size(2), top_k)) return py::none();
   const int64_t T = x.size(0), H = x.size(1), E = router.size(0), I = down.size(2);
-  if (T > mts::kMoeTokensMax || H <= 0 || H % 8 != 0 || H > (1 << 20) || x.stride(1) != 1 || !aligned16(x) || (T > 1 && x.stride(0) % 8 != 0)) return py::none();
-  if (E < 1 || E > 64 || top_k < 1 || top_k > 8 || top_k > E || I <= 0 || I % 8 != 0 || I > (1 << 20)) return py::none();
-  if (router.size(1) != H || (router.scalar_type() != at::kFloat && router.scalar_type() != at::kBFloat16)) return py::none();
   if (gate_up.size(0) != E || gate_up.size(1) != 2 * I || gate_up.size(2) != H || down.size(0) != E || down.size(1) != H) return py::none();
   if (gate_up.scalar_type() != at::kBFloat16 || down.scalar_type() != at::kBFloat16) return py::none();
-  for (const Tensor* w : {&router, &gate_up, &down})
+  for (const Tensor* w : {&gate_up, &down})
     if (w->device() != x.device() || !w->is_contiguous() || !aligned16(*w)) return py::none();
   if (at::GradMode::is_enabled() && (x.requires_grad() || router.requires_grad() || gate_up.requires_grad() || down.requires_grad())) return py::none();
   c10::cuda::CUDAGuard guard(x.device());
@@ -173,4 +180,5 @@ void bind_decode(pybind11::module_& m) {
       .def("read", &KvLayer::read)
       .def("attend", &KvLayer::attend);
   m.def("moe_tokens", &moe_tokens);
+  m.def("moe_tokens_fits", &moe_tokens_fits);
 }

@@ -966,7 +966,8 @@ class NativeOpsBackend(TorchOpsBackend):
         y = ext().moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k, normalize, status) if status is not None else None
         if y is None:
             check_moe_tokens(x, router_weight, gate_up_proj, down_proj, top_k)
-            if status is not None and x.dtype == torch.bfloat16 and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in (gate_up_proj, down_proj)):
+            if status is not None and ext().moe_tokens_fits(x, router_weight, down_proj.shape[2], top_k) \
+                    and all(w.device == x.device and w.dtype in (torch.float32, torch.bfloat16) for w in (gate_up_proj, down_proj)):
                 # fp32 parameters: their bf16 copies, as in the other operators
                 y = ext().moe_tokens(x, router_weight.detach(), bf16_weight(gate_up_proj), bf16_weight(down_proj), top_k, normalize, status)
         if y is not None:

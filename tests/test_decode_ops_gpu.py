@@ -428,6 +428,24 @@ def test_moe_tokens_crowded_ties_strides_and_weights(ops):
     assert ops.moe_tokens(x[:0], r, gu, dn, 2, normalize=True).shape == (0, 256)
 
 
+def test_moe_tokens_copies_no_weights_that_it_does_not_use(ops):
+    """fp32 weights and a call that the kernels do not cover: the plain form reads the weights as they are."""
+
+    from mini_train_sys_b200.ops.native_backend import kept_bf16
+
+    x, r, gu, dn = moe_inputs(65, 16, 256, 64, 6)
+    weights = [torch.nn.Parameter(t.float()) for t in (gu, dn)]
+    before = ops.dispatch["moe_tokens:fallback"]
+    with torch.no_grad():
+        for rows_, top_k in ((x, 2), (x[:8].float(), 2), (x[:8], 9)):
+            ops.moe_tokens(rows_, r, *weights, top_k, normalize=True)
+            assert all(kept_bf16(w) is None for w in weights)
+        assert ops.dispatch["moe_tokens:fallback"] == before + 3
+        ops.dispatch.subtract({"moe_tokens:fallback": 3})
+        assert torch.equal(ops.moe_tokens(x[:8], r, *weights, 2, normalize=True), ops.moe_tokens(x[:8], r, gu, dn, 2, normalize=True))
+    assert all(kept_bf16(w) is not None for w in weights)
+
+
 def test_moe_tokens_on_two_streams_and_replayed(ops):
     x, r, gu, dn = moe_inputs(12, 8, 768, 1024, 3)
     want = ops.moe_tokens(x, r, gu, dn, 2, normalize=True)
