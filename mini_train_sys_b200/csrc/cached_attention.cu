@@ -38,7 +38,8 @@ namespace cg = cooperative_groups;
 
 constexpr int BLK = kCacheBlock;
 constexpr int kWarps = 4;
-// Resident CTAs an SM: what fits in registers (four with eight query rows) and, at D = 128, in shared memory.
+// Resident CTAs an SM: what fits in registers (four with eight query rows) and, at D = 128, in shared memory as long as the counts of
+// units leave room (resident_ctas).
 __host__ __device__ constexpr int ctas_per_sm(int D, int nq) { return nq > 1 ? 2 : D == 128 ? 3 : 4; }
 constexpr int kBatchMax = 2048;          // sequences: their units are counted in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
@@ -106,9 +107,19 @@ __device__ __forceinline__ void count_units(const Params& p, int* prefix, int* s
 __host__ __device__ constexpr int pieces(int D) { return D < 128 ? 1 : 2; }
 __host__ __device__ constexpr int ring_stages(int D) { return D < 64 ? 2 : 1; }
 __host__ __device__ constexpr int stage_bytes(int D, int NQ) { return record_bytes(D) + 8 * NQ * D * 2; }
+__host__ __device__ constexpr int ring_bytes(int D, int NQ) { return kWarps * ring_stages(D) * stage_bytes(D, NQ); }
+__host__ __device__ constexpr int exchange_bytes(int D, int NQ) { return kWarps * D * (8 * NQ + 1) * 4; }
+__host__ __device__ constexpr int result_bytes(int D, int NQ) { return 8 * NQ * (D + 2) * 4; }
+// The rings, and where they were: the exchange of the warps' outputs with the CTA's result behind it.
 __host__ __device__ constexpr int shared_bytes(int D, int NQ) {
-  const int ring = kWarps * ring_stages(D) * stage_bytes(D, NQ), exchange = kWarps * D * (8 * NQ + 1) * 4;
-  return ring > exchange ? ring : exchange;
+  const int joined = exchange_bytes(D, NQ) + result_bytes(D, NQ);
+  return ring_bytes(D, NQ) > joined ? ring_bytes(D, NQ) : joined;
+}
+// Resident CTAs an SM with the counts of units of `counted` sequences behind that: an SM has 228 KB, 1 KB of it is taken for a CTA,
+// and statistics and barriers are below 512 bytes for every eight rows.
+__host__ inline int resident_ctas(int D, int nq, int counted) {
+  const int room = (228 << 10) / (shared_bytes(D, nq) + (counted > 0 ? (counted + 1) * 4 : 0) + 512 * nq + 1024);
+  return room < ctas_per_sm(D, nq) ? room : ctas_per_sm(D, nq);
 }
 
 // `bytes` (a multiple of 16, like both addresses) from global to shared memory; completion is counted on the barrier.
@@ -272,7 +283,7 @@ cached_attention_kernel(const Params p) {
   constexpr int STAGES = ring_stages(D);
   constexpr int STAGE = stage_bytes(D, NQ), KEYS = kCacheHead, VALUES = KEYS + BLK * D, QUERIES = VALUES + BLK * D;
   constexpr int KB = D / 4;              // bytes of a key that a lane owns
-  extern __shared__ __align__(16) uint8_t smem[];          // rings (afterwards the exchange of the outputs), prefix
+  extern __shared__ __align__(16) uint8_t smem[];          // rings (afterwards the exchange of the outputs and the result), prefix
   __shared__ float ml_sm[kWarps][ROWS][2];
   __shared__ int scratch[kWarps];
   constexpr int SPLIT = pieces(D), PIECE = BLK * D / SPLIT;
@@ -721,7 +732,7 @@ cached_attention_kernel(const Params p) {
   __syncthreads();
   const int live = span_of(p, cur.b).y * p.group, row0 = cur.tile * ROWS;
   const bool whole = c0 == item_begin && c1 == item_end;
-  float* result = reinterpret_cast<float*>(smem + shared_bytes(D, NQ));                  // [ROWS][D + 2] of this CTA, where the counts would be
+  float* result = reinterpret_cast<float*>(smem + exchange_bytes(D, NQ));                // [ROWS][D + 2] of this CTA
   for (int i = threadIdx.x; i < ROWS * D; i += kWarps * 32) {
     const int r = i / D, d = i % D, row = row0 + r;
     if (row >= live) break;
@@ -971,7 +982,7 @@ Plan plan_for(int B, int Hkv, int Hq, int T, int D, int blocks) {
   auto tiles = [&](int nq) { return (rows + 8 * nq - 1) / (8 * nq); };
   for (pl.nq = 1; pl.nq <= most; ++pl.nq) {
     pl.row_tiles = tiles(pl.nq);
-    const long long slots = (long long)device_sm_count() * ctas_per_sm(D, pl.nq), items = (long long)B * Hkv * pl.row_tiles;
+    const long long slots = (long long)device_sm_count() * resident_ctas(D, pl.nq, 0), items = (long long)B * Hkv * pl.row_tiles;
     pl.cluster = 1;
     while (pl.cluster < 8 && pl.cluster * kWarps < blocks) pl.cluster *= 2;
     while (pl.cluster > 1 && items * pl.cluster > slots) pl.cluster /= 2;
@@ -982,37 +993,44 @@ Plan plan_for(int B, int Hkv, int Hq, int T, int D, int blocks) {
   pl.nq = (rows + 7) / 8 < most ? (rows + 7) / 8 : most;
   pl.row_tiles = tiles(pl.nq);
   pl.cluster = 0;
-  const long long units = (long long)B * Hkv * pl.row_tiles * blocks, slots = (long long)device_sm_count() * ctas_per_sm(D, pl.nq);
+  const long long units = (long long)B * Hkv * pl.row_tiles * blocks, slots = (long long)device_sm_count() * resident_ctas(D, pl.nq, B);
   pl.ctas = int(units < slots ? units : slots);
   return pl;
 }
 
-template <typename K>
-cudaError_t allow_shared(K kernel, int bytes, std::atomic<bool> (&ready)[64]) {
+// Allows a kernel its dynamic shared memory, once a device.
+template <typename T, int D, int NQ, bool CLUSTER>
+cudaError_t allow_shared() {
+  static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (ready[dev]) return cudaSuccess;
-  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  err = cudaFuncSetAttribute(cached_attention_kernel<T, D, NQ, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             shared_bytes(D, NQ) + (CLUSTER ? 0 : (kBatchMax + 1) * 4));
   if (err == cudaSuccess) ready[dev] = true;
   return err;
+}
+
+// CTAs of a plan's kernel that an SM holds at once, by the runtime.
+template <typename T, int D, int NQ>
+cudaError_t measured_residency(const Plan& pl, int B, int* ctas) {
+  const cudaError_t err = pl.cluster > 0 ? allow_shared<T, D, NQ, true>() : allow_shared<T, D, NQ, false>();
+  if (err != cudaSuccess) return err;
+  const auto kernel = pl.cluster > 0 ? cached_attention_kernel<T, D, NQ, true> : cached_attention_kernel<T, D, NQ, false>;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(ctas, kernel, kWarps * 32, size_t(shared_bytes(D, NQ)) + (pl.cluster > 0 ? 0 : (B + 1) * 4));
 }
 
 template <typename T, int D, int NQ>
 cudaError_t launch_typed(const Params& p, int cluster, cudaStream_t stream) {
   const int bytes = shared_bytes(D, NQ);
-  if (cluster > 0) {
-    static std::atomic<bool> ready[64];
-    const size_t shared = size_t(bytes) + 8 * NQ * (D + 2) * 4;
-    const cudaError_t err = allow_shared(cached_attention_kernel<T, D, NQ, true>, int(shared), ready);
-    if (err != cudaSuccess) return err;
-    ++g_launch_count;
-    return launch_chained(cached_attention_kernel<T, D, NQ, true>, dim3(unsigned(p.ctas)), kWarps * 32, shared, cluster, stream, p);
-  }
-  static std::atomic<bool> ready[64];
-  cudaError_t err = allow_shared(cached_attention_kernel<T, D, NQ, false>, bytes + (kBatchMax + 1) * 4, ready);
+  cudaError_t err = cluster > 0 ? allow_shared<T, D, NQ, true>() : allow_shared<T, D, NQ, false>();
   if (err != cudaSuccess) return err;
+  if (cluster > 0) {
+    ++g_launch_count;
+    return launch_chained(cached_attention_kernel<T, D, NQ, true>, dim3(unsigned(p.ctas)), kWarps * 32, size_t(bytes), cluster, stream, p);
+  }
   const long long rows = (long long)p.B * p.Hkv * p.group * p.T;
   if (rows > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   ++g_launch_count;
@@ -1027,12 +1045,35 @@ cudaError_t launch_typed(const Params& p, int cluster, cudaStream_t stream) {
   return launch_chained(join_parts_kernel<T, D>, dim3(unsigned(rows)), kJoinThreads, size_t(p.B + 1 + 2 * (p.ctas + 2 * kWarps)) * 4, 0, stream, p, 8 * NQ);
 }
 
-template <typename T, int D>
-cudaError_t launch_dim(const Params& p, const Plan& pl, cudaStream_t stream) {
-  if (pl.nq == 1) return launch_typed<T, D, 1>(p, pl.cluster, stream);
-  if (pl.nq == 2) return launch_typed<T, D, 2>(p, pl.cluster, stream);
-  if constexpr (D != 128) return pl.nq == 3 ? launch_typed<T, D, 3>(p, pl.cluster, stream) : launch_typed<T, D, 4>(p, pl.cluster, stream);
-  return cudaErrorInvalidValue;
+struct Launch {
+  const Params& p;
+  int cluster;
+  cudaStream_t stream;
+  template <typename T, int D, int NQ> cudaError_t run() const { return launch_typed<T, D, NQ>(p, cluster, stream); }
+};
+struct Residency {
+  const Plan& plan;
+  int B, *ctas;
+  template <typename T, int D, int NQ> cudaError_t run() const { return measured_residency<T, D, NQ>(plan, B, ctas); }
+};
+// f.run of the kernel that serves a type, a head dimension and a row tile.
+template <typename F>
+cudaError_t for_kernel(bool fp16, int D, int nq, const F& f) {
+  auto rows = [&](auto t, auto d) -> cudaError_t {
+    constexpr int kD = decltype(d)::value;
+    using T = decltype(t);
+    if (nq == 1) return f.template run<T, kD, 1>();
+    if (nq == 2) return f.template run<T, kD, 2>();
+    if constexpr (kD != 128) return nq == 3 ? f.template run<T, kD, 3>() : f.template run<T, kD, 4>();
+    return cudaErrorInvalidValue;
+  };
+  auto dims = [&](auto t) -> cudaError_t {
+    if (D == 32) return rows(t, std::integral_constant<int, 32>());
+    if (D == 64) return rows(t, std::integral_constant<int, 64>());
+    if (D == 128) return rows(t, std::integral_constant<int, 128>());
+    return cudaErrorInvalidValue;
+  };
+  return fp16 ? dims(__half()) : dims(__nv_bfloat16());
 }
 
 }  // namespace
@@ -1058,10 +1099,15 @@ cudaError_t launch_cached_attention(const CachedAttentionArgs& a) {
   p.row_tiles = pl.row_tiles; p.ctas = pl.ctas;
   p.q = a.q.p; p.sb = a.q.sb; p.sh = a.q.sh; p.st = a.q.st;
   p.o = a.o; p.part = a.workspace; p.sm_log2 = a.scale * kLog2e; p.status = a.status;
-  if (c.D == 32) return c.fp16 ? launch_dim<__half, 32>(p, pl, a.stream) : launch_dim<__nv_bfloat16, 32>(p, pl, a.stream);
-  if (c.D == 64) return c.fp16 ? launch_dim<__half, 64>(p, pl, a.stream) : launch_dim<__nv_bfloat16, 64>(p, pl, a.stream);
-  if (c.D == 128) return c.fp16 ? launch_dim<__half, 128>(p, pl, a.stream) : launch_dim<__nv_bfloat16, 128>(p, pl, a.stream);
-  return cudaErrorInvalidValue;
+  return for_kernel(c.fp16, c.D, pl.nq, Launch{p, pl.cluster, a.stream});
+}
+
+cudaError_t cached_attention_plan(int B, int Hkv, int Hq, int T, int D, int blocks, bool fp16, CachedAttentionPlan* out) {
+  const Plan pl = plan_for(B, Hkv, Hq, T, D, blocks);
+  out->rows = 8 * pl.nq;
+  out->ctas = pl.ctas;
+  out->cluster = pl.cluster;
+  return for_kernel(fp16, D, pl.nq, Residency{pl, B, &out->resident});
 }
 
 }  // namespace mts

@@ -60,6 +60,11 @@ struct CachedAttentionArgs {
 bool cached_attention_fits(int B, int Hkv, int Hq, int T, int D, int blocks);
 size_t cached_attention_workspace_floats(int B, int Hkv, int Hq, int T, int D, int blocks);
 cudaError_t launch_cached_attention(const CachedAttentionArgs& a);
+// How such a call is launched: rows of a tile, CTAs, CTAs of a cluster (0: one list of units for all), and the CTAs that an SM holds at once.
+struct CachedAttentionPlan {
+  int rows, ctas, cluster, resident;
+};
+cudaError_t cached_attention_plan(int B, int Hkv, int Hq, int T, int D, int blocks, bool fp16, CachedAttentionPlan* plan);
 
 // ---- mixture of experts for a few tokens ----------------------------------------------------------------------------
 constexpr int kMoeTokensMax = 64;

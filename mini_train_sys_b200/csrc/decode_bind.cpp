@@ -133,6 +133,17 @@ struct KvLayer {
   static mts::Strided rows_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 };
 
+// (rows of a tile, CTAs, CTAs of a cluster or 0, CTAs that an SM holds at once) of a call with these extents on the current device
+py::tuple cached_attention_plan(int64_t B, int64_t Hkv, int64_t Hq, int64_t T, int64_t D, int64_t blocks, bool fp16) {
+  TORCH_CHECK(B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && T > 0 && blocks > 0 && (D == 32 || D == 64 || D == 128), "unsupported extents");
+  TORCH_CHECK(B <= 65535 && Hkv <= 65535 && blocks <= (1 << 24) && T <= (1 << 24) && Hq / Hkv * T <= (1 << 24) &&
+                  mts::cached_attention_fits(int(B), int(Hkv), int(Hq), int(T), int(D), int(blocks)), "unsupported extents");
+  mts::CachedAttentionPlan plan{};
+  const cudaError_t e = mts::cached_attention_plan(int(B), int(Hkv), int(Hq), int(T), int(D), int(blocks), fp16, &plan);
+  TORCH_CHECK(e == cudaSuccess, "cached_attention_plan failed: ", cudaGetErrorString(e));
+  return py::make_tuple(plan.rows, plan.ctas, plan.cluster, plan.resident);
+}
+
 // What the kernels cover of a layer with experts of width I, its weights aside.
 bool moe_tokens_fits(const Tensor& x, const Tensor& router, int64_t I, int64_t top_k) {
   if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() != 2 || router.dim() != 2) return false;
@@ -179,6 +190,7 @@ void bind_decode(pybind11::module_& m) {
       .def("append", &KvLayer::append)
       .def("read", &KvLayer::read)
       .def("attend", &KvLayer::attend);
+  m.def("cached_attention_plan", &cached_attention_plan);
   m.def("moe_tokens", &moe_tokens);
   m.def("moe_tokens_fits", &moe_tokens_fits);
 }

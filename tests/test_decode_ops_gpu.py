@@ -205,6 +205,36 @@ def test_a_non_finite_token_stays_in_its_sequence_and_its_block(ops):
     assert outs[1][1, :, 70:].isnan().all()
 
 
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_the_plan_of_an_attention_fits_on_the_machine(ops, dim, fp16):
+    """As many CTAs as are resident at once: single items and lists of units, small tiles and large, few sequences and thousands."""
+
+    from mini_train_sys_b200.ops.native_backend import ext
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    kinds = set()
+    for batch in (1, 4, 17, 40, 64, 600, 660, 2048):
+        for group, new in ((1, 1), (8, 1), (1, 17), (3, 9), (4, 32)):
+            for blocks in (1, 8, 32, 600):
+                rows_, ctas, cluster, resident = ext().cached_attention_plan(batch, 4, 4 * group, new, dim, blocks, fp16)
+                assert 0 < ctas <= sms * resident, (batch, group, new, blocks)
+                assert cluster == 0 or ctas % cluster == 0
+                kinds.add((cluster > 0, rows_))
+    assert {(True, 8), (False, 8), (False, 16 if dim == 128 else 32)} <= kinds
+
+
+def test_cached_attention_of_more_sequences_than_leave_room_for_three_ctas(ops):
+    lengths = [70 + 40 * (b % 5 == 0) + b % 7 for b in range(700)]
+    k, v = rows(700, 1, 120, 128, 34), rows(700, 1, 120, 128, 35, spread=False)
+    q = rows(700, 2, 1, 128, 36, spread=False)
+    cache = QuantizedKVCache(layers=1, batch=700, kv_heads=1, head_dim=128, capacity=1024, device=DEV)
+    fill(ops, cache, 0, k, v, lengths)
+    cache.begin()
+    ops.kv_append(cache, 0, *[torch.stack([x[b, :, n:n + 1] for b, n in enumerate(lengths)]) for x in (k, v)])
+    assert_attention(ops.cached_attention(q, cache, 0), q, k, v, lengths, [1] * 700)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim,group,batch,capacity", [(32, 1, 1, 256), (64, 3, 2, 256), (64, 24, 3, 8192), (128, 1, 2, 256), (128, 8, 40, 4096)])
 @pytest.mark.parametrize("start", [0, 70, 100])
