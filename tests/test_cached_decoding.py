@@ -277,6 +277,21 @@ def test_a_session_is_reset_before_and_after_its_capture():
 
 
 @pytest.mark.gpu
+def test_a_step_in_training_mode_is_refused_before_and_after_the_capture():
+    model = make_model("moe", ops="native", device="cuda", dtype=torch.bfloat16, hidden=256, seq_len=256)
+    ids = torch.randint(0, 97, (2, 20), device="cuda")
+    eager, replayed = (DecodeSession(model, 2, graph=g) for g in (False, True))
+    for s in (eager, replayed):
+        s.prompt(ids[:, :10])
+    for i in range(10, 20):
+        model.train()
+        with pytest.raises(RuntimeError, match="eval"):
+            replayed.step(ids[:, i:i + 1])
+        model.eval()
+        assert torch.equal(eager.step(ids[:, i:i + 1]), replayed.step(ids[:, i:i + 1])), i
+
+
+@pytest.mark.gpu
 def test_a_graph_recorded_on_an_empty_cache_is_right_at_every_length():
     model = make_model("dense", ops="native", device="cuda", dtype=torch.bfloat16, hidden=256, seq_len=256)
     ids = torch.randint(0, 97, (2, 80), device="cuda")

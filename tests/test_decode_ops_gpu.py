@@ -538,6 +538,32 @@ def test_operators_that_read_what_the_one_before_wrote(ops, tokens, experts, hid
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_native_and_plain_forms_share_a_cache(ops):
+    """Calls whose strides send one operator of a step to the plain form, on a cache that the kernels fill and read too."""
+
+    n, steps = 60, [1, 3, 5, 70, 2]
+    total = n + sum(steps)
+    k, v, q = rows(2, 2, total, 64, 41), rows(2, 2, total, 64, 42, spread=False), rows(2, 4, total, 64, 43, spread=False)
+    odd = [torch.empty(2, t.shape[1], total, 66, device=DEV, dtype=t.dtype) for t in (k, v, q)]      # rows on no 16 bytes
+    for dst, src in zip(odd, (k, v, q)):
+        dst[..., :64] = src
+    cache = QuantizedKVCache(layers=1, batch=2, kv_heads=2, head_dim=64, capacity=256, device=DEV)
+    fill(ops, cache, 0, k, v, [n, n])
+    before, at = dict(ops.dispatch), n
+    for i, c in enumerate(steps):
+        sources = odd if i % 2 else (k, v, q)
+        ks, vs = (t[:, :, at:at + c, :64] for t in sources[:2])
+        qs = (q if i % 2 else odd[2])[:, :, at:at + c, :64]
+        cache.begin(padded=c)
+        ops.kv_append(cache, 0, ks, vs)
+        assert_attention(ops.cached_attention(qs, cache, 0), q[:, :, at:at + c], k, v, [at, at], [c, c])
+        cache.commit()
+        at += c
+    for op, plain in (("kv_append", 2), ("cached_attention", 3)):
+        assert ops.dispatch[f"{op}:fallback"] == before.get(f"{op}:fallback", 0) + plain
+        ops.dispatch.subtract({f"{op}:fallback": plain})
+
+
 def test_what_the_kernels_do_not_cover_takes_the_plain_path(ops):
     before = dict(ops.dispatch)
     cache = QuantizedKVCache(layers=1, batch=1, kv_heads=2, head_dim=48, capacity=128, device=DEV)
