@@ -12,14 +12,14 @@
 // single long one, keep every SM busy, and a warp streams across the ends of sequences.  A second kernel joins the parts of
 // the (sequence, head, row tile) items that were cut.
 // What bounds it: reading the codes, 2 D bytes per token and K/V head.  Measured on the GPU (replayed graph, caches flushed), one new
-// token: 64 ragged sequences of up to 2,048 tokens, 12 heads of 64, 24.7 us (101 MB, 4.1 TB/s); one of 131,071 tokens, 16 heads
-// on 4 of 64, 20.9 us (67 MB, 3.2 TB/s); eight ragged ones of up to 32,768, 32 heads on 8 of 128, 54.3 us (269 MB, 4.9 TB/s).  The first
-// two are short streams behind a launch and the counting of units, and before the join.
+// token: 64 ragged sequences of up to 2,048 tokens, 12 heads of 64, 24.7 us (95 MB, 3.8 TB/s); one of 131,071 tokens, 16 heads
+// on 4 of 64, 21.1 us (67 MB, 3.2 TB/s); eight ragged ones of up to 32,768 (146,699 tokens in all), 32 heads on 8 of 128, 56.4 us (301 MB,
+// 5.3 TB/s).  The first two are short streams behind a launch and the counting of units, and before the join.
 //
-// Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2), so bf16
-// queries keep their eight bits in fp16.  Probabilities are rounded to fp16 (2^-11 of each, at a scale of 2^14 so that the
-// smallest kept one is 2^-38 of the largest); the sum of probabilities, the maximum and the output accumulators are fp32.  In
-// the unfinished block, whose values are bf16, a probability is the sum of two bf16 values.
+// Rounding: codes are exact in fp16.  A query row is scaled by the power of two that brings its largest value to [1, 2): bf16 queries
+// keep their eight bits in fp16 down to 2^-17 of that value, and lose up to 2^-25 of it below.  Probabilities are rounded to fp16
+// (2^-11 of each, at a scale of 2^14 so that the smallest kept one is 2^-38 of the largest); the sum of probabilities, the maximum and
+// the output accumulators are fp32.  In the unfinished block, whose values are bf16, a probability is the sum of two bf16 values.
 #include "decode.cuh"
 #include "launch.cuh"
 #include "ops.cuh"
@@ -564,7 +564,7 @@ cached_attention_kernel(const Params p) {
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
               const uint32_t f[4] = {a[0][2 * i], a[1][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]};
-              Act<T>::mma(s[m][n], f, Act<T>::from_half2(qf[n][i][0]), Act<T>::from_half2(qf[n][i][1]));   // eight bits: exact
+              Act<T>::mma(s[m][n], f, Act<T>::from_half2(qf[n][i][0]), Act<T>::from_half2(qf[n][i][1]));   // eight bits at most: exact
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -970,9 +970,9 @@ struct Plan {
   int nq, row_tiles, ctas, cluster;      // cluster: 0 for the list of units
 };
 
-// Where a cluster of up to eight CTAs has at most two blocks a warp and all clusters fit on the machine, an item is the work of one
+// Where a cluster of up to eight CTAs has at most two blocks a warp and there is room for all CTAs at once, an item is the work of one
 // cluster, which joins its parts through distributed shared memory: one launch, no counting of units.  Such problems are bound by
-// latency, so the smallest row tile that allows it is taken (17 rows over 2,000 tokens in tiles of 8: 12.4 us, in one of 24: 12.8).
+// latency, so the smallest row tile that allows it is taken (17 rows over 2,000 tokens in tiles of 8: 0.4 us of 12.8 less than in one of 24).
 // Otherwise rows are taken in tiles of up to 32 (16 at D = 128, where the accumulators of 32 would not fit in registers), so that the
 // cache is read as few times as possible, by as many CTAs as are resident at once, or as there can be units for.
 // The capacity decides, not the lengths, which only the device knows.

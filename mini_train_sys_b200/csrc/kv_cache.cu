@@ -5,8 +5,8 @@
 // What bounds them: appending reads the new tokens once and writes their codes, 3 bytes a value (and q, 4 bytes a value); reading
 // back reads a byte a value and writes four.  So they are bound by memory for a prompt and by their launch for one token.
 // Measured on the GPU (replayed graph, caches flushed), an append and a read-back of 12 heads of 64: one sequence of 448 tokens,
-// one new, 5.2 us; 64 ragged sequences of up to 512 tokens, one new, 18.2 us (51 MB, 2.8 TB/s); 16 ragged prompts of up to
-// 2,048 tokens 78.2 us (338 MB, 4.3 TB/s), of which the append, whose conversions keep the issue slots busy, takes half.
+// one new, 5.2 us; 64 ragged sequences of up to 512 tokens, one new, 17.7 us (51 MB, 2.9 TB/s); 16 ragged prompts of up to
+// 2,048 tokens 75.8 us (338 MB, 4.5 TB/s), of which the append, whose conversions keep the issue slots busy, takes half.
 #include "decode.cuh"
 #include "launch.cuh"
 #include "ops.cuh"
@@ -48,11 +48,13 @@ __device__ __forceinline__ void rotate8(Vec8T<T>& lo, Vec8T<T>& hi, const T* c, 
 }
 
 // Codes of eight values of a block whose largest magnitude is amax: 127 x / amax to the nearest integer, a half to the even one.
-// With whole mantissas, x = X 2^i and amax = A 2^j, a half is 254 X 2^(i-j) = A (2n + 1).  127 is prime, so it divides 2n + 1 (then n
-// is 63: x is half of amax, not a rare value) or A.  Where it does not divide A, everything else is at least 1 / (2 A) >= 2^-12 from a
-// half, and a product with 127 / amax, made two units in the last place too large, is right: it is off by 4e-5 at most, and takes
-// half of amax to just above 63.5, hence to 64, the even one.  Adding 1.5 * 2^23 leaves the integer in the low bits of the sum.
-// Blocks with other A (and with a subnormal or huge amax) take correctly rounded quotients, scaled by a power of two.
+// With whole mantissas, and in units of amax's last place, amax = A and x = X 2^-d; a half is 254 X = A 2^d (2n + 1).  127 is prime, so
+// it divides 2n + 1 (then n is 63: x is half of amax, not a rare value) or A.  Where it does not divide A, the difference of the two sides
+// is a whole number, an even one for d > 0, so everything else is at least 1 / (2 A) from a half for d = 0 and 2^-d / A for d > 0: more than
+// 2^-12 and 2^-11 2^-d in fp16, and than these in bf16.  A product with 127 / amax, rounded and made two units in the last place too large,
+// is off by at most 2.5 x 2^-23 of itself: 127 x 2.5 x 2^-23 = 3.8e-5 for d = 0 and, since X < 2 A, 7.6e-5 2^-d above, less than either
+// distance.  It takes half of amax to just above 63.5, hence to 64, the even one.  Adding 1.5 * 2^23 leaves the integer in the low bits of the
+// sum.  Blocks with other A (and with a subnormal or huge amax) take correctly rounded quotients, scaled by a power of two.
 struct Quantizer {
   float amax, inv;
   bool quick;

@@ -1,6 +1,7 @@
-// Warp-level matrix products and fragment helpers shared by the decoding kernels.  These kernels are bound by reading
-// 8-bit keys or expert weights once; eight query rows or tokens ride on every weight, far below what one 128-row tcgen05 tile
-// would need to be worth its shared-memory staging, so fragments are loaded straight from global memory into registers.
+// Warp-level matrix products and fragment helpers shared by the decoding kernels.  These kernels are bound by reading 8-bit keys and values
+// or expert weights, which bulk copies bring to a ring of each warp in shared memory.  From there a lane takes its fragments to registers,
+// where codes become fp16, and eight query rows or tokens ride on every weight: the tensor pipe is 9 to 18 % busy.  A tcgen05 tile would need
+// the converted operand back in shared memory and 128 rows of it before the first product.
 //
 // m16n8k16, lane = 4 g + c:  A: a0 (row g, k 2c..), a1 (row g + 8, k 2c..), a2 (row g, k 2c + 8..), a3 (row g + 8, k 2c + 8..)
 //                            B: b0 (k 2c.., column g), b1 (k 2c + 8.., column g);  C: c0 c1 (row g, columns 2c 2c+1), c2 c3 (row g + 8)

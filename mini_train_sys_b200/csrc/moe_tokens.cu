@@ -4,9 +4,10 @@
 //   y = sum_k w_k Wd[e_k] (silu(Wg[e_k] x) * (Wu[e_k] x))
 //
 // What bounds it: reading the weights of every expert that has a token, 6 H I bytes each, once.  Weight rows are the row operand of
-// m16n8k16 and the tokens of their expert the columns (8 at a time), so one pass over the weights serves up to 64 tokens.  Every warp
-// streams its own weight tiles through a ring in shared memory, 8 KB a TMA copy and 16 or 24 KB in flight a warp, across the ends of
-// items: 128 to 192 KB in flight an SM, and no barrier between warps inside a stream.
+// m16n8k16 and the tokens of their expert the columns (8 at a time), so one pass over an expert's weights serves up to 32 of its
+// tokens, and an expert with more is streamed again for every 32.  Every warp streams its own weight tiles
+// through a ring in shared memory, 8 KB a TMA copy and 16 or 24 KB in flight a warp, across the ends of items: 128 to 192 KB in
+// flight an SM, and no barrier between warps inside a stream.
 //   0  Routing reads x and the router's weight.  Up to 48 KB of them every CTA of the first kernel reads for itself (a launch costs
 //      more); above that one cluster of eight CTAs routes in a kernel of its own.
 //   1  A warp takes (entry, 8 columns of the hidden layer) items, an entry being an expert and its tokens: 8 gate rows and 8 up rows
@@ -15,9 +16,10 @@
 //   2  The (32 output rows, expert, 128 columns) units of the down projections are one list, cut into equal parts for the CTAs; what
 //      a CTA has of a row tile is added in shared memory, and where a tile was cut its last CTA adds the parts, in order.
 //
-// Measured on the GPU (replayed graph, caches flushed): one token, 2 of 8 experts of 768 x 1,024, 12.4 us (9.4 MB of weights: two launches'
-// latency); 64 tokens of the same 30.5 us (38 MB); 17 tokens, 8 of 64 experts of 2,048 x 1,024, 134 us (58 of them asked for, 0.72 GB,
-// 5.4 TB/s, the routing kernel's 11 us included); 8 tokens, 2 of 8 experts of 4,096 x 14,336, 383 us (2.5 GB, 6.6 TB/s).
+// Measured on the GPU (replayed graph, caches flushed): one token, 2 of 8 experts of 768 x 1,024, 12.1 us (9.4 MB of weights: two launches'
+// latency); 64 tokens of the same 30.5 us (38 MB); 17 tokens, 8 of 64 experts of 2,048 x 1,024, 133 us (58 of them asked for, 0.73 GB,
+// 5.5 TB/s, the routing kernel's 11 us included); 8 tokens, 2 of 8 experts of 4,096 x 14,336, 386 us where they ask for seven (2.47 GB,
+// 6.4 TB/s), some 440 where for all eight.
 //
 // Rounding: logits, softmax, sums and the hidden values are fp32 (the router's fp32 weight enters the tensor cores as the sum of three
 // bf16 values, 24 bits); a hidden value enters the second product as the sum of two (2^-16), so y is rounded to bf16 once.
@@ -941,10 +943,14 @@ bool encode_weights(CUtensorMap* map, const void* base, long long cols, long lon
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Bytes of x and the router's weight up to which every CTA of the first kernel routes by itself.
+// Bytes of x and the router's weight up to which every CTA of the first kernel routes by itself.  Measured in place against in a kernel of
+// its own: 8 experts of 768, one token (26 KB) 12.2 against 14.2 us for the layer, 8 (36 KB) 16.6 and 16.9, 12 (42 KB) 18.4 and 17.6, 16
+// (48 KB) 19.2 and 18.3, 24 (60 KB) 21.5 and 19.2; one token of 16 experts of 1,024 (66 KB) 13.5 and 14.4, of 32 (130 KB) 15.2 and 14.9.
 constexpr long long kRouteInPlace = 48 * 1024;
 constexpr long long kPrefetchBytes = 48ll << 20;
-// Units of a CTA up to which the second kernel gives a row tile to CTAs of its own.
+// Units of a CTA up to which the second kernel gives a row tile to CTAs of its own.  Measured with and without, the layer: 8 experts of 768 x
+// 1,024, one token (2.6 units) 12.0 and 14.9 us, 64 tokens (16 units) 30.4 and 33.4; of 768 x 2,048 (31) 41.9 and 43.8; of 2,048 x 2,048 (62)
+// 48.8 and 51.2; of 2,048 x 8,192 (221) 140.0 and 141.2: what it saves is a few microseconds at any size, a small part above the border.
 constexpr long long kSmallUnits = 32;
 
 size_t part_bytes(int T, int E) { return size_t(kWarps) * ((E + 15) / 16 * 16) * ((T + 7) / 8 * 8) * 4; }

@@ -147,7 +147,7 @@ class DenseFeedForward(nn.Module):
         return self(x, ops, residual=residual).hidden_states
 
 
-FEW_TOKENS = 64     # up to which the experts' weights are streamed once for all tokens instead of sorting rows for grouped GEMMs
+FEW_TOKENS = 64     # up to which an expert's weights are streamed once for every 32 of its tokens instead of sorting rows for grouped GEMMs
 
 
 class MoEFeedForward(nn.Module):

@@ -23,7 +23,6 @@ from collections import Counter
 import torch
 
 from mini_train_sys_b200.models.ops import RouterPostprocessOutput
-from mini_train_sys_b200.ops import kv_cache
 from mini_train_sys_b200.ops.build import load_extension
 from mini_train_sys_b200.ops.torch_backend import TorchOpsBackend, check_moe_tokens, check_router_args
 
