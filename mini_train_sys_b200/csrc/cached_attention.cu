@@ -110,13 +110,16 @@ __host__ __device__ constexpr int stage_bytes(int D, int NQ) { return record_byt
 __host__ __device__ constexpr int ring_bytes(int D, int NQ) { return kWarps * ring_stages(D) * stage_bytes(D, NQ); }
 __host__ __device__ constexpr int exchange_bytes(int D, int NQ) { return kWarps * D * (8 * NQ + 1) * 4; }
 __host__ __device__ constexpr int result_bytes(int D, int NQ) { return 8 * NQ * (D + 2) * 4; }
-// The rings, and where they were: the exchange of the warps' outputs with the CTA's result behind it.
+// The rings, and where they were: the exchange of the warps' outputs with the CTA's result behind it.  With the result behind the rings two CTAs
+// of 128 dims fit an SM instead of three: 24 sequences of 500 tokens, 32 heads on 8, took 22.2 us and now 14.1; 50 of 500, 8 heads, 24.6 and
+// 16.9; but 8 of 500, 32 heads, 13.7 and 15.8.
 __host__ __device__ constexpr int shared_bytes(int D, int NQ) {
   const int joined = exchange_bytes(D, NQ) + result_bytes(D, NQ);
   return ring_bytes(D, NQ) > joined ? ring_bytes(D, NQ) : joined;
 }
 // Resident CTAs an SM with the counts of units of `counted` sequences behind that: an SM has 228 KB, 1 KB of it is taken for a CTA,
-// and statistics and barriers are below 512 bytes for every eight rows.
+// and statistics and barriers are below 512 bytes for every eight rows.  (700 sequences of 1,000 tokens, 2 heads on 1 of 128: 60.7 us planned for
+// two CTAs an SM, 72.5 for three, of which two fit; 1,000 of 1,000, 8 heads on 4: 269 and 253.)
 __host__ inline int resident_ctas(int D, int nq, int counted) {
   const int room = (228 << 10) / (shared_bytes(D, nq) + (counted > 0 ? (counted + 1) * 4 : 0) + 512 * nq + 1024);
   return room < ctas_per_sm(D, nq) ? room : ctas_per_sm(D, nq);
